@@ -401,6 +401,212 @@ typedef struct mrtdf_bundle_paths {
  * MRTDF_PATH_MAX - 1 bytes is MRTDF_ERR_RANGE. No GPU is needed. */
 int mrtdf_resolve_inference_bundle(const char* cache_root, const char* tag, mrtdf_bundle_paths* out);
 
+/* ---- operators ---------------------------------------------------------------
+ * Operators of speculative and long-running decoding, on device buffers that
+ * the caller owns. No counterpart in the reference, whose speculative path
+ * (depthformer/decode.cpp:150-237) drafts one chain and re-attends with the
+ * single-chain kernels. Each call checks its arguments on the host, queues its
+ * kernels on `stream` (a cudaStream_t, NULL = the legacy default stream) of
+ * `device` and returns without waiting. It allocates nothing, keeps nothing
+ * between calls and may be captured into a CUDA graph; calls on different
+ * streams or from different threads may overlap as long as no buffer that one
+ * of them writes (workspaces included) is used by another. The caller's
+ * current device is as before when a call returns. Nothing on the host sees
+ * the values in device memory: what a kernel does with a length, a parent, a
+ * path or a position that makes no sense is said with each operator, and none
+ * of them makes it read or write outside the buffers.
+ *
+ * `struct_bytes` is sizeof() of the structure it is in; MRTDF_ERR_INVALID when
+ * it is not (a caller compiled against another header).
+ */
+
+/* Rows of head_dim contiguous elements of the cache's dtype: row (l, b, h, n)
+ * of layer, sequence, head and node starts at ptr + l * stride_l + b * stride_b
+ * + h * stride_h + n * stride_n elements. Every row starts on a 16-byte
+ * boundary; strides are not negative. (The rows of a fused q|k|v projection
+ * are three such views of one buffer.) */
+typedef struct mrtdf_rows {
+  void* ptr;
+  int64_t stride_l, stride_b, stride_h, stride_n;
+} mrtdf_rows;
+
+/* A KV cache: row (l, b, h, t) at l * stride_l + b * stride_b + h * stride_h +
+ * t * stride_t elements in k and in v, t < capacity; 16-byte boundaries and
+ * non-negative strides as above. At most 1024 sequences, layers and kv heads
+ * and 2^24 rows (MRTDF_ERR_RANGE). lens[b] rows of sequence b are in use in
+ * every layer and head; a sequence whose length is outside [0, capacity] is
+ * passed over (each operator says what that means). pos[l][b][h][t], when not
+ * NULL, is the position in the text of the token in that row; NULL means row t
+ * holds position t. next_pos[b] is the position of the next token (NULL: lens[b]);
+ * pos needs it. */
+typedef struct mrtdf_cache {
+  size_t struct_bytes;
+  void* k;
+  void* v;
+  int64_t stride_l, stride_b, stride_h, stride_t;
+  int32_t layers, batch, kv_heads, capacity, head_dim /* 64 or 128 */, dtype /* MRTDF_DTYPE_* */, device;
+  const int32_t* lens;     /* (batch) */
+  int32_t* pos;            /* (layers, batch, kv_heads, capacity) or NULL */
+  const int32_t* next_pos; /* (batch) or NULL */
+} mrtdf_cache;
+
+/* The KV cache of a stream as an operator's cache: kind 0 temporal self, 1
+ * depth self, 2 cross attention; one layer, or all of them when layer < 0.
+ * `len`, if not NULL, receives the rows in use. lens, pos and next_pos of
+ * `out` are NULL: the caller adds its own device arrays. The buffers belong to
+ * the stream; work on them is ordered with the stream's own by using
+ * mrtdf_stream_cuda(st). */
+int mrtdf_stream_cache(mrtdf_stream* st, int kind, int layer, mrtdf_cache* out, int* len);
+
+/*
+ * Attention of a tree of drafted tokens over a cache. Node i of sequence b
+ * hangs below node parents[b][i] < i, or below the last cached token (-1); a
+ * node with any other parent, and every node below it, is absent (padding).
+ * Query row (h, i) sees the cached rows t < lens[b] and the drafted rows of
+ * its ancestors and itself:
+ *   x = scale * q . k + rel_bias[h][clamp(next_pos[b] + depth(i) - position(row), 0, rel_len - 1)]
+ *   out = sum softmax(x) v,   lse = ln sum exp x
+ * where depth(i) counts i's ancestors and a drafted row's position is
+ * next_pos[b] + its depth. `heads` query heads share kv_heads in order (head h
+ * reads kv head h / (heads / kv_heads)). One node and parents NULL is a plain
+ * decode step; parents NULL with more nodes is a chain. 1 <= nodes <= 64,
+ * nodes * heads / kv_heads <= 1024. Scores, softmax statistics and sums are
+ * float32; float32 products use split tf32 operands (2^-23 relative), finite
+ * inputs below 2^127 in rows that are seen. The rows of an absent node, and of
+ * a sequence that is passed over, are zeros with lse = -inf; so is a row whose
+ * every score is -inf. Values in rows that a query row does not see do not
+ * reach it, NaN and infinities included. No rounding but that of the result
+ * depends on how the work is split; results are the same from run to run.
+ */
+typedef struct mrtdf_tree_args {
+  size_t struct_bytes;
+  mrtdf_rows q;     /* (batch, heads, nodes) rows */
+  mrtdf_rows k_new; /* (batch, kv_heads, nodes) rows, not in the cache yet */
+  mrtdf_rows v_new;
+  mrtdf_rows out; /* (batch, heads, nodes) rows */
+  float* lse;     /* (batch, heads, nodes) or NULL */
+  const int32_t* parents;  /* (batch, nodes) or NULL */
+  const float* rel_bias;   /* (heads, rel_len) or NULL */
+  void* workspace;         /* mrtdf_tree_attention_workspace bytes, 16-byte aligned; contents do not matter */
+  size_t workspace_bytes;
+  int32_t heads, nodes, rel_len;
+  float scale; /* 1.0 for the T5 attention of this engine */
+} mrtdf_tree_args;
+
+/* Workspace of a call with these sizes (0: none). Depends on the sizes and the
+ * device only, not on device memory; args' pointers must be set as for the
+ * call, workspace aside. */
+int mrtdf_tree_attention_workspace(const mrtdf_cache* cache, const mrtdf_tree_args* args, size_t* bytes);
+int mrtdf_tree_attention(const mrtdf_cache* cache, const mrtdf_tree_args* args, void* stream);
+
+/*
+ * The attention weight that each cached row collects (what mrtdf_cache_evict
+ * ranks rows by). path[b] lists the accepted nodes of sequence b, increasing
+ * and ended by the first entry that is not a node above the one before it (or
+ * by path_len); nodes that no longer fit into the capacity are left out. With
+ * q, k_new and lse of the verification (for every layer of the cache):
+ *   mass_out[t] = decay * mass[t] + sum over the query heads of the kv head and
+ *                 the path's nodes r of exp(x(r, t) - lse(r))        t < lens[b]
+ *   mass_out[lens[b] + j] = the same sum for the path's own row j, over r >= j
+ * that is where mrtdf_cache_commit puts the path's rows. Other entries are left
+ * as they are; mass_out may be mass. Node r of the path has depth r. A row with
+ * lse = -inf adds nothing; a sequence that is passed over is left alone. Sums
+ * are float32, one owner and one order each.
+ */
+typedef struct mrtdf_mass_args {
+  size_t struct_bytes;
+  mrtdf_rows q;     /* (layers, batch, heads, nodes) rows */
+  mrtdf_rows k_new; /* (layers, batch, kv_heads, nodes) rows */
+  const float* lse;      /* (layers, batch, heads, nodes) */
+  const int32_t* path;   /* (batch, path_len) */
+  const float* rel_bias; /* (heads, rel_len) or NULL, shared by the layers */
+  const float* mass;     /* (layers, batch, kv_heads, capacity) */
+  float* mass_out;
+  int32_t heads, nodes, path_len, rel_len;
+  float scale, decay;
+} mrtdf_mass_args;
+int mrtdf_cache_mass(const mrtdf_cache* cache, const mrtdf_mass_args* args, void* stream);
+
+/*
+ * Appends the accepted path to the cache of every layer: row lens[b] + j of K
+ * and V takes row path[b][j] of k_new and v_new, pos (if any) gets next_pos[b]
+ * + j, and lens_out[b] = lens[b] + nodes taken, next_pos_out[b] = next_pos[b] +
+ * the same. The path is read as by mrtdf_cache_mass. Rows behind the new length
+ * are left as they are. lens_out and next_pos_out are other buffers than lens
+ * and next_pos; a sequence that is passed over keeps both.
+ */
+typedef struct mrtdf_commit_args {
+  size_t struct_bytes;
+  mrtdf_rows k_new, v_new; /* (layers, batch, kv_heads, nodes) rows */
+  const int32_t* path;     /* (batch, path_len) */
+  int32_t* lens_out;       /* (batch) */
+  int32_t* next_pos_out;   /* (batch) or NULL */
+  int32_t nodes, path_len;
+} mrtdf_commit_args;
+int mrtdf_cache_commit(const mrtdf_cache* cache, const mrtdf_commit_args* args, void* stream);
+
+/*
+ * Eviction by collected weight. A sequence with more than `budget` rows keeps,
+ * in every layer and kv head by itself, the budget rows that come first by:
+ * protected (position >= next_pos[b] - recent, or < sinks), then the larger
+ * mass, then the lower row; a mass that is NaN comes last. Rows below the
+ * budget that are kept stay where they are; the i-th evicted row below the
+ * budget takes K, V, mass and pos of the i-th kept row at or above it, so at
+ * most the evicted rows are written (attention goes by pos, not by row order).
+ * mass_out and pos_out get the kept rows' entries (and those of sequences
+ * within the budget); they may be mass and cache.pos. lens_out[b] = min(lens[b],
+ * budget), another buffer than lens; a sequence that is passed over keeps its
+ * length and is left alone. Rows and entries at and above the new length are
+ * left as they are. recent + sinks <= budget; capacity <= 2^20 rows.
+ */
+typedef struct mrtdf_evict_args {
+  size_t struct_bytes;
+  const float* mass; /* (layers, batch, kv_heads, capacity) */
+  float* mass_out;
+  int32_t* pos_out;  /* (layers, batch, kv_heads, capacity) */
+  int32_t* lens_out; /* (batch) */
+  int32_t budget, recent, sinks;
+} mrtdf_evict_args;
+int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* args, void* stream);
+
+/*
+ * Product with 4-bit weights: out[m][n] = sum_k x[m][k] (scales[n][k / group] *
+ * q[n][k] + biases[n][k / group]), q in 0 .. 15. packed[n][j] holds column 2 j
+ * in its low half and 2 j + 1 in its high half. x, scales and biases are of
+ * `dtype`; out is of out_dtype (float32 for float32 x). The weights are not
+ * rounded: sums of x times whole numbers are scaled in float32. 1 <= m <= 64,
+ * k <= 2^17 a multiple of the group (32, 64 or 128), n <= 2^24; x's rows and
+ * packed on 16-byte boundaries.
+ */
+typedef struct mrtdf_q4_args {
+  size_t struct_bytes;
+  const void* x;      /* (m, k), x_stride elements from row to row */
+  const void* packed; /* (n, k / 2) bytes */
+  const void* scales; /* (n, k / group) */
+  const void* biases; /* (n, k / group) */
+  void* out;          /* (m, n), out_stride elements from row to row */
+  int64_t x_stride, out_stride;
+  int32_t m, n, k, group, dtype, out_dtype, device;
+} mrtdf_q4_args;
+int mrtdf_q4_linear(const mrtdf_q4_args* args, void* stream);
+
+/*
+ * Weights (n, k) of `dtype` to the form that mrtdf_q4_linear takes: per group
+ * of columns bias = min, scale = (max - min) / 15, both rounded to dtype, and
+ * q = (w - bias) / scale with those two, rounded to the nearest (ties to even)
+ * and clamped to 0 .. 15; a scale of 0 gives q = 0. Weights are finite.
+ */
+typedef struct mrtdf_q4_pack_args {
+  size_t struct_bytes;
+  const void* w; /* (n, k), w_stride elements from row to row */
+  void* packed;
+  void* scales;
+  void* biases;
+  int64_t w_stride;
+  int32_t n, k, group, dtype, device;
+} mrtdf_q4_pack_args;
+int mrtdf_q4_quantize(const mrtdf_q4_pack_args* args, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,930 @@
+// Attention of a tree of drafted tokens over a KV cache, and the attention
+// weight that each cached row has collected.
+//
+// Tree attention. Node i of sequence b sits at depth d_i (its proper ancestors
+// in the tree); row (head, i) sees every cached row t < len and the drafted
+// rows of its ancestors and itself:
+//   x_t = scale q . k_t + bias[head, clamp(next_pos + d_i - pos_t, 0, R - 1)]
+//   out = sum_t exp(x_t - m) v_t / sum_t exp(x_t - m),  lse = m + ln sum
+// in one pass over the rows with a running maximum m. All statistics and
+// sums are float32.
+//
+// The work is bound by the cache: 2 head_dim elements per cached row are read
+// for at most 64 x group queries. The nodes of one kv head's query heads are
+// stacked to one operand of up to 64 rows (more: several blocks, which read
+// the cache from L2 after the first). A CTA of four warps works on tiles of 64
+// keys; WM warps share a key range with 16 rows each, and the 4 / WM key
+// groups stream their own 16 * WM keys of each tile through a private
+// cp.async ring, so a group waits for nobody until its item ends.
+#include "cache_ops.cuh"
+#include "cache_tile.cuh"
+
+namespace mrtdf {
+namespace {
+
+constexpr int kTile = 64;      // keys per CTA tile
+constexpr int kThreads = 128;  // four warps
+constexpr int kStages = 3;
+
+// ---- schedule ----------------------------------------------------------------
+// A sequence's tiles: ceil((len + nodes) / 64), at least one. A length outside
+// [0, capacity] makes the sequence empty (len -1 here).
+__device__ __forceinline__ int checked_len(const CacheView& c, int b) {
+  const int l = c.lens[b];
+  return l < 0 || l > c.capacity ? -1 : l;
+}
+__device__ __forceinline__ int tiles_of(int len, int extra) { return (max(len, 0) + extra + kTile - 1) / kTile; }
+
+// lens[b] and first[b] = tiles of all items before sequence b's, for b <= B.
+// All 128 threads; ends with a barrier.
+__device__ void build_schedule(const CacheView& c, int layers, int batch, int items, int extra, int* lens, int* first) {
+  __shared__ int warp_sum[kThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, per = (batch + kThreads - 1) / kThreads;
+  int sum = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < batch) {
+      const int l = checked_len(c, b);
+      lens[b] = l;
+      sum += tiles_of(l, extra) * items;
+    }
+  }
+  int run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
+  }
+  if (lane == 31) warp_sum[tid >> 5] = run;
+  __syncthreads();
+  run -= sum;
+  for (int w = 0; w < (tid >> 5); ++w) run += warp_sum[w];
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < batch) {
+      first[b] = run;
+      run += tiles_of(lens[b], extra) * items;
+      if (b == batch - 1) first[batch] = run;
+    }
+  }
+  __syncthreads();
+}
+
+// Position in the list of tiles: sequence-major, then item, then tile.
+struct Cursor {
+  int w, b, item, tile, tiles, len;
+  __device__ __forceinline__ void seek(int at, const int* lens, const int* first, int batch, int items, int extra) {
+    w = at;
+    int lo = 0, hi = batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    len = lens[b];
+    tiles = tiles_of(len, extra);
+    const int rem = at - first[b];
+    item = rem / tiles;
+    tile = rem - item * tiles;
+  }
+  __device__ __forceinline__ void next(const int* lens, int batch, int items, int extra) {
+    ++w;
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++item < items) return;
+    item = 0;
+    if (++b < batch) {
+      len = lens[b];
+      tiles = tiles_of(len, extra);
+    }
+  }
+};
+
+// CTA c of g takes tiles [share(c), share(c + 1)) of `total`.
+__device__ __forceinline__ int share(int c, int g, int total) { return (int)((long long)c * total / g); }
+// The CTA whose run holds tile w.
+__device__ __forceinline__ int owner(int w, int g, int total) {
+  return (int)((((long long)w + 1) * g - 1) / total);
+}
+// CTAs that take part: a run has two tiles or more, or there is one tile each.
+__device__ __forceinline__ int active(int grid, int total) { return max(1, min(grid, total / 2)); }
+
+// ---- the tree ------------------------------------------------------------------
+// seen[i]: bit j set when node j is node i or an ancestor; 0 for a node that is
+// absent (its chain holds a parent outside [-1, i)). One warp; pointer
+// doubling: after k rounds a node knows 2^k links of its chain.
+__device__ void node_masks(unsigned long long* seen, const int32_t* parents, int nodes, bool there, int lane) {
+  constexpr int kRoot = -1, kAbsent = -2;
+  unsigned long long m[2];
+  int up[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = lane + 32 * h;
+    const int p = i < nodes ? (parents ? parents[i] : i - 1) : kAbsent;
+    up[h] = p < kRoot || p >= i ? kAbsent : p;
+    m[h] = 1ull << i;
+  }
+#pragma unroll
+  for (int round = 0; round < 6; ++round) {
+    unsigned long long om[2];
+    int ou[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int from = up[h] & 31;
+      const unsigned long long a = __shfl_sync(0xffffffffu, m[0], from), b = __shfl_sync(0xffffffffu, m[1], from);
+      const int c = __shfl_sync(0xffffffffu, up[0], from), d = __shfl_sync(0xffffffffu, up[1], from);
+      om[h] = up[h] >= 32 ? b : a;
+      ou[h] = up[h] >= 32 ? d : c;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (up[h] >= 0) {
+        m[h] |= om[h];
+        up[h] = ou[h];
+      }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = lane + 32 * h;
+    seen[i] = there && i < nodes && up[h] == kRoot ? m[h] : 0ull;
+  }
+  __syncwarp();
+}
+
+template <int WM>
+__device__ __forceinline__ void group_sync(int group) {
+  if constexpr (WM == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(WM * 32) : "memory");
+}
+
+__device__ __forceinline__ bool nonfinite(uint32_t w, __nv_bfloat16) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+__device__ __forceinline__ bool nonfinite(uint32_t w, float) { return (w & 0x7f800000u) == 0x7f800000u; }
+
+// Columns 8 n + 2 c, + 1 of value row `row`.
+template <int D>
+__device__ __forceinline__ float2 val2(uint32_t vals, int row, int n, int c, __nv_bfloat16) {
+  const uint32_t w = lds32(vals + Rows<__nv_bfloat16, D>::val_at(row, n) + 4 * c);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <int D>
+__device__ __forceinline__ float2 val2(uint32_t vals, int row, int n, int c, float) {
+  const uint32_t at = vals + Rows<float, D>::val_at(row, 2 * n + (c >> 1)) + 8 * (c & 1);
+  return make_float2(__uint_as_float(lds32(at)), __uint_as_float(lds32(at + 4)));
+}
+
+__device__ __forceinline__ void store2(__nv_bfloat16* p, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+
+// Shared memory of the attention kernel.
+template <typename T, int D, int WM>
+struct TreeSmem {
+  static constexpr int kStageBytes = 2 * kTile * Rows<T, D>::kBytes;
+  static constexpr int kMergeBytes = WM == 1 ? 2 * 16 * D * 4 : WM == 2 ? 32 * D * 4 : 0;
+  static constexpr int kScoreBytes = 16 * kTile * WM * 4;  // four warps x 16 rows x 16 WM keys
+  static constexpr int kScratch = kMergeBytes > kScoreBytes ? kMergeBytes : kScoreBytes;
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kPos = kStages * kTile * 4;
+  static constexpr int kStat = 4 * 32 * 16;        // four floats per lane
+  static constexpr int kSeen = 4 * kOpMaxNodes * 8;
+  static constexpr int kFixed = kRing + kScratch + kStat + kSeen + kPos;
+  static int bytes(int batch) { return kFixed + (2 * batch + 1) * 4; }
+};
+
+template <typename T, int D, int WM, bool BIAS>
+__global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_constant__ TreeParams p) {
+  using R = Rows<T, D>;
+  using S = TreeSmem<T, D, WM>;
+  constexpr int WK = 4 / WM, KT = 16 * WM, NT = KT / 8, MB = 16 * WM, ND = D / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* scratch = smem + S::kRing;
+  float4* stat = reinterpret_cast<float4*>(scratch + S::kScratch);
+  unsigned long long* seen_all = reinterpret_cast<unsigned long long*>(scratch + S::kScratch + S::kStat);
+  int* pos_s = reinterpret_cast<int*>(scratch + S::kScratch + S::kStat + S::kSeen);
+  int* lens = pos_s + kStages * kTile;
+  int* first = lens + p.c.batch;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, group = warp / WM;
+  const int g = lane >> 2, c = lane & 3, gt = wm * 32 + lane;
+  unsigned long long* seen = seen_all + warp * kOpMaxNodes;
+  const int batch = p.c.batch, items = p.c.kv_heads * p.row_blocks, nodes = p.nodes;
+  const int heads_per = p.heads / p.c.kv_heads, rows = heads_per * nodes;
+  build_schedule(p.c, 1, batch, items, nodes, lens, first);
+
+  // This CTA's run of tiles.
+  const int total = first[batch];
+  int w0, w1, parts;
+  if (p.stream) {
+    parts = active(p.grid, total);
+    if ((int)blockIdx.x >= parts) {
+      pdl_launch_dependents();
+      return;
+    }
+    w0 = share(blockIdx.x, parts, total);
+    w1 = share(blockIdx.x + 1, parts, total);
+  } else {
+    const int all = batch * items, i0 = share(blockIdx.x, p.grid, all), i1 = share(blockIdx.x + 1, p.grid, all);
+    parts = 0;
+    if (i0 >= i1) return;
+    auto start = [&](int i) {
+      if (i == all) return total;
+      const int b = i / items;
+      return first[b] + (i - b * items) * tiles_of(lens[b], nodes);
+    };
+    w0 = start(i0);
+    w1 = start(i1);
+  }
+
+  const uint32_t ring = smem_u32(smem) + group * (2 * KT * R::kBytes);
+  const T* kc = reinterpret_cast<const T*>(p.c.k);
+  const T* vc = reinterpret_cast<const T*>(p.c.v);
+  const T* kn = reinterpret_cast<const T*>(p.k_new.ptr);
+  const T* vn = reinterpret_cast<const T*>(p.v_new.ptr);
+
+  // Group's keys of the tile at `cur` into ring stage `st`.
+  auto fetch = [&](const Cursor& cur, int st) {
+    const int kvh = cur.item / p.row_blocks, len = max(cur.len, 0), key0 = cur.tile * kTile + group * KT;
+    const T* kb = kc + cur.b * p.c.sb + kvh * p.c.sh;
+    const T* vb = vc + cur.b * p.c.sb + kvh * p.c.sh;
+    const uint32_t kd = ring + st * S::kStageBytes, vd = kd + KT * R::kBytes;
+    constexpr int CH = R::kChunks;
+#pragma unroll
+    for (int i = 0; i < D * (int)sizeof(T) / 32; ++i) {
+      const int idx = gt + i * WM * 32, row = idx / CH, ch = idx % CH, j = key0 + row;
+      const T *ks, *vs;
+      if (j < len) {
+        ks = kb + j * p.c.st;
+        vs = vb + j * p.c.st;
+      } else {
+        const int n = min(j - len, nodes - 1);
+        ks = kn + cur.b * p.k_new.sb + kvh * p.k_new.sh + n * p.k_new.sn;
+        vs = vn + cur.b * p.v_new.sb + kvh * p.v_new.sh + n * p.v_new.sn;
+      }
+      const bool on = j < len + nodes;
+      cp_async16_zfill(kd + R::key_at(row, ch), ks + ch * (16 / sizeof(T)), on);
+      cp_async16_zfill(vd + R::val_at(row, ch), vs + ch * (16 / sizeof(T)), on);
+    }
+    if (BIAS && p.c.pos && gt < KT) {
+      const int j = key0 + gt;
+      const int32_t* ps = p.c.pos + (int64_t)(cur.b * p.c.kv_heads + kvh) * p.c.capacity;
+      cp_async4_zfill(smem_u32(pos_s + st * kTile + group * KT + gt), ps + min(j, max(len - 1, 0)), j < len);
+    }
+  };
+
+  Cursor ahead, cur;
+  ahead.seek(w0, lens, first, batch, items, nodes);
+  cur = ahead;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (ahead.w < w1) {
+      fetch(ahead, i);
+      ahead.next(lens, batch, items, nodes);
+    }
+    cp_async_commit();
+  }
+
+  QFrag<T, D> q;
+  float o[ND][4], m0 = 0, m1 = 0, l0 = 0, l1 = 0, far0 = 0, far1 = 0;
+  unsigned long long see0 = 0, see1 = 0;
+  const float *tab0 = nullptr, *tab1 = nullptr;
+  int at0 = 0, at1 = 0, next = 0, masks_of = -1, first_tile = 0;
+  bool fresh = true;
+
+  for (int st = 0, fill = kStages - 1; cur.w < w1; cur.next(lens, batch, items, nodes)) {
+    cp_async_wait<kStages - 2>();
+    group_sync<WM>(group);
+    if (ahead.w < w1) {
+      fetch(ahead, fill);
+      ahead.next(lens, batch, items, nodes);
+    }
+    cp_async_commit();
+    const int len = max(cur.len, 0), kvh = cur.item / p.row_blocks, row0 = (cur.item % p.row_blocks) * MB + wm * 16;
+
+    if (fresh) {  // a new item: its rows, statistics and masks
+      fresh = false;
+      first_tile = cur.tile;
+      if (masks_of != cur.b) {
+        masks_of = cur.b;
+        __syncwarp();
+        node_masks(seen, p.parents ? p.parents + cur.b * nodes : nullptr, nodes, cur.len >= 0, lane);
+        next = p.c.next_pos ? p.c.next_pos[cur.b] : len;
+      }
+      const T *q0 = nullptr, *q1 = nullptr;
+      see0 = see1 = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row0 + g + 8 * h;
+        if (r < rows) {
+          const int hd = r / nodes, n = r - hd * nodes, head = kvh * heads_per + hd;
+          const T* qr = reinterpret_cast<const T*>(p.q.ptr) + cur.b * p.q.sb + head * p.q.sh + n * p.q.sn;
+          const unsigned long long s = seen[n];
+          (h ? q1 : q0) = qr;
+          (h ? see1 : see0) = s;
+          if (BIAS) {
+            const float* t = p.rel_bias + (int64_t)head * p.rel_len;
+            (h ? tab1 : tab0) = t;
+            (h ? at1 : at0) = (int)((unsigned)next + (unsigned)(__popcll(s) - (s ? 1 : 0)));
+            (h ? far1 : far0) = t[p.rel_len - 1];
+          }
+        } else if (BIAS) {
+          (h ? tab1 : tab0) = p.rel_bias;
+        }
+      }
+      q.load(q0, q1, lane);
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.f;
+#pragma unroll
+      for (int n = 0; n < ND; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    }
+
+    const uint32_t keys = ring + st * S::kStageBytes, vals = keys + KT * R::kBytes;
+    const int key0 = cur.tile * kTile + group * KT;
+    if (key0 < len + nodes) {
+      float s[NT][4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      qk_tile<D, NT>(s, q, keys, lane);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] *= p.scale;
+
+      const bool tail = key0 + KT > len;
+      // Position of this lane's key 8 j + 2 c + e: stored, the slot, or the
+      // drafted node's.
+      auto key_pos = [&](int k) {
+        const int key = key0 + k;
+        if (key >= len) {
+          const unsigned long long s = key - len < nodes ? seen[key - len] : 0ull;
+          return (int)((unsigned)next + (unsigned)(__popcll(s) - (s ? 1 : 0)));
+        }
+        return p.c.pos ? pos_s[st * kTile + group * KT + k] : key;
+      };
+      if (BIAS) {
+        int ps[NT][2];
+        bool near = tail;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            ps[j][e] = key_pos(8 * j + 2 * c + e);
+            near |= (int)((unsigned)next - (unsigned)ps[j][e]) < p.rel_len - 1;
+          }
+        if (__any_sync(0xffffffffu, near)) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d0 = min(max((int)((unsigned)at0 - (unsigned)ps[j][e]), 0), p.rel_len - 1);
+              const int d1 = min(max((int)((unsigned)at1 - (unsigned)ps[j][e]), 0), p.rel_len - 1);
+              s[j][e] += __ldg(tab0 + d0);
+              s[j][2 + e] += __ldg(tab1 + d1);
+            }
+        } else {  // every key is further than the table: its last entry
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            s[j][0] += far0;
+            s[j][1] += far0;
+            s[j][2] += far1;
+            s[j][3] += far1;
+          }
+        }
+      }
+      auto visible = [&](int key, unsigned long long see) {
+        if (key < len) return see != 0;
+        return key - len < nodes && (see >> (key - len) & 1) != 0;
+      };
+      if (tail) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = key0 + 8 * j + 2 * c + e;
+            if (!visible(key, see0)) s[j][e] = -INFINITY;
+            if (!visible(key, see1)) s[j][2 + e] = -INFINITY;
+          }
+      }
+
+      float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
+        x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+      }
+#pragma unroll
+      for (int i = 1; i < 4; i <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, i));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, i));
+      }
+      x0 = fmaxf(x0, m0);
+      x1 = fmaxf(x1, m1);
+      // A row that has seen nothing keeps m = -inf; 0 stands in for it below.
+      const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+        const float f0 = ex2((m0 - u0) * kLog2e), f1 = ex2((m1 - u1) * kLog2e);
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          o[n][0] *= f0;
+          o[n][1] *= f0;
+          o[n][2] *= f1;
+          o[n][3] *= f1;
+        }
+        m0 = x0;
+        m1 = x1;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        s[j][0] = ex2((s[j][0] - u0) * kLog2e);
+        s[j][1] = ex2((s[j][1] - u0) * kLog2e);
+        s[j][2] = ex2((s[j][2] - u1) * kLog2e);
+        s[j][3] = ex2((s[j][3] - u1) * kLog2e);
+        l0 += s[j][0] + s[j][1];
+        l1 += s[j][2] + s[j][3];
+      }
+
+      // 0 x inf: where a drafted value row that some row must not see is not
+      // finite, the products are added one by one, only where they count.
+      bool odd = false;
+      if (tail) {
+        for (int i = lane; i < KT * R::kBytes / 4; i += 32) odd |= nonfinite(lds32(vals + 4 * i), T());
+        odd = __any_sync(0xffffffffu, odd);
+      }
+      if (odd) {
+        float* ps = reinterpret_cast<float*>(scratch) + warp * (16 * KT);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ps[(g + 8 * (e >> 1)) * KT + 8 * j + 2 * c + (e & 1)] = s[j][e];
+        __syncwarp();
+        for (int k = 0; k < KT; ++k) {
+          const bool v0 = visible(key0 + k, see0), v1 = visible(key0 + k, see1);
+          const float p0 = ps[g * KT + k], p1 = ps[(g + 8) * KT + k];
+#pragma unroll
+          for (int n = 0; n < ND; ++n) {
+            const float2 v = val2<D>(vals, k, n, c, T());
+            if (v0) {
+              o[n][0] += p0 * v.x;
+              o[n][1] += p0 * v.y;
+            }
+            if (v1) {
+              o[n][2] += p1 * v.x;
+              o[n][3] += p1 * v.y;
+            }
+          }
+        }
+        __syncwarp();
+      } else {
+        pv_tile<D, NT>(o, s, vals, lane, T());
+      }
+    }
+    st = st + 1 == kStages ? 0 : st + 1;
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+
+    if (cur.tile + 1 < cur.tiles && cur.w + 1 < w1) continue;
+    // ---- the item's run ends here: join the key groups, write ----------------
+    fresh = true;
+#pragma unroll
+    for (int i = 1; i < 4; i <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, i);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, i);
+    }
+    if constexpr (WK > 1) {
+      float4* buf = reinterpret_cast<float4*>(scratch);
+      __syncthreads();  // nobody still reads scores or an earlier join there
+#pragma unroll
+      for (int half = WK / 2; half >= 1; half >>= 1) {
+        const int slot = ((group % half) * WM + wm) * 32 + lane;
+        if (group >= half && group < 2 * half) {
+#pragma unroll
+          for (int n = 0; n < ND; ++n)
+            buf[(((group % half) * WM + wm) * ND + n) * 32 + lane] = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
+          stat[slot] = make_float4(m0, m1, l0, l1);
+        }
+        __syncthreads();
+        if (group < half) {
+          const float4 t = stat[slot];
+          const float x0 = fmaxf(m0, t.x), x1 = fmaxf(m1, t.y);
+          const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
+          const float a0 = ex2((m0 - u0) * kLog2e), a1 = ex2((m1 - u1) * kLog2e);
+          const float b0 = ex2((t.x - u0) * kLog2e), b1 = ex2((t.y - u1) * kLog2e);
+          l0 = l0 * a0 + t.z * b0;
+          l1 = l1 * a1 + t.w * b1;
+          m0 = x0;
+          m1 = x1;
+#pragma unroll
+          for (int n = 0; n < ND; ++n) {
+            const float4 v = buf[(((group % half) * WM + wm) * ND + n) * 32 + lane];
+            o[n][0] = o[n][0] * a0 + v.x * b0;
+            o[n][1] = o[n][1] * a0 + v.y * b0;
+            o[n][2] = o[n][2] * a1 + v.z * b1;
+            o[n][3] = o[n][3] * a1 + v.w * b1;
+          }
+        }
+        __syncthreads();
+      }
+    }
+    if (group == 0) {
+      const bool whole = first_tile == 0 && cur.tile + 1 == cur.tiles;
+      if (!see0) {
+        m0 = -INFINITY;
+        l0 = 0.f;
+      }
+      if (!see1) {
+        m1 = -INFINITY;
+        l1 = 0.f;
+      }
+      if (whole) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = row0 + g + 8 * h;
+          if (r >= rows) continue;
+          const int hd = r / nodes, n = r - hd * nodes, head = kvh * heads_per + hd;
+          const float l = h ? l1 : l0, m = h ? m1 : m0, inv = l == 0.f ? 0.f : 1.f / l;
+          T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + cur.b * p.out.sb + head * p.out.sh + n * p.out.sn;
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const float a = h ? o[i][2] : o[i][0], b = h ? o[i][3] : o[i][1];
+            store2(dst + 8 * i + 2 * c, l == 0.f ? 0.f : a * inv, l == 0.f ? 0.f : b * inv);
+          }
+          if (p.lse && c == 0)
+            p.lse[((int64_t)cur.b * p.heads + head) * nodes + n] = l == 0.f ? -INFINITY : m + logf(l);
+        }
+      } else {
+        // Slot 1: a run that starts an item; slot 0: one that goes on with it.
+        float* part = p.ws + (int64_t)(blockIdx.x * 2 + (first_tile == 0)) * MB * (D + 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = wm * 16 + g + 8 * h;
+#pragma unroll
+          for (int i = 0; i < ND; ++i)
+            store2(part + r * D + 8 * i + 2 * c, h ? o[i][2] : o[i][0], h ? o[i][3] : o[i][1]);
+          if (c == 0) {
+            part[MB * D + r] = h ? m1 : m0;
+            part[MB * D + MB + r] = h ? l1 : l0;
+          }
+        }
+      }
+    }
+  }
+  pdl_launch_dependents();
+}
+
+// Joins the partial rows of items that several CTAs worked on: a warp per row.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_constant__ TreeParams p, int mb) {
+  extern __shared__ __align__(16) int sched[];
+  int *lens = sched, *first = sched + p.c.batch;
+  const int items = p.c.kv_heads * p.row_blocks, nodes = p.nodes;
+  build_schedule(p.c, 1, p.c.batch, items, nodes, lens, first);
+  const int b = blockIdx.x / items, item = blockIdx.x % items, total = first[p.c.batch];
+  const int parts = active(p.grid, total), tiles = tiles_of(lens[b], nodes), w = first[b] + item * tiles;
+  const int c0 = owner(w, parts, total), c1 = owner(w + tiles - 1, parts, total);
+  pdl_wait();
+  if (c0 == c1) return;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5);
+  const int heads_per = p.heads / p.c.kv_heads, row = (item % p.row_blocks) * mb + r;
+  if (r >= mb || row >= heads_per * nodes) return;
+  auto part = [&](int c) { return p.ws + (int64_t)(c * 2 + (c == c0)) * mb * (D + 2); };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part(c)[mb * D + r]);
+  m = warp_max(m);
+  const float u = m == -INFINITY ? 0.f : m;
+  constexpr int V = D / 32;
+  float acc[V] = {}, sum = 0.f;
+  for (int cb = c0; cb <= c1; cb += 32) {
+    const int mine = cb + lane;
+    float wt = 0.f;
+    if (mine <= c1) {
+      wt = ex2((part(mine)[mb * D + r] - u) * kLog2e);
+      const float l = part(mine)[mb * D + mb + r];
+      sum += l == 0.f ? 0.f : l * wt;
+    }
+    const int n = min(32, c1 - cb + 1);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float f = __shfl_sync(0xffffffffu, wt, i);
+      const float* src = part(cb + i) + r * D + lane * V;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float v = src[k];
+        if (!(f == 0.f)) acc[k] += v * f;
+      }
+    }
+  }
+  sum = warp_sum(sum);
+  const int hd = row / nodes, n = row - hd * nodes, head = (item / p.row_blocks) * heads_per + hd;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + n * p.out.sn + lane * V;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int k = 0; k < V; k += 2)
+    store2(dst + k, sum == 0.f ? 0.f : acc[k] * inv, sum == 0.f ? 0.f : acc[k + 1] * inv);
+  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + head) * nodes + n] = sum == 0.f ? -INFINITY : m + logf(sum);
+}
+
+// ---- collected weight ------------------------------------------------------------
+// mass_out[t] = decay mass[t] + sum over the accepted path's rows (head, i) of
+// exp(x_t - lse) for cached rows t < len, and for the path's own rows, which
+// commit will put at len + j, the sum over i >= j. The softmax statistics come
+// from the attention (lse), so only the keys are read again: head_dim elements
+// and 8 bytes of weight per cached row bound it. A warp owns 16 keys of a tile
+// and sums its columns over all rows, so every sum has one owner and one order.
+constexpr int kMassRows = 64;  // query rows held in shared memory at a time
+
+template <typename T, int D>
+struct MassSmem {
+  static constexpr int kStageBytes = kTile * Rows<T, D>::kBytes;
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kQ = kMassRows * Rows<T, D>::kBytes;
+  static constexpr int kFixed = kRing + kQ + kStages * kTile * 4 + kMassRows * 4 + kOpMaxNodes * 4;
+  static int bytes(int batch) { return kFixed + (2 * batch + 1) * 4; }
+};
+
+// Row fragments from shared memory rows in the key layout.
+template <int D>
+__device__ __forceinline__ void q_from_smem(QFrag<__nv_bfloat16, D>& q, uint32_t base, int lane) {
+  const int m = lane >> 3, r = lane & 7;
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+    ldsm_x4_g(q.a[ks], base + Rows<__nv_bfloat16, D>::key_at((m & 1) * 8 + r, 2 * ks + (m >> 1)));
+}
+template <int D>
+__device__ __forceinline__ void q_from_smem(QFrag<float, D>& q, uint32_t base, int lane) {
+  const int m = lane >> 3, r = lane & 7;
+#pragma unroll
+  for (int ks = 0; ks < D / 8; ++ks)
+    ldsm_x4_g(q.a[ks], base + Rows<float, D>::key_at((m & 1) * 8 + r, 2 * ks + (m >> 1)));
+}
+
+// Nodes of the accepted path: up to the first entry that is not a node after
+// the one before it, as many as fit into the cache. One warp.
+__device__ int path_nodes(const int32_t* path, int path_len, int nodes, int room, int lane) {
+  int n = 0;
+  for (int base = 0; base < path_len; base += 32) {
+    const int i = base + lane;
+    const int v = i < path_len ? path[i] : -1, before = i > 0 && i <= path_len ? path[i - 1] : -1;
+    const unsigned ok = __ballot_sync(0xffffffffu, v > before && v >= 0 && v < nodes);
+    const int run = ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
+    n += run;
+    if (run < 32) break;
+  }
+  return min(n, room);
+}
+
+template <typename T, int D, bool BIAS>
+__global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_constant__ MassParams p) {
+  using R = Rows<T, D>;
+  using S = MassSmem<T, D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* q_s = smem + S::kRing;
+  int* pos_s = reinterpret_cast<int*>(q_s + S::kQ);
+  float* lse_s = reinterpret_cast<float*>(pos_s + kStages * kTile);
+  int* path_s = reinterpret_cast<int*>(lse_s + kMassRows);
+  int* lens = path_s + kOpMaxNodes;
+  int* first = lens + p.c.batch;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int batch = p.c.batch, items = p.c.layers * p.c.kv_heads, extra = p.path_len;
+  const int heads_per = p.heads / p.c.kv_heads;
+  build_schedule(p.c, 1, batch, items, extra, lens, first);
+  const int total = first[batch], parts = active(p.grid, total);
+  if ((int)blockIdx.x >= parts) return;
+  const int w0 = share(blockIdx.x, parts, total), w1 = share(blockIdx.x + 1, parts, total);
+  const uint32_t ring = smem_u32(smem) + warp * (16 * R::kBytes);
+
+  Cursor cur;
+  cur.seek(w0, lens, first, batch, items, extra);
+  while (cur.w < w1) {
+    // One item's run of tiles [t0, t1): layer, sequence, kv head.
+    const int layer = cur.item / p.c.kv_heads, kvh = cur.item % p.c.kv_heads, b = cur.b;
+    const int t0 = cur.tile, t1 = min(cur.tiles, cur.tile + (w1 - cur.w)), len = max(cur.len, 0);
+    const bool there = cur.len >= 0;
+    __syncthreads();  // the item before is done with the path and the rows
+    int count = 0;
+    if (there) count = path_nodes(p.path + b * p.path_len, p.path_len, p.nodes, p.c.capacity - len, lane);
+    for (int i = tid; i < p.path_len; i += kThreads) path_s[i] = i < count ? p.path[b * p.path_len + i] : 0;
+    const int rows = heads_per * count, next = p.c.next_pos ? p.c.next_pos[b] : len;
+    const int64_t row_at = ((int64_t)(layer * batch + b) * p.c.kv_heads + kvh) * p.c.capacity;
+    const T* kb = reinterpret_cast<const T*>(p.c.k) + layer * p.c.sl + b * p.c.sb + kvh * p.c.sh;
+    const T* kn = reinterpret_cast<const T*>(p.k_new.ptr) + layer * p.k_new.sl + b * p.k_new.sb + kvh * p.k_new.sh;
+    __syncthreads();
+
+    auto fetch = [&](int tile, int st) {
+      const int key0 = tile * kTile + warp * 16;
+      const uint32_t kd = ring + st * S::kStageBytes;
+      constexpr int CH = R::kChunks;
+#pragma unroll
+      for (int i = 0; i < CH / 2; ++i) {
+        const int idx = lane + i * 32, row = idx / CH, ch = idx % CH, j = key0 + row;
+        const T* ks = j < len ? kb + j * p.c.st : kn + path_s[min(j - len, p.path_len - 1)] * p.k_new.sn;
+        cp_async16_zfill(kd + R::key_at(row, ch), ks + ch * (16 / sizeof(T)), rows > 0 && j < len + count);
+      }
+      if (BIAS && p.c.pos && lane < 16) {
+        const int j = key0 + lane;
+        cp_async4_zfill(smem_u32(pos_s + st * kTile + warp * 16 + lane), p.c.pos + row_at + min(j, max(len - 1, 0)), j < len);
+      }
+    };
+
+    // Rows in blocks of 64 (one block where the path is empty: the decay).
+    for (int rb = 0; rb == 0 || rb < rows; rb += kMassRows) {
+      const int here = min(kMassRows, rows - rb);
+      if (rb) __syncthreads();
+      for (int i = tid; i < kMassRows * R::kChunks; i += kThreads) {
+        const int row = i / R::kChunks, ch = i % R::kChunks, r = rb + row;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < here) {
+          const int hd = r / count, n = path_s[r - hd * count], head = kvh * heads_per + hd;
+          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q.ptr) + layer * p.q.sl + b * p.q.sb +
+                                              head * p.q.sh + n * p.q.sn + ch * (16 / sizeof(T)));
+          if (ch == 0) lse_s[row] = p.lse[((int64_t)(layer * batch + b) * p.heads + head) * p.nodes + n];
+        }
+        *reinterpret_cast<uint4*>(q_s + R::key_at(row, ch)) = v;
+      }
+      for (int i = 0; i < kStages - 1; ++i) {
+        if (t0 + i < t1) fetch(t0 + i, i);
+        cp_async_commit();
+      }
+      __syncthreads();
+      QFrag<T, D> q;
+      if (here <= 16) q_from_smem<D>(q, smem_u32(q_s), lane);
+
+      for (int t = t0, st = 0, fill = kStages - 1; t < t1; ++t) {
+        cp_async_wait<kStages - 2>();
+        __syncwarp();
+        if (t + kStages - 1 < t1) fetch(t + kStages - 1, fill);
+        cp_async_commit();
+        const int key0 = t * kTile + warp * 16;
+        const uint32_t keys = ring + st * S::kStageBytes;
+        // Lane's weights: keys 8 j + 2 c + e, from the lanes with g = 0.
+        float old[2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = key0 + 8 * j + 2 * c + e;
+            old[j][e] = g == 0 && key < len + count && there
+                            ? (rb ? p.mass_out[row_at + key] : key < len ? p.decay * p.mass[row_at + key] : 0.f)
+                            : 0.f;
+          }
+        float col[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        for (int mt = 0; mt * 16 < here; ++mt) {
+          if (here > 16) q_from_smem<D>(q, smem_u32(q_s) + mt * 16 * R::kBytes, lane);
+          float s[2][4] = {};
+          qk_tile<D, 2>(s, q, keys, lane);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = mt * 16 + g + 8 * h, r = rb + row;
+            if (row >= here) continue;
+            const int hd = r / count, i = r - hd * count;
+            const float lse = lse_s[row];
+            const float* tab = BIAS ? p.rel_bias + (int64_t)(kvh * heads_per + hd) * p.rel_len : nullptr;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = key0 + 8 * j + 2 * c + e;
+                float x = s[j][2 * h + e] * p.scale;
+                if (BIAS) {
+                  const int at = key >= len ? next + (key - len)
+                                 : p.c.pos  ? pos_s[st * kTile + warp * 16 + 8 * j + 2 * c + e]
+                                            : key;
+                  const int d = min(max((int)((unsigned)(next + i) - (unsigned)at), 0), p.rel_len - 1);
+                  x += __ldg(tab + d);
+                }
+                // A row whose softmax is empty (lse = -inf) gives nothing.
+                const bool on = key - len <= i && lse != -INFINITY;
+                col[j][e] += on ? ex2((x - lse) * kLog2e) : 0.f;
+              }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) col[j][e] += __shfl_xor_sync(0xffffffffu, col[j][e], o);
+            const int key = key0 + 8 * j + 2 * c + e;
+            if (g == 0 && key < len + count && there) p.mass_out[row_at + key] = old[j][e] + col[j][e];
+          }
+        st = st + 1 == kStages ? 0 : st + 1;
+        fill = fill + 1 == kStages ? 0 : fill + 1;
+      }
+      cp_async_wait<0>();
+    }
+    // To the next item.
+    cur.w += t1 - t0;
+    if (t1 == cur.tiles && cur.w < w1) {
+      cur.w -= 1;
+      cur.tile = cur.tiles - 1;
+      cur.next(lens, batch, items, extra);
+    }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <typename T, int D, int WM, bool BIAS>
+cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
+  auto* k = tree_attn_kernel<T, D, WM, BIAS>;
+  const int bytes = TreeSmem<T, D, WM>::bytes(p.c.batch);
+  cudaError_t e = allow_smem(k, bytes);
+  if (e != cudaSuccess) return e;
+  k<<<p.grid, kThreads, bytes, s>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !p.stream) return e;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.c.batch * p.c.kv_heads * p.row_blocks, (16 * WM + 3) / 4);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (2 * p.c.batch + 1) * 4;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, p, 16 * WM);
+}
+
+template <typename T, int D>
+cudaError_t tree_variant(const TreeParams& p, int wm, cudaStream_t s) {
+  if (p.rel_bias)
+    return wm == 1 ? tree_run<T, D, 1, true>(p, s) : wm == 2 ? tree_run<T, D, 2, true>(p, s) : tree_run<T, D, 4, true>(p, s);
+  return wm == 1 ? tree_run<T, D, 1, false>(p, s) : wm == 2 ? tree_run<T, D, 2, false>(p, s) : tree_run<T, D, 4, false>(p, s);
+}
+
+// Warps that share a key range: one per 16 query rows, up to four.
+int tree_wm(const TreeParams& p) {
+  const int rows = p.heads / p.c.kv_heads * p.nodes;
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+}
+int tree_smem(const TreeParams& p, int wm) {
+  const int b = p.c.batch;
+  const bool f = p.c.dtype == 0;
+  if (p.c.head_dim == 64) {
+    if (f) return wm == 1 ? TreeSmem<float, 64, 1>::bytes(b) : wm == 2 ? TreeSmem<float, 64, 2>::bytes(b) : TreeSmem<float, 64, 4>::bytes(b);
+    return wm == 1 ? TreeSmem<__nv_bfloat16, 64, 1>::bytes(b) : wm == 2 ? TreeSmem<__nv_bfloat16, 64, 2>::bytes(b) : TreeSmem<__nv_bfloat16, 64, 4>::bytes(b);
+  }
+  if (f) return wm == 1 ? TreeSmem<float, 128, 1>::bytes(b) : wm == 2 ? TreeSmem<float, 128, 2>::bytes(b) : TreeSmem<float, 128, 4>::bytes(b);
+  return wm == 1 ? TreeSmem<__nv_bfloat16, 128, 1>::bytes(b) : wm == 2 ? TreeSmem<__nv_bfloat16, 128, 2>::bytes(b) : TreeSmem<__nv_bfloat16, 128, 4>::bytes(b);
+}
+
+constexpr int kSmSmem = 227 * 1024;
+
+}  // namespace
+
+cudaError_t plan_tree_attention(TreeParams& p, int sms, size_t* ws_floats) {
+  const int wm = tree_wm(p), mb = 16 * wm, rows = p.heads / p.c.kv_heads * p.nodes;
+  p.row_blocks = (rows + mb - 1) / mb;
+  const int items = p.c.batch * p.c.kv_heads * p.row_blocks;
+  const int per_sm = max(1, min(4, kSmSmem / (tree_smem(p, wm) + 1024)));
+  const int slots = sms * per_sm, most = (p.c.capacity + p.nodes + kTile - 1) / kTile;
+  // Short caches: an item is a few tiles, whole items per CTA need no join.
+  p.stream = most > 4;
+  p.grid = p.stream ? (int)min((long long)slots, max(1ll, (long long)items * most / 2)) : min(items, slots);
+  *ws_floats = p.stream ? (size_t)p.grid * 2 * mb * (p.c.head_dim + 2) : 0;
+  return cudaSuccess;
+}
+
+cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t s) {
+  const int wm = tree_wm(p);
+  if (p.c.dtype == 0) return p.c.head_dim == 64 ? tree_variant<float, 64>(p, wm, s) : tree_variant<float, 128>(p, wm, s);
+  return p.c.head_dim == 64 ? tree_variant<__nv_bfloat16, 64>(p, wm, s) : tree_variant<__nv_bfloat16, 128>(p, wm, s);
+}
+
+namespace {
+template <typename T, int D, bool BIAS>
+cudaError_t mass_run(MassParams& p, cudaStream_t s) {
+  auto* k = cache_mass_kernel<T, D, BIAS>;
+  const int bytes = MassSmem<T, D>::bytes(p.c.batch);
+  cudaError_t e = allow_smem(k, bytes);
+  if (e != cudaSuccess) return e;
+  int dev = 0;
+  e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const int per_sm = max(1, min(4, kSmSmem / (bytes + 1024)));
+  const long long most = (long long)p.c.batch * p.c.layers * p.c.kv_heads * ((p.c.capacity + p.path_len + kTile - 1) / kTile);
+  p.grid = (int)min((long long)op_sm_count(dev) * per_sm, max(1ll, most / 2));
+  k<<<p.grid, kThreads, bytes, s>>>(p);
+  return cudaGetLastError();
+}
+template <typename T, int D>
+cudaError_t mass_variant(MassParams& p, cudaStream_t s) {
+  return p.rel_bias ? mass_run<T, D, true>(p, s) : mass_run<T, D, false>(p, s);
+}
+}  // namespace
+
+cudaError_t launch_cache_mass(MassParams& p, cudaStream_t s) {
+  if (p.c.dtype == 0) return p.c.head_dim == 64 ? mass_variant<float, 64>(p, s) : mass_variant<float, 128>(p, s);
+  return p.c.head_dim == 64 ? mass_variant<__nv_bfloat16, 64>(p, s) : mass_variant<__nv_bfloat16, 128>(p, s);
+}
+
+}  // namespace mrtdf

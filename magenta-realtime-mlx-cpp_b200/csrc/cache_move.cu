@@ -1,0 +1,383 @@
+// Rows of a KV cache that move: commit of an accepted path, eviction by
+// collected weight. Both are bound by the rows they move (head_dim elements
+// of K and V, read once and written once) and by latency when there are few.
+#include "cache_ops.cuh"
+#include "common.cuh"
+#include "decode_device.cuh"
+
+namespace mrtdf {
+namespace {
+
+constexpr int kMoveThreads = 256;
+
+// Nodes of the accepted path: up to the first entry that is not a node after
+// the one before it, as many as fit into the cache. One warp.
+__device__ int accepted(const int32_t* path, int path_len, int nodes, int room, int lane) {
+  int n = 0;
+  for (int base = 0; base < path_len; base += 32) {
+    const int i = base + lane;
+    const int v = i < path_len ? path[i] : -1, before = i > 0 && i <= path_len ? path[i - 1] : -1;
+    const unsigned ok = __ballot_sync(0xffffffffu, v > before && v >= 0 && v < nodes);
+    const int run = ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
+    n += run;
+    if (run < 32) break;
+  }
+  return min(n, room);
+}
+
+// K[len + j] = K_new[path[j]], V alike, pos[len + j] = next_pos + j for every
+// layer and kv head of sequence blockIdx.y. The accepted rows of all layers
+// are one flat list of 16-byte chunks, so a sequence's CTAs share it evenly
+// whatever its path length. Each thread has four K and four V loads in flight.
+template <int CH>  // 16-byte chunks per row
+__global__ __launch_bounds__(kMoveThreads) void cache_commit_kernel(const __grid_constant__ CommitParams p, int esize) {
+  const int b = blockIdx.y, lane = threadIdx.x & 31;
+  const int len = p.c.lens[b];
+  const bool there = len >= 0 && len <= p.c.capacity;
+  const int count = there ? accepted(p.path + (int64_t)b * p.path_len, p.path_len, p.nodes, p.c.capacity - len, lane) : 0;
+  const int next = p.c.next_pos ? p.c.next_pos[b] : len;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.lens_out[b] = len + count;
+    if (p.next_pos_out) p.next_pos_out[b] = (int)((unsigned)next + (unsigned)count);
+  }
+  if (!count) return;
+  const int heads = p.c.layers * p.c.kv_heads;
+  const long long total = (long long)heads * count * CH;
+  const long long stride = (long long)gridDim.x * kMoveThreads;
+  uint8_t *kc = (uint8_t*)p.c.k, *vc = (uint8_t*)p.c.v;
+  const uint8_t *kn = (const uint8_t*)p.k_new.ptr, *vn = (const uint8_t*)p.v_new.ptr;
+  for (long long i0 = (long long)blockIdx.x * kMoveThreads + threadIdx.x; i0 < total; i0 += 4 * stride) {
+    uint4 kv[4], vv[4];
+    int64_t to[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long i = i0 + u * stride;
+      if (i >= total) continue;
+      const int ch = (int)(i % CH), row = (int)(i / CH), j = row % count, hd = row / count;
+      const int layer = hd / p.c.kv_heads, kvh = hd - layer * p.c.kv_heads;
+      const int n = p.path[(int64_t)b * p.path_len + j];
+      const int64_t kf = layer * p.k_new.sl + b * p.k_new.sb + kvh * p.k_new.sh + n * p.k_new.sn;
+      const int64_t vf = layer * p.v_new.sl + b * p.v_new.sb + kvh * p.v_new.sh + n * p.v_new.sn;
+      kv[u] = *reinterpret_cast<const uint4*>(kn + kf * esize + ch * 16);
+      vv[u] = *reinterpret_cast<const uint4*>(vn + vf * esize + ch * 16);
+      to[u] = (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh + (int64_t)(len + j) * p.c.st) * esize + ch * 16;
+      if (ch == 0 && p.c.pos)
+        p.c.pos[((int64_t)(layer * p.c.batch + b) * p.c.kv_heads + kvh) * p.c.capacity + len + j] =
+            (int)((unsigned)next + (unsigned)j);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + u * stride >= total) continue;
+      *reinterpret_cast<uint4*>(kc + to[u]) = kv[u];
+      *reinterpret_cast<uint4*>(vc + to[u]) = vv[u];
+    }
+  }
+}
+
+// ---- eviction ----------------------------------------------------------------------
+// One thread-block cluster per (layer, sequence, kv head); CTA r looks after
+// slots [r * slice, (r + 1) * slice). Kept are the `budget` slots that come
+// first by (protected, weight from the largest, slot from the lowest); a
+// weight that is NaN comes last. The threshold is found by three histogram
+// passes over an order-preserving 32-bit key (11, 11, 10 bits) whose counts
+// the cluster adds up over distributed shared memory. Kept slots go into a
+// bitmap; the i-th evicted slot below the budget (a hole) takes the i-th kept
+// slot at or above it. Holes are below the budget and sources at or above it,
+// so every row moves once, in place, in any order.
+constexpr int kEvictThreads = 256;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMaxCluster = 8;
+constexpr int kSliceMax = 1 << 17;  // slots per CTA: the bitmap's size
+constexpr int kKeysMax = 8192;      // slots whose keys stay in shared memory
+constexpr int kListMax = 2048;      // moves per CTA and round
+
+struct EvictSmem {
+  uint32_t keys[kKeysMax];
+  int hist[kBins];
+  int all[kBins];
+  int list_to[kListMax], list_from[kListMax];
+  int cluster_eq[kMaxCluster], cluster_hole[kMaxCluster], cluster_fill[kMaxCluster];
+  int warp_a[kEvictWarps], warp_b[kEvictWarps];
+  int found[2];
+};
+
+__device__ __forceinline__ int ld_cluster(const int* local, uint32_t rank) {
+  uint32_t ra;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(ra) : "memory");
+  return v;
+}
+
+// Order of weights: larger first, -0 = +0, NaN last (0).
+__device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0u : float_order_key(w + 0.f); }
+
+__global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid_constant__ EvictParams p, int ranks,
+                                                                     int chunks, int esize) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  EvictSmem& s = *reinterpret_cast<EvictSmem*>(raw);
+  uint32_t* bitmap = reinterpret_cast<uint32_t*>(raw + sizeof(EvictSmem));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = ranks > 1 ? (int)cluster_ctarank() : 0;
+  const int item = blockIdx.x / ranks, kvh = item % p.c.kv_heads, lb = item / p.c.kv_heads;
+  const int b = lb % p.c.batch, layer = lb / p.c.batch;
+  const int raw_len = p.c.lens[b], cap = p.c.capacity;
+  const int len = raw_len < 0 || raw_len > cap ? 0 : raw_len;
+  if (item == b * p.c.kv_heads && rank == 0 && tid == 0) p.lens_out[b] = raw_len > cap ? raw_len : min(raw_len, p.budget);
+  const int64_t row_at = (int64_t)item * cap;
+  const float* mass = p.mass + row_at;
+  const int32_t* pos = p.c.pos + row_at;
+  float* mass_out = p.mass_out + row_at;
+  int32_t* pos_out = p.pos_out + row_at;
+  const bool apart = mass != mass_out || pos != pos_out;
+
+  if (len <= p.budget) {  // uniform over the cluster
+    if (apart)
+      for (int t = rank * kEvictThreads + tid; t < len; t += ranks * kEvictThreads) {
+        mass_out[t] = mass[t];
+        pos_out[t] = pos[t];
+      }
+    return;
+  }
+
+  // Slots of this CTA and of each of its warps, both multiples of 32 long.
+  const int per_warp = ((len + ranks * kEvictWarps - 1) / (ranks * kEvictWarps) + 31) / 32 * 32;
+  const int slice = per_warp * kEvictWarps, lo = min(rank * slice, len), hi = min(lo + slice, len);
+  const bool held = slice <= kKeysMax;
+  const long long safe_from = (long long)p.c.next_pos[b] - p.recent;
+  auto key_of = [&](int t) {
+    const int at = pos[t];
+    return at >= safe_from || at < p.sinks ? 0xffffffffu : weight_key(mass[t]);
+  };
+  auto meet = [&] {
+    if (ranks > 1) cluster_sync();
+    else __syncthreads();
+  };
+
+  // The key of the budget-th slot, top bits first.
+  uint32_t prefix = 0;
+  int need = p.budget;  // slots still to take among those with this prefix
+  constexpr int kShift[3] = {21, 10, 0};
+  constexpr int kBits[3] = {11, 11, 10};
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? kShift[0] : pass == 1 ? kShift[1] : kShift[2];
+    const int bits = pass == 2 ? kBits[2] : kBits[0], bins = 1 << bits;
+    for (int i = tid; i < kBins; i += kEvictThreads) s.hist[i] = 0;
+    __syncthreads();
+    for (int t = lo + tid; t < hi; t += kEvictThreads) {
+      uint32_t k;
+      if (held && pass) k = s.keys[t - lo];
+      else {
+        k = key_of(t);
+        if (held) s.keys[t - lo] = k;
+      }
+      if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&s.hist[(k >> shift) & (bins - 1)], 1);
+    }
+    meet();
+    if (ranks > 1) {
+      // Each CTA adds up its share of the bins and hands it to all.
+      const int share = kBins / ranks;
+      for (int i = tid; i < share; i += kEvictThreads) {
+        const int bin = rank * share + i;
+        int sum = 0;
+        for (int r = 0; r < ranks; ++r) sum += ld_cluster(&s.hist[bin], r);
+        for (int r = 0; r < ranks; ++r) st_cluster_u32(&s.all[bin], r, (uint32_t)sum);
+      }
+      meet();
+    }
+    const int* all = ranks > 1 ? s.all : s.hist;
+    // Bins from the top: thread i has bins [top - 8 i, top - 8 (i + 1)).
+    constexpr int kPer = kBins / kEvictThreads;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) mine += all[kBins - 1 - (tid * kPer + i)];
+    int run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += v;
+    }
+    if (lane == 31) s.warp_a[warp] = run;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) run += s.warp_a[w];
+    int before = run - mine;
+    if (before < need && run >= need) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int bin = kBins - 1 - (tid * kPer + i), n = all[bin];
+        if (before < need && before + n >= need) {
+          s.found[0] = bin;
+          s.found[1] = need - before;
+        }
+        before += n;
+      }
+    }
+    __syncthreads();
+    prefix = prefix << bits | (uint32_t)s.found[0];
+    need = s.found[1];
+    __syncthreads();
+  }
+  const uint32_t edge = prefix;  // slots above it are kept, `need` of its equals too
+
+  // Equal slots before each warp's first one, over CTAs and warps in slot order.
+  const int w_lo = min(lo + warp * per_warp, hi), w_hi = min(w_lo + per_warp, hi);
+  auto key_at = [&](int t) { return held ? s.keys[t - lo] : key_of(t); };
+  int eq = 0;
+  for (int t = w_lo + lane; t < w_hi; t += 32) eq += key_at(t) == edge;
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (lane == 0) s.warp_a[warp] = eq;
+  __syncthreads();
+  auto tell = [&](int* slots, int value) {  // value of this CTA into slots[rank] of every CTA
+    if (ranks > 1) {
+      if (tid < ranks) st_cluster_u32(&slots[rank], tid, (uint32_t)value);
+    } else if (tid == 0) {
+      slots[0] = value;
+    }
+  };
+  auto sum_of = [&](const int* v, int n) {
+    int x = 0;
+    for (int i = 0; i < n; ++i) x += v[i];
+    return x;
+  };
+  tell(s.cluster_eq, sum_of(s.warp_a, kEvictWarps));
+  meet();
+  int eq_before = sum_of(s.cluster_eq, rank) + sum_of(s.warp_a, warp);
+
+  // Bitmap of kept slots; holes and fills of each warp.
+  int holes = 0, fills = 0;
+  uint32_t* words = bitmap + warp * (per_warp / 32);
+  for (int t = w_lo; t < w_hi; t += 32) {
+    const bool in = t + lane < w_hi;
+    const uint32_t k = in ? key_at(t + lane) : 0u;
+    const unsigned same = __ballot_sync(0xffffffffu, in && k == edge);
+    const bool keep = in && (k > edge || (k == edge && eq_before + __popc(same & ((1u << lane) - 1)) < need));
+    const unsigned kept = __ballot_sync(0xffffffffu, keep), used = __ballot_sync(0xffffffffu, in);
+    const unsigned below = t + 32 <= p.budget ? 0xffffffffu : t >= p.budget ? 0u : (1u << (p.budget - t)) - 1;
+    eq_before += __popc(same);
+    holes += __popc(~kept & used & below);
+    fills += __popc(kept & ~below);
+    if (lane == 0) words[(t - w_lo) / 32] = kept;
+  }
+  if (lane == 0) {
+    s.warp_b[warp] = holes;
+    s.list_to[warp] = fills;
+  }
+  __syncthreads();
+  const int my_holes = sum_of(s.warp_b, kEvictWarps), my_fills = sum_of(s.list_to, kEvictWarps);
+  const int hole_here = sum_of(s.warp_b, warp), fill_here = sum_of(s.list_to, warp);
+  tell(s.cluster_hole, my_holes);
+  tell(s.cluster_fill, my_fills);
+  meet();
+  const int hole0 = sum_of(s.cluster_hole, rank) + hole_here, fill0 = sum_of(s.cluster_fill, rank) + fill_here;
+  const int moves = sum_of(s.cluster_hole, ranks);
+
+  // Rounds of up to kListMax moves per CTA: move m is CTA m % ranks's.
+  uint8_t* kc = (uint8_t*)p.c.k + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
+  uint8_t* vc = (uint8_t*)p.c.v + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
+  for (int from = 0; from < moves; from += kListMax * ranks) {
+    const int upto = min(moves, from + kListMax * ranks);
+    int h = hole0, f = fill0;
+    for (int t = w_lo; t < w_hi && (h < upto || f < upto); t += 32) {
+      const unsigned kept = words[(t - w_lo) / 32], used = w_hi - t >= 32 ? 0xffffffffu : (1u << (w_hi - t)) - 1;
+      const unsigned below = t + 32 <= p.budget ? 0xffffffffu : t >= p.budget ? 0u : (1u << (p.budget - t)) - 1;
+      const unsigned hm = ~kept & used & below, fm = kept & ~below, lt = (1u << lane) - 1;
+      const int hr = h + __popc(hm & lt), fr = f + __popc(fm & lt);
+      auto put = [&](int* list, int m) {
+        const int at = (m - from) / ranks;
+        if (ranks > 1) st_cluster_u32(&list[at], (uint32_t)((m - from) % ranks), (uint32_t)(t + lane));
+        else list[at] = t + lane;
+      };
+      if ((hm >> lane & 1) && hr >= from && hr < upto) put(s.list_to, hr);
+      if ((fm >> lane & 1) && fr >= from && fr < upto) put(s.list_from, fr);
+      h += __popc(hm);
+      f += __popc(fm);
+    }
+    meet();
+    const int mine = (upto - from - rank + ranks - 1) / ranks;
+    const int work = mine * chunks;
+    for (int i0 = tid; i0 < work; i0 += 4 * kEvictThreads) {
+      uint4 kv[4], vv[4];
+      int64_t to[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kEvictThreads;
+        if (i >= work) continue;
+        const int m = i / chunks, ch = i - m * chunks, src = s.list_from[m], dst = s.list_to[m];
+        kv[u] = *reinterpret_cast<const uint4*>(kc + src * p.c.st * esize + ch * 16);
+        vv[u] = *reinterpret_cast<const uint4*>(vc + src * p.c.st * esize + ch * 16);
+        to[u] = dst * p.c.st * esize + ch * 16;
+        if (ch == 0) {
+          mass_out[dst] = mass[src];
+          pos_out[dst] = pos[src];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i0 + u * kEvictThreads >= work) continue;
+        *reinterpret_cast<uint4*>(kc + to[u]) = kv[u];
+        *reinterpret_cast<uint4*>(vc + to[u]) = vv[u];
+      }
+    }
+    if (from + kListMax * ranks < moves) meet();  // the lists are used again
+  }
+  // Weights and positions that stay in their slots.
+  if (apart)
+    for (int t = w_lo + lane; t < min(w_hi, p.budget); t += 32)
+      if (words[(t - w_lo) / 32] >> ((t - w_lo) & 31) & 1) {
+        mass_out[t] = mass[t];
+        pos_out[t] = pos[t];
+      }
+  if (ranks > 1) cluster_sync();  // no CTA leaves while another may still write its lists
+}
+
+}  // namespace
+
+cudaError_t launch_cache_commit(const CommitParams& p, cudaStream_t s) {
+  const int esize = p.c.dtype == 0 ? 4 : 2, chunks = p.c.head_dim * esize / 16;
+  const long long most = (long long)p.c.layers * p.c.kv_heads * p.path_len * chunks;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  // Four chunks per thread, at most a few waves over the batch.
+  const long long want = (most + 4 * kMoveThreads - 1) / (4 * kMoveThreads);
+  const int waves = max(1, 16 * op_sm_count(dev) / p.c.batch);
+  const dim3 grid((unsigned)min(want, (long long)waves), p.c.batch);
+  switch (chunks) {
+    case 8: cache_commit_kernel<8><<<grid, kMoveThreads, 0, s>>>(p, esize); break;
+    case 16: cache_commit_kernel<16><<<grid, kMoveThreads, 0, s>>>(p, esize); break;
+    default: cache_commit_kernel<32><<<grid, kMoveThreads, 0, s>>>(p, esize); break;
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s) {
+  const int esize = p.c.dtype == 0 ? 4 : 2, chunks = p.c.head_dim * esize / 16;
+  const int items = p.c.layers * p.c.batch * p.c.kv_heads, cap = p.c.capacity;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  // Enough CTAs to fill the GPU twice, with at least 512 slots each.
+  int ranks = 1;
+  while (ranks < kMaxCluster && (cap > ranks * (kSliceMax / 2) || (items * ranks < 2 * op_sm_count(dev) && cap >= ranks * 1024)))
+    ranks *= 2;
+  const int per_warp = ((cap + ranks * kEvictWarps - 1) / (ranks * kEvictWarps) + 31) / 32 * 32;
+  const int bytes = (int)sizeof(EvictSmem) + per_warp * kEvictWarps / 8;
+  e = cudaFuncSetAttribute(cache_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(items * ranks));
+  cfg.blockDim = dim3(kEvictThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, cache_evict_kernel, p, ranks, chunks, esize);
+}
+
+}  // namespace mrtdf

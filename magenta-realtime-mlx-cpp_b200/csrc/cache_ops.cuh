@@ -1,0 +1,89 @@
+// Cache operators on caller-owned device buffers: parameters, limits and
+// launchers. Kernels in cache_attn.cu (tree attention, collected weight) and
+// cache_move.cu (commit, eviction); argument checks in cache_ops.cpp.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace mrtdf {
+
+// Rows of head_dim contiguous elements: row (l, b, h, n) starts at
+// ptr + l * sl + b * sb + h * sh + n * sn elements, 16-byte aligned.
+struct RowsView {
+  const void* ptr;
+  int64_t sl, sb, sh, sn;
+};
+
+struct CacheView {
+  void* k;
+  void* v;
+  int64_t sl, sb, sh, st;
+  int layers, batch, kv_heads, capacity, head_dim, dtype;
+  const int32_t* lens;      // (batch)
+  int32_t* pos;             // (layers, batch, kv_heads, capacity) or NULL: the slot number
+  const int32_t* next_pos;  // (batch) or NULL: lens
+};
+
+constexpr int kOpMaxNodes = 64;
+constexpr int kOpMaxRows = 1024;  // nodes (or path nodes) x query heads of one kv head
+constexpr int kOpMaxBatch = 1024;
+constexpr int kOpMaxCapacity = 1 << 24;
+
+struct TreeParams {
+  CacheView c;
+  RowsView q, k_new, v_new, out;
+  float* lse;              // (batch, heads, nodes) or NULL
+  const int32_t* parents;  // (batch, nodes) or NULL: a chain
+  const float* rel_bias;   // (heads, rel_len) or NULL
+  float* ws;               // partial rows, tree_workspace_floats()
+  int heads, nodes, rel_len;
+  float scale;
+  int grid;       // CTAs of the attention kernel
+  int row_blocks; // blocks of query rows per (sequence, kv head)
+  int stream;     // 1: equal runs of key tiles per CTA, joined afterwards; 0: whole items
+};
+
+struct MassParams {
+  CacheView c;
+  RowsView q, k_new;
+  const float* lse;      // (layers, batch, heads, nodes)
+  const int32_t* path;   // (batch, path_len)
+  const float* rel_bias;
+  const float* mass;     // (layers, batch, kv_heads, capacity)
+  float* mass_out;
+  int heads, nodes, path_len, rel_len;
+  float scale, decay;
+  int grid;
+};
+
+struct CommitParams {
+  CacheView c;
+  RowsView k_new, v_new;
+  const int32_t* path;
+  int32_t* lens_out;
+  int32_t* next_pos_out;
+  int nodes, path_len;
+};
+
+struct EvictParams {
+  CacheView c;
+  const float* mass;
+  float* mass_out;
+  int32_t* pos_out;
+  int32_t* lens_out;
+  int budget, recent, sinks;
+};
+
+// Multiprocessors of a device, asked once (148 when the driver does not say).
+int op_sm_count(int device);
+
+// Chooses the variant and the grid (p.grid, p.row_blocks, p.stream) for a GPU
+// of `sms` multiprocessors; gives the floats of workspace the launch needs.
+cudaError_t plan_tree_attention(TreeParams& p, int sms, size_t* ws_floats);
+cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t s);
+cudaError_t launch_cache_mass(MassParams& p, cudaStream_t s);
+cudaError_t launch_cache_commit(const CommitParams& p, cudaStream_t s);
+cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s);
+
+}  // namespace mrtdf

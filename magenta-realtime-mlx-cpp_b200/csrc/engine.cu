@@ -1791,6 +1791,35 @@ int mrtdf_probe_set_cache(mrtdf_stream* st, int kind, int layer, const float* k,
   });
 }
 
+int mrtdf_stream_cache(mrtdf_stream* st, int kind, int layer, mrtdf_cache* out, int* len) {
+  return guarded([&] {
+    if (!st || !out) throw Error{MRTDF_ERR_INVALID, "stream_cache: NULL argument"};
+    const mrtdf_engine* E = st->eng;
+    const mrtdf_config& c = E->c;
+    if (kind < 0 || kind > 2) throw Error{MRTDF_ERR_RANGE, "stream_cache: cache kind"};
+    const int layers = kind == 1 ? c.num_depth_layers : c.num_temporal_layers;
+    const int cap = kind == 0 ? c.max_frames : kind == 1 ? c.rvq_depth : c.max_encoder_length;
+    if (layer >= layers) throw Error{MRTDF_ERR_RANGE, "stream_cache: layer"};
+    *out = mrtdf_cache{};
+    out->struct_bytes = sizeof(mrtdf_cache);
+    out->stride_t = 64;
+    out->stride_h = (int64_t)cap * 64;
+    out->stride_b = out->stride_h * c.num_heads;
+    out->stride_l = out->stride_b * st->B;
+    out->layers = layer < 0 ? layers : 1;
+    out->batch = st->B;
+    out->kv_heads = c.num_heads;
+    out->capacity = cap;
+    out->head_dim = 64;
+    out->dtype = c.dtype;
+    out->device = E->device;
+    const size_t skip = layer < 0 ? 0 : act_bytes(E, (size_t)out->stride_l * layer);
+    out->k = (uint8_t*)(kind == 0 ? st->tk : kind == 1 ? st->dk : st->ck) + skip;
+    out->v = (uint8_t*)(kind == 0 ? st->tv : kind == 1 ? st->dv : st->cv) + skip;
+    if (len) *len = kind == 0 ? st->t_len : kind == 1 ? st->d_len : st->S;
+  });
+}
+
 int mrtdf_probe_decoder_layer(mrtdf_stream* st, int stack, int layer, int pos, const float* x, float* out) {
   return guarded([&] {
     if (!st || !x || !out) throw Error{MRTDF_ERR_INVALID, "NULL argument"};
