@@ -827,18 +827,14 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
 }
 
 // ---- host --------------------------------------------------------------------------
-template <typename K>
-cudaError_t allow_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <typename T, int D, int WM, bool BIAS>
 cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
-  auto* k = tree_attn_kernel<T, D, WM, BIAS>;
+  constexpr auto K = tree_attn_kernel<T, D, WM, BIAS>;
+  static_assert(TreeSmem<T, D, WM>::kFixed + (2 * kOpMaxBatch + 1) * 4 <= kOpMaxSmem, "fits");
   const int bytes = TreeSmem<T, D, WM>::bytes(p.c.batch);
-  cudaError_t e = allow_smem(k, bytes);
+  cudaError_t e = allow_smem<K>();
   if (e != cudaSuccess) return e;
-  k<<<p.grid, kThreads, bytes, s>>>(p);
+  K<<<p.grid, kThreads, bytes, s>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess || !p.stream) return e;
   cudaLaunchAttribute attr;
@@ -903,9 +899,9 @@ cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t s) {
 namespace {
 template <typename T, int D, bool BIAS>
 cudaError_t mass_run(MassParams& p, cudaStream_t s) {
-  auto* k = cache_mass_kernel<T, D, BIAS>;
+  constexpr auto K = cache_mass_kernel<T, D, BIAS>;
   const int bytes = MassSmem<T, D>::bytes(p.c.batch);
-  cudaError_t e = allow_smem(k, bytes);
+  cudaError_t e = allow_smem<K>();
   if (e != cudaSuccess) return e;
   int dev = 0;
   e = cudaGetDevice(&dev);
@@ -913,7 +909,7 @@ cudaError_t mass_run(MassParams& p, cudaStream_t s) {
   const int per_sm = max(1, min(4, kSmSmem / (bytes + 1024)));
   const long long most = (long long)p.c.batch * p.c.layers * p.c.kv_heads * ((p.c.capacity + p.path_len + kTile - 1) / kTile);
   p.grid = (int)min((long long)op_sm_count(dev) * per_sm, max(1ll, most / 2));
-  k<<<p.grid, kThreads, bytes, s>>>(p);
+  K<<<p.grid, kThreads, bytes, s>>>(p);
   return cudaGetLastError();
 }
 template <typename T, int D>

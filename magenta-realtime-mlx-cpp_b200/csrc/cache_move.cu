@@ -364,7 +364,7 @@ cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s) {
     ranks *= 2;
   const int per_warp = ((cap + ranks * kEvictWarps - 1) / (ranks * kEvictWarps) + 31) / 32 * 32;
   const int bytes = (int)sizeof(EvictSmem) + per_warp * kEvictWarps / 8;
-  e = cudaFuncSetAttribute(cache_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  e = allow_smem<cache_evict_kernel>();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;

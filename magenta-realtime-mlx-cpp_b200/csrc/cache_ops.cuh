@@ -6,7 +6,25 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace mrtdf {
+
+// Lets kernel `K` use up to kOpMaxSmem bytes of dynamic shared memory on the
+// current device; the attribute is set once per device.
+constexpr int kOpMaxSmem = 226 * 1024;
+template <auto K>
+cudaError_t allow_smem() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, kOpMaxSmem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Rows of head_dim contiguous elements: row (l, b, h, n) starts at
 // ptr + l * sl + b * sb + h * sh + n * sn elements, 16-byte aligned.

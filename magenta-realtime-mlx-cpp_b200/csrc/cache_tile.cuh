@@ -4,8 +4,12 @@
 //
 // float32: x = hi + lo + r with hi, lo of 11 significant bits, |r| <= 2^-24 |x|
 // or so; hi hi + hi lo + lo hi leaves out lo lo (2^-24 relative), so a product
-// is as exact as a float32 multiply. Three m16n8k8 issue faster than the
-// 1024 FMAs they replace, which keeps a few rows bound by memory.
+// is as exact as a float32 multiply. The matrix instructions truncate their
+// sums; the small products therefore go to accumulators of their own, and a
+// tile's p . v is summed apart and added with a rounded add (one accumulator
+// through a cache of 1006 rows: 1.1e-6 off against 5.6e-7 for float32 FMAs).
+// Three m16n8k8 issue faster than the 1024 FMAs they replace, which keeps a
+// few rows bound by memory.
 //
 // Shared-memory rows hold head_dim elements in 16-byte chunks; chunk c of row
 // r sits at chunk c ^ swizzle(r). Key rows use r & 7, so the eight rows of one
@@ -139,6 +143,7 @@ template <int D, int NT>
 __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<float, D>& q, uint32_t keys, int lane) {
   using R = Rows<float, D>;
   const int m = lane >> 3, r = lane & 7;
+  float low[NT][4] = {};
 #pragma unroll
   for (int ks = 0; ks < D / 8; ++ks) {
     uint32_t ah[4], al[4];
@@ -152,12 +157,16 @@ __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<float, D>& q,
       for (int i = 0; i < 4; ++i) split_tf32(b[i], bh[i], bl[i]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        mma_tf32(s[2 * jp + h], al, bh[2 * h], bh[2 * h + 1]);
-        mma_tf32(s[2 * jp + h], ah, bl[2 * h], bl[2 * h + 1]);
+        mma_tf32(low[2 * jp + h], al, bh[2 * h], bh[2 * h + 1]);
+        mma_tf32(low[2 * jp + h], ah, bl[2 * h], bl[2 * h + 1]);
         mma_tf32(s[2 * jp + h], ah, bh[2 * h], bh[2 * h + 1]);
       }
     }
   }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[j][e] += low[j][e];
 }
 
 // o[n][.] += p . value rows of the tile at `vals` (p in the layout of s).
@@ -192,26 +201,32 @@ template <int D, int NT>
 __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint32_t vals, int lane, float) {
   using R = Rows<float, D>;
   const int g = lane >> 2, c = lane & 3;
+  // k index c of a product is key 2 c of its eight, c + 4 is key 2 c + 1, so
+  // the scores' layout is the operand's layout.
+  uint32_t ah[NT][4], al[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    // k index c of the product is key 2 c of the eight, c + 4 is key 2 c + 1,
-    // so the scores' layout is the operand's layout.
-    const uint32_t a[4] = {__float_as_uint(p[j][0]), __float_as_uint(p[j][2]), __float_as_uint(p[j][1]),
-                           __float_as_uint(p[j][3])};
-    uint32_t ah[4], al[4];
+    split_tf32(__float_as_uint(p[j][0]), ah[j][0], al[j][0]);
+    split_tf32(__float_as_uint(p[j][2]), ah[j][1], al[j][1]);
+    split_tf32(__float_as_uint(p[j][1]), ah[j][2], al[j][2]);
+    split_tf32(__float_as_uint(p[j][3]), ah[j][3], al[j][3]);
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
+  for (int n = 0; n < D / 8; ++n) {
+    const int chunk = 2 * n + (g >> 2);
+    float add[4] = {};
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      const int chunk = 2 * n + (g >> 2);
+    for (int j = 0; j < NT; ++j) {
       uint32_t bh[2], bl[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         split_tf32(lds32(vals + R::val_at(8 * j + 2 * c + h, chunk) + 4 * (g & 3)), bh[h], bl[h]);
-      mma_tf32(o[n], al, bh[0], bh[1]);
-      mma_tf32(o[n], ah, bl[0], bl[1]);
-      mma_tf32(o[n], ah, bh[0], bh[1]);
+      mma_tf32(add, al[j], bh[0], bh[1]);
+      mma_tf32(add, ah[j], bl[0], bl[1]);
+      mma_tf32(add, ah[j], bh[0], bh[1]);
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] += add[e];
   }
 }
 

@@ -17,6 +17,7 @@
 // The k index of a product is arbitrary as long as both operands agree: lane
 // (g, c) unpacks whole words of 8 columns from its own rows, and x lies in
 // shared memory in the order in which the lanes ask for it.
+#include "cache_ops.cuh"
 #include "cache_tile.cuh"
 #include "q4.cuh"
 
@@ -304,11 +305,11 @@ cudaError_t q4_run(const Q4Params& p, cudaStream_t s) {
   int body = COLS * (chunk * 2 + 64) + chunk / G * COLS * 4;
   const int tail = WK * WR * 16 * (COLS + 1) * 4;
   const int bytes = kWarps * kRing * kStageBytes + (body > tail ? body : tail);
-  auto* k = q4_linear_kernel<T, O, G, NT, WR>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  constexpr auto K = q4_linear_kernel<T, O, G, NT, WR>;
+  cudaError_t e = allow_smem<K>();
   if (e != cudaSuccess) return e;
   const dim3 grid((p.n + WR * 16 - 1) / (WR * 16), (p.m + rows - 1) / rows);
-  k<<<grid, kThreads, bytes, s>>>(p, per, chunk);
+  K<<<grid, kThreads, bytes, s>>>(p, per, chunk);
   return cudaGetLastError();
 }
 

@@ -29,9 +29,6 @@ struct Q4PackParams {
   int n, k, group;
 };
 
-// Multiprocessors of a device, asked once (148 when the driver does not say).
-int op_sm_count(int device);
-
 // dtype (of x, scales, biases) and out_dtype: MRTDF_DTYPE_*.
 cudaError_t launch_q4_linear(const Q4Params& p, int dtype, int out_dtype, cudaStream_t s);
 cudaError_t launch_q4_quantize(const Q4PackParams& p, int dtype, cudaStream_t s);

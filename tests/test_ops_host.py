@@ -4,6 +4,7 @@ here with addresses that are never used. No GPU needed."""
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import pytest
 
@@ -11,12 +12,25 @@ torch = pytest.importorskip("torch")
 
 NOT_A_NUMBER = float("nan")
 
+# sizeof-exact layouts of the C structures (native alignment).
+_CACHE = struct.Struct("@QQQ4q7iQQQ")
+_TREE = struct.Struct("@Q" + "Q4q" * 4 + "QQQQQiiif0Q")
+_MASS = struct.Struct("@Q" + "Q4q" * 2 + "QQQQQiiiiff0Q")
+_COMMIT = struct.Struct("@Q" + "Q4q" * 2 + "QQQii0Q")
+_EVICT = struct.Struct("@QQQQQiii0Q")
+_Q4 = struct.Struct("@QQQQQQqq7i0Q")
+_PACK = struct.Struct("@QQQQQq5i0Q")
+
 
 @pytest.fixture(scope="module")
 def ops(mrtdf):
     import mrtops
 
-    mrtops.lib()
+    L = mrtops.lib()
+    for n in ("tree_attention", "cache_mass", "cache_commit", "cache_evict"):
+        getattr(L, "mrtdf_" + n).argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p]
+    L.mrtdf_tree_attention_workspace.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]
+    L.mrtdf_q4_linear.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
     return mrtops
 
 
@@ -29,26 +43,26 @@ class Call:
 
     def __init__(self, ops):
         self.ops = ops
-        self.cache = dict(size=ops._CACHE.size, k=256, v=256, sl=65536, sb=32768, sh=8192, st=64, layers=1, batch=2,
+        self.cache = dict(size=_CACHE.size, k=256, v=256, sl=65536, sb=32768, sh=8192, st=64, layers=1, batch=2,
                           kv_heads=2, capacity=128, head_dim=64, dtype=1, device=0, lens=256, pos=0, next_pos=0)
-        self.tree = dict(size=ops._TREE.size, q=rows(), k_new=rows(), v_new=rows(), out=rows(), lse=0, parents=0, rel_bias=0,
+        self.tree = dict(size=_TREE.size, q=rows(), k_new=rows(), v_new=rows(), out=rows(), lse=0, parents=0, rel_bias=0,
                          workspace=0, workspace_bytes=0, heads=4, nodes=8, rel_len=0, scale=1.0)
-        self.mass = dict(size=ops._MASS.size, q=rows(), k_new=rows(), lse=256, path=256, rel_bias=0, mass=256, mass_out=256,
+        self.mass = dict(size=_MASS.size, q=rows(), k_new=rows(), lse=256, path=256, rel_bias=0, mass=256, mass_out=256,
                          heads=4, nodes=8, path_len=4, rel_len=0, scale=1.0, decay=1.0)
-        self.commit = dict(size=ops._COMMIT.size, k_new=rows(), v_new=rows(), path=256, lens_out=512, next_pos_out=0, nodes=8,
+        self.commit = dict(size=_COMMIT.size, k_new=rows(), v_new=rows(), path=256, lens_out=512, next_pos_out=0, nodes=8,
                            path_len=4)
-        self.evict = dict(size=ops._EVICT.size, mass=256, mass_out=256, pos_out=256, lens_out=512, budget=64, recent=8, sinks=1)
-        self.q4 = dict(size=ops._Q4.size, x=256, packed=256, scales=256, biases=256, out=256, x_stride=128, out_stride=64, m=2,
+        self.evict = dict(size=_EVICT.size, mass=256, mass_out=256, pos_out=256, lens_out=512, budget=64, recent=8, sinks=1)
+        self.q4 = dict(size=_Q4.size, x=256, packed=256, scales=256, biases=256, out=256, x_stride=128, out_stride=64, m=2,
                        n=64, k=128, group=32, dtype=1, out_dtype=1, device=0)
-        self.pack = dict(size=ops._PACK.size, w=256, packed=256, scales=256, biases=256, w_stride=128, n=4, k=128, group=32,
+        self.pack = dict(size=_PACK.size, w=256, packed=256, scales=256, biases=256, w_stride=128, n=4, k=128, group=32,
                          dtype=1, device=0)
 
     def bytes(self, what):
         flat = []
         for v in getattr(self, what).values():
             flat += list(v) if isinstance(v, tuple) else [v]
-        return getattr(self.ops, {"cache": "_CACHE", "tree": "_TREE", "mass": "_MASS", "commit": "_COMMIT", "evict": "_EVICT",
-                                  "q4": "_Q4", "pack": "_PACK"}[what]).pack(*flat)
+        return {"cache": _CACHE, "tree": _TREE, "mass": _MASS, "commit": _COMMIT, "evict": _EVICT, "q4": _Q4,
+                "pack": _PACK}[what].pack(*flat)
 
     def run(self, what):
         L = self.ops.lib()
@@ -121,7 +135,7 @@ def test_null_structures(ops):
     assert L.mrtdf_cache_evict(c.bytes("cache"), None, None) == 1
     assert L.mrtdf_q4_linear(None, None) == 1 and L.mrtdf_q4_quantize(None, None) == 1
     assert L.mrtdf_tree_attention_workspace(c.bytes("cache"), c.bytes("tree"), None) == 1
-    assert L.mrtdf_stream_cache(None, 0, 0, ctypes.create_string_buffer(ops._CACHE.size), None) == 1
+    assert L.mrtdf_stream_cache(None, 0, 0, ctypes.create_string_buffer(_CACHE.size), None) == 1
 
 
 def test_attention_takes_one_layer(ops):
