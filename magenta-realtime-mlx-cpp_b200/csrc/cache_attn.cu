@@ -37,7 +37,7 @@ __device__ __forceinline__ int tiles_of(int len, int extra) { return (max(len, 0
 
 // lens[b] and first[b] = tiles of all items before sequence b's, for b <= B.
 // All 128 threads; ends with a barrier.
-__device__ void build_schedule(const CacheView& c, int layers, int batch, int items, int extra, int* lens, int* first) {
+__device__ void build_schedule(const CacheView& c, int batch, int items, int extra, int* lens, int* first) {
   __shared__ int warp_sum[kThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, per = (batch + kThreads - 1) / kThreads;
   int sum = 0;
@@ -70,10 +70,11 @@ __device__ void build_schedule(const CacheView& c, int layers, int batch, int it
   __syncthreads();
 }
 
-// Position in the list of tiles: sequence-major, then item, then tile.
+// Position in the list of tiles: sequence-major, then outer, inner (an item is
+// one pair of them), then tile.
 struct Cursor {
-  int w, b, item, tile, tiles, len;
-  __device__ __forceinline__ void seek(int at, const int* lens, const int* first, int batch, int items, int extra) {
+  int w, b, outer, inner, tile, tiles, len;
+  __device__ __forceinline__ void seek(int at, const int* lens, const int* first, int batch, int inners, int extra) {
     w = at;
     int lo = 0, hi = batch - 1;
     while (lo < hi) {
@@ -84,20 +85,27 @@ struct Cursor {
     b = lo;
     len = lens[b];
     tiles = tiles_of(len, extra);
-    const int rem = at - first[b];
-    item = rem / tiles;
+    const int rem = at - first[b], item = rem / tiles;
     tile = rem - item * tiles;
+    outer = item / inners;
+    inner = item - outer * inners;
   }
-  __device__ __forceinline__ void next(const int* lens, int batch, int items, int extra) {
+  // True when the next tile is another item's.
+  __device__ __forceinline__ bool next(const int* lens, int batch, int outers, int inners, int extra) {
     ++w;
-    if (++tile < tiles) return;
+    if (++tile < tiles) return false;
     tile = 0;
-    if (++item < items) return;
-    item = 0;
-    if (++b < batch) {
-      len = lens[b];
-      tiles = tiles_of(len, extra);
+    if (++inner == inners) {
+      inner = 0;
+      if (++outer == outers) {
+        outer = 0;
+        if (++b < batch) {
+          len = lens[b];
+          tiles = tiles_of(len, extra);
+        }
+      }
     }
+    return true;
   }
 };
 
@@ -166,12 +174,12 @@ __device__ __forceinline__ bool nonfinite(uint32_t w, float) { return (w & 0x7f8
 // Columns 8 n + 2 c, + 1 of value row `row`.
 template <int D>
 __device__ __forceinline__ float2 val2(uint32_t vals, int row, int n, int c, __nv_bfloat16) {
-  const uint32_t w = lds32(vals + Rows<__nv_bfloat16, D>::val_at(row, n) + 4 * c);
+  const uint32_t w = lds32(vals + Rows<__nv_bfloat16, D>::at(row, n) + 4 * c);
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 template <int D>
 __device__ __forceinline__ float2 val2(uint32_t vals, int row, int n, int c, float) {
-  const uint32_t at = vals + Rows<float, D>::val_at(row, 2 * n + (c >> 1)) + 8 * (c & 1);
+  const uint32_t at = vals + Rows<float, D>::at(row, 2 * n + (c >> 1)) + 8 * (c & 1);
   return make_float2(__uint_as_float(lds32(at)), __uint_as_float(lds32(at + 4)));
 }
 
@@ -195,11 +203,25 @@ struct TreeSmem {
   static int bytes(int batch) { return kFixed + (2 * batch + 1) * 4; }
 };
 
-template <typename T, int D, int WM, bool BIAS>
-__global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_constant__ TreeParams p) {
+// HALF: at most eight rows, so lanes' rows g + 8 do not exist. CTAs per SM
+// follow the shared memory (56 KB: four of them, three with a bias, whose
+// positions take the registers of the fourth).
+template <typename T, int D, bool BIAS>
+constexpr int tree_ctas() {
+  return sizeof(T) * D == 128 ? (BIAS ? 3 : 4) : sizeof(T) * D == 256 ? 2 : 1;
+}
+template <typename T, int D, int WM, bool BIAS, bool HALF>
+__global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_kernel(const __grid_constant__ TreeParams p) {
   using R = Rows<T, D>;
   using S = TreeSmem<T, D, WM>;
   constexpr int WK = 4 / WM, KT = 16 * WM, NT = KT / 8, MB = 16 * WM, ND = D / 8;
+  constexpr int ROWS = HALF ? 2 : 4;  // a lane's scores of eight keys
+  // bf16 scores without a bias are kept in powers of two (one multiply and one
+  // add per weight). The others stay in natural units: a bias may be the
+  // lowest float32, and float32 weights keep the last bits of x - m.
+  constexpr bool POW2 = !BIAS && sizeof(T) == 2;
+  const float unit = POW2 ? p.scale * kLog2e : p.scale;
+  auto weight = [](float x) { return ex2(POW2 ? x : x * kLog2e); };
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* scratch = smem + S::kRing;
   float4* stat = reinterpret_cast<float4*>(scratch + S::kScratch);
@@ -211,9 +233,9 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, group = warp / WM;
   const int g = lane >> 2, c = lane & 3, gt = wm * 32 + lane;
   unsigned long long* seen = seen_all + warp * kOpMaxNodes;
-  const int batch = p.c.batch, items = p.c.kv_heads * p.row_blocks, nodes = p.nodes;
+  const int batch = p.c.batch, blocks = p.row_blocks, items = p.c.kv_heads * blocks, nodes = p.nodes;
   const int heads_per = p.heads / p.c.kv_heads, rows = heads_per * nodes;
-  build_schedule(p.c, 1, batch, items, nodes, lens, first);
+  build_schedule(p.c, batch, items, nodes, lens, first);
 
   // This CTA's run of tiles.
   const int total = first[batch];
@@ -245,45 +267,59 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
   const T* kn = reinterpret_cast<const T*>(p.k_new.ptr);
   const T* vn = reinterpret_cast<const T*>(p.v_new.ptr);
 
-  // Group's keys of the tile at `cur` into ring stage `st`.
-  auto fetch = [&](const Cursor& cur, int st) {
-    const int kvh = cur.item / p.row_blocks, len = max(cur.len, 0), key0 = cur.tile * kTile + group * KT;
-    const T* kb = kc + cur.b * p.c.sb + kvh * p.c.sh;
-    const T* vb = vc + cur.b * p.c.sb + kvh * p.c.sh;
-    const uint32_t kd = ring + st * S::kStageBytes, vd = kd + KT * R::kBytes;
-    constexpr int CH = R::kChunks;
+  // Group's keys of the tile at `ahead` into ring stage `st`. A lane copies one
+  // 16-byte chunk of rows r0, r0 + RS, ...: the rows' swizzle is a constant
+  // apart (r0 < RS), so a chunk costs two 64-bit adds for its sources.
+  constexpr int CH = R::kChunks, RS = WM * 32 / CH, COPIES = KT / RS;
+  const int r0 = gt / CH, ch = gt % CH;
+  const uint32_t x0 = (uint32_t)((ch ^ (r0 & 7)) << 4);
+  const int64_t row_step = (int64_t)RS * p.c.st;
+  Cursor ahead;
+  const T *kb = nullptr, *vb = nullptr;  // this lane's chunk of row 0 of ahead's item
+  auto enter = [&] {
+    const int64_t at = ahead.b * p.c.sb + ahead.outer * p.c.sh + ch * (16 / (int)sizeof(T));
+    kb = kc + at;
+    vb = vc + at;
+  };
+  auto fetch = [&](int st) {
+    const int len = max(ahead.len, 0), key0 = ahead.tile * kTile + group * KT;
+    const uint32_t kd = ring + st * S::kStageBytes + r0 * R::kBytes, vd = kd + KT * R::kBytes;
+    if (key0 + KT <= len) {
+      const int64_t at = (int64_t)(key0 + r0) * p.c.st;
+      const T *ks = kb + at, *vs = vb + at;
 #pragma unroll
-    for (int i = 0; i < D * (int)sizeof(T) / 32; ++i) {
-      const int idx = gt + i * WM * 32, row = idx / CH, ch = idx % CH, j = key0 + row;
-      const T *ks, *vs;
-      if (j < len) {
-        ks = kb + j * p.c.st;
-        vs = vb + j * p.c.st;
-      } else {
-        const int n = min(j - len, nodes - 1);
-        ks = kn + cur.b * p.k_new.sb + kvh * p.k_new.sh + n * p.k_new.sn;
-        vs = vn + cur.b * p.v_new.sb + kvh * p.v_new.sh + n * p.v_new.sn;
+      for (int i = 0; i < COPIES; ++i) {
+        const uint32_t to = i * RS * R::kBytes + (x0 ^ ((i * RS & 7) << 4));
+        cp_async16(kd + to, ks);
+        cp_async16(vd + to, vs);
+        ks += row_step;
+        vs += row_step;
       }
-      const bool on = j < len + nodes;
-      cp_async16_zfill(kd + R::key_at(row, ch), ks + ch * (16 / sizeof(T)), on);
-      cp_async16_zfill(vd + R::val_at(row, ch), vs + ch * (16 / sizeof(T)), on);
+    } else {
+#pragma unroll 2
+      for (int i = 0; i < COPIES; ++i) {
+        const int j = key0 + r0 + i * RS, n = min(j - len, nodes - 1), el = ch * (16 / (int)sizeof(T));
+        const T* ks = j < len ? kb + j * p.c.st : kn + ahead.b * p.k_new.sb + ahead.outer * p.k_new.sh + n * p.k_new.sn + el;
+        const T* vs = j < len ? vb + j * p.c.st : vn + ahead.b * p.v_new.sb + ahead.outer * p.v_new.sh + n * p.v_new.sn + el;
+        const uint32_t to = i * RS * R::kBytes + (x0 ^ ((i * RS & 7) << 4));
+        cp_async16_zfill(kd + to, ks, j < len + nodes);
+        cp_async16_zfill(vd + to, vs, j < len + nodes);
+      }
     }
     if (BIAS && p.c.pos && gt < KT) {
       const int j = key0 + gt;
-      const int32_t* ps = p.c.pos + (int64_t)(cur.b * p.c.kv_heads + kvh) * p.c.capacity;
+      const int32_t* ps = p.c.pos + (int64_t)(ahead.b * p.c.kv_heads + ahead.outer) * p.c.capacity;
       cp_async4_zfill(smem_u32(pos_s + st * kTile + group * KT + gt), ps + min(j, max(len - 1, 0)), j < len);
     }
+    if (ahead.next(lens, batch, p.c.kv_heads, blocks, nodes)) enter();
   };
 
-  Cursor ahead, cur;
-  ahead.seek(w0, lens, first, batch, items, nodes);
-  cur = ahead;
+  ahead.seek(w0, lens, first, batch, blocks, nodes);
+  Cursor cur = ahead;
+  enter();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
-    if (ahead.w < w1) {
-      fetch(ahead, i);
-      ahead.next(lens, batch, items, nodes);
-    }
+    if (ahead.w < w1) fetch(i);
     cp_async_commit();
   }
 
@@ -294,15 +330,12 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
   int at0 = 0, at1 = 0, next = 0, masks_of = -1, first_tile = 0;
   bool fresh = true;
 
-  for (int st = 0, fill = kStages - 1; cur.w < w1; cur.next(lens, batch, items, nodes)) {
+  for (int st = 0, fill = kStages - 1; cur.w < w1; cur.next(lens, batch, p.c.kv_heads, blocks, nodes)) {
     cp_async_wait<kStages - 2>();
     group_sync<WM>(group);
-    if (ahead.w < w1) {
-      fetch(ahead, fill);
-      ahead.next(lens, batch, items, nodes);
-    }
+    if (ahead.w < w1) fetch(fill);
     cp_async_commit();
-    const int len = max(cur.len, 0), kvh = cur.item / p.row_blocks, row0 = (cur.item % p.row_blocks) * MB + wm * 16;
+    const int len = max(cur.len, 0), kvh = cur.outer, row0 = cur.inner * MB + wm * 16;
 
     if (fresh) {  // a new item: its rows, statistics and masks
       fresh = false;
@@ -351,7 +384,7 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] *= p.scale;
+        for (int e = 0; e < ROWS; ++e) s[j][e] *= unit;
 
       const bool tail = key0 + KT > len;
       // Position of this lane's key 8 j + 2 c + e: stored, the slot, or the
@@ -380,17 +413,21 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int d0 = min(max((int)((unsigned)at0 - (unsigned)ps[j][e]), 0), p.rel_len - 1);
-              const int d1 = min(max((int)((unsigned)at1 - (unsigned)ps[j][e]), 0), p.rel_len - 1);
               s[j][e] += __ldg(tab0 + d0);
-              s[j][2 + e] += __ldg(tab1 + d1);
+              if (!HALF) {
+                const int d1 = min(max((int)((unsigned)at1 - (unsigned)ps[j][e]), 0), p.rel_len - 1);
+                s[j][2 + e] += __ldg(tab1 + d1);
+              }
             }
         } else {  // every key is further than the table: its last entry
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             s[j][0] += far0;
             s[j][1] += far0;
-            s[j][2] += far1;
-            s[j][3] += far1;
+            if (!HALF) {
+              s[j][2] += far1;
+              s[j][3] += far1;
+            }
           }
         }
       }
@@ -405,7 +442,7 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
           for (int e = 0; e < 2; ++e) {
             const int key = key0 + 8 * j + 2 * c + e;
             if (!visible(key, see0)) s[j][e] = -INFINITY;
-            if (!visible(key, see1)) s[j][2 + e] = -INFINITY;
+            if (!HALF && !visible(key, see1)) s[j][2 + e] = -INFINITY;
           }
       }
 
@@ -413,19 +450,17 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         x0 = fmaxf(x0, fmaxf(s[j][0], s[j][1]));
-        x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
+        if (!HALF) x1 = fmaxf(x1, fmaxf(s[j][2], s[j][3]));
       }
 #pragma unroll
       for (int i = 1; i < 4; i <<= 1) {
         x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, i));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, i));
+        if (!HALF) x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, i));
       }
-      x0 = fmaxf(x0, m0);
-      x1 = fmaxf(x1, m1);
-      // A row that has seen nothing keeps m = -inf; 0 stands in for it below.
-      const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-        const float f0 = ex2((m0 - u0) * kLog2e), f1 = ex2((m1 - u1) * kLog2e);
+      if (__any_sync(0xffffffffu, x0 > m0 || (!HALF && x1 > m1))) {
+        x0 = fmaxf(x0, m0);
+        x1 = fmaxf(x1, m1);
+        const float f0 = x0 == -INFINITY ? 1.f : weight(m0 - x0), f1 = x1 == -INFINITY ? 1.f : weight(m1 - x1);
         l0 *= f0;
         l1 *= f1;
 #pragma unroll
@@ -438,14 +473,18 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
         m0 = x0;
         m1 = x1;
       }
+      // A row that has seen nothing keeps m = -inf; 0 stands in for it.
+      const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        s[j][0] = ex2((s[j][0] - u0) * kLog2e);
-        s[j][1] = ex2((s[j][1] - u0) * kLog2e);
-        s[j][2] = ex2((s[j][2] - u1) * kLog2e);
-        s[j][3] = ex2((s[j][3] - u1) * kLog2e);
+        s[j][0] = weight(s[j][0] - u0);
+        s[j][1] = weight(s[j][1] - u0);
         l0 += s[j][0] + s[j][1];
-        l1 += s[j][2] + s[j][3];
+        if (!HALF) {
+          s[j][2] = weight(s[j][2] - u1);
+          s[j][3] = weight(s[j][3] - u1);
+          l1 += s[j][2] + s[j][3];
+        }
       }
 
       // 0 x inf: where a drafted value row that some row must not see is not
@@ -480,7 +519,7 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
         }
         __syncwarp();
       } else {
-        pv_tile<D, NT>(o, s, vals, lane, T());
+        pv_tile<D, NT, HALF>(o, s, vals, lane, T());
       }
     }
     st = st + 1 == kStages ? 0 : st + 1;
@@ -511,8 +550,8 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
           const float4 t = stat[slot];
           const float x0 = fmaxf(m0, t.x), x1 = fmaxf(m1, t.y);
           const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
-          const float a0 = ex2((m0 - u0) * kLog2e), a1 = ex2((m1 - u1) * kLog2e);
-          const float b0 = ex2((t.x - u0) * kLog2e), b1 = ex2((t.y - u1) * kLog2e);
+          const float a0 = weight(m0 - u0), a1 = weight(m1 - u1);
+          const float b0 = weight(t.x - u0), b1 = weight(t.y - u1);
           l0 = l0 * a0 + t.z * b0;
           l1 = l1 * a1 + t.w * b1;
           m0 = x0;
@@ -531,6 +570,10 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
     }
     if (group == 0) {
       const bool whole = first_tile == 0 && cur.tile + 1 == cur.tiles;
+      if (POW2) {  // partial rows and lse are in natural units
+        m0 *= kLn2;
+        m1 *= kLn2;
+      }
       if (!see0) {
         m0 = -INFINITY;
         l0 = 0.f;
@@ -541,7 +584,7 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
       }
       if (whole) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < ROWS / 2; ++h) {
           const int r = row0 + g + 8 * h;
           if (r >= rows) continue;
           const int hd = r / nodes, n = r - hd * nodes, head = kvh * heads_per + hd;
@@ -559,7 +602,7 @@ __global__ __launch_bounds__(kThreads) void tree_attn_kernel(const __grid_consta
         // Slot 1: a run that starts an item; slot 0: one that goes on with it.
         float* part = p.ws + (int64_t)(blockIdx.x * 2 + (first_tile == 0)) * MB * (D + 2);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < ROWS / 2; ++h) {
           const int r = wm * 16 + g + 8 * h;
 #pragma unroll
           for (int i = 0; i < ND; ++i)
@@ -581,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_consta
   extern __shared__ __align__(16) int sched[];
   int *lens = sched, *first = sched + p.c.batch;
   const int items = p.c.kv_heads * p.row_blocks, nodes = p.nodes;
-  build_schedule(p.c, 1, p.c.batch, items, nodes, lens, first);
+  build_schedule(p.c, p.c.batch, items, nodes, lens, first);
   const int b = blockIdx.x / items, item = blockIdx.x % items, total = first[p.c.batch];
   const int parts = active(p.grid, total), tiles = tiles_of(lens[b], nodes), w = first[b] + item * tiles;
   const int c0 = owner(w, parts, total), c1 = owner(w + tiles - 1, parts, total);
@@ -651,14 +694,14 @@ __device__ __forceinline__ void q_from_smem(QFrag<__nv_bfloat16, D>& q, uint32_t
   const int m = lane >> 3, r = lane & 7;
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks)
-    ldsm_x4_g(q.a[ks], base + Rows<__nv_bfloat16, D>::key_at((m & 1) * 8 + r, 2 * ks + (m >> 1)));
+    ldsm_x4_g(q.a[ks], base + Rows<__nv_bfloat16, D>::at((m & 1) * 8 + r, 2 * ks + (m >> 1)));
 }
 template <int D>
 __device__ __forceinline__ void q_from_smem(QFrag<float, D>& q, uint32_t base, int lane) {
   const int m = lane >> 3, r = lane & 7;
 #pragma unroll
   for (int ks = 0; ks < D / 8; ++ks)
-    ldsm_x4_g(q.a[ks], base + Rows<float, D>::key_at((m & 1) * 8 + r, 2 * ks + (m >> 1)));
+    ldsm_x4_g(q.a[ks], base + Rows<float, D>::at((m & 1) * 8 + r, 2 * ks + (m >> 1)));
 }
 
 // Nodes of the accepted path: up to the first entry that is not a node after
@@ -689,19 +732,19 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
   int* first = lens + p.c.batch;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-  const int batch = p.c.batch, items = p.c.layers * p.c.kv_heads, extra = p.path_len;
+  const int batch = p.c.batch, kv = p.c.kv_heads, items = p.c.layers * kv, extra = p.path_len;
   const int heads_per = p.heads / p.c.kv_heads;
-  build_schedule(p.c, 1, batch, items, extra, lens, first);
+  build_schedule(p.c, batch, items, extra, lens, first);
   const int total = first[batch], parts = active(p.grid, total);
   if ((int)blockIdx.x >= parts) return;
   const int w0 = share(blockIdx.x, parts, total), w1 = share(blockIdx.x + 1, parts, total);
   const uint32_t ring = smem_u32(smem) + warp * (16 * R::kBytes);
 
   Cursor cur;
-  cur.seek(w0, lens, first, batch, items, extra);
+  cur.seek(w0, lens, first, batch, kv, extra);
   while (cur.w < w1) {
     // One item's run of tiles [t0, t1): layer, sequence, kv head.
-    const int layer = cur.item / p.c.kv_heads, kvh = cur.item % p.c.kv_heads, b = cur.b;
+    const int layer = cur.outer, kvh = cur.inner, b = cur.b;
     const int t0 = cur.tile, t1 = min(cur.tiles, cur.tile + (w1 - cur.w)), len = max(cur.len, 0);
     const bool there = cur.len >= 0;
     __syncthreads();  // the item before is done with the path and the rows
@@ -714,15 +757,28 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
     const T* kn = reinterpret_cast<const T*>(p.k_new.ptr) + layer * p.k_new.sl + b * p.k_new.sb + kvh * p.k_new.sh;
     __syncthreads();
 
+    // As in tree_attn_kernel: a lane copies one chunk of every RS-th row.
+    constexpr int CH = R::kChunks, RS = 32 / CH;
+    const int r0 = lane / CH, ch = lane % CH, el = ch * (16 / (int)sizeof(T));
+    const uint32_t x0 = (uint32_t)((ch ^ (r0 & 7)) << 4);
+    const T* kl = kb + el;
     auto fetch = [&](int tile, int st) {
       const int key0 = tile * kTile + warp * 16;
-      const uint32_t kd = ring + st * S::kStageBytes;
-      constexpr int CH = R::kChunks;
+      const uint32_t kd = ring + st * S::kStageBytes + r0 * R::kBytes;
+      if (key0 + 16 <= len && rows > 0) {
+        const T* ks = kl + (int64_t)(key0 + r0) * p.c.st;
 #pragma unroll
-      for (int i = 0; i < CH / 2; ++i) {
-        const int idx = lane + i * 32, row = idx / CH, ch = idx % CH, j = key0 + row;
-        const T* ks = j < len ? kb + j * p.c.st : kn + path_s[min(j - len, p.path_len - 1)] * p.k_new.sn;
-        cp_async16_zfill(kd + R::key_at(row, ch), ks + ch * (16 / sizeof(T)), rows > 0 && j < len + count);
+        for (int i = 0; i < 16 / RS; ++i) {
+          cp_async16(kd + i * RS * R::kBytes + (x0 ^ ((i * RS & 7) << 4)), ks);
+          ks += RS * p.c.st;
+        }
+      } else {
+#pragma unroll 2
+        for (int i = 0; i < 16 / RS; ++i) {
+          const int j = key0 + r0 + i * RS;
+          const T* ks = j < len ? kl + j * p.c.st : kn + path_s[min(j - len, p.path_len - 1)] * p.k_new.sn + el;
+          cp_async16_zfill(kd + i * RS * R::kBytes + (x0 ^ ((i * RS & 7) << 4)), ks, rows > 0 && j < len + count);
+        }
       }
       if (BIAS && p.c.pos && lane < 16) {
         const int j = key0 + lane;
@@ -743,7 +799,7 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
                                               head * p.q.sh + n * p.q.sn + ch * (16 / sizeof(T)));
           if (ch == 0) lse_s[row] = p.lse[((int64_t)(layer * batch + b) * p.heads + head) * p.nodes + n];
         }
-        *reinterpret_cast<uint4*>(q_s + R::key_at(row, ch)) = v;
+        *reinterpret_cast<uint4*>(q_s + R::at(row, ch)) = v;
       }
       for (int i = 0; i < kStages - 1; ++i) {
         if (t0 + i < t1) fetch(t0 + i, i);
@@ -821,15 +877,15 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
     if (t1 == cur.tiles && cur.w < w1) {
       cur.w -= 1;
       cur.tile = cur.tiles - 1;
-      cur.next(lens, batch, items, extra);
+      cur.next(lens, batch, p.c.layers, kv, extra);
     }
   }
 }
 
 // ---- host --------------------------------------------------------------------------
-template <typename T, int D, int WM, bool BIAS>
+template <typename T, int D, int WM, bool BIAS, bool HALF>
 cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
-  constexpr auto K = tree_attn_kernel<T, D, WM, BIAS>;
+  constexpr auto K = tree_attn_kernel<T, D, WM, BIAS, HALF>;
   static_assert(TreeSmem<T, D, WM>::kFixed + (2 * kOpMaxBatch + 1) * 4 <= kOpMaxSmem, "fits");
   const int bytes = TreeSmem<T, D, WM>::bytes(p.c.batch);
   cudaError_t e = allow_smem<K>();
@@ -850,11 +906,16 @@ cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, p, 16 * WM);
 }
 
+template <typename T, int D, bool BIAS>
+cudaError_t tree_variant(const TreeParams& p, int wm, cudaStream_t s) {
+  if (p.heads / p.c.kv_heads * p.nodes <= 8) return tree_run<T, D, 1, BIAS, true>(p, s);
+  return wm == 1   ? tree_run<T, D, 1, BIAS, false>(p, s)
+         : wm == 2 ? tree_run<T, D, 2, BIAS, false>(p, s)
+                   : tree_run<T, D, 4, BIAS, false>(p, s);
+}
 template <typename T, int D>
 cudaError_t tree_variant(const TreeParams& p, int wm, cudaStream_t s) {
-  if (p.rel_bias)
-    return wm == 1 ? tree_run<T, D, 1, true>(p, s) : wm == 2 ? tree_run<T, D, 2, true>(p, s) : tree_run<T, D, 4, true>(p, s);
-  return wm == 1 ? tree_run<T, D, 1, false>(p, s) : wm == 2 ? tree_run<T, D, 2, false>(p, s) : tree_run<T, D, 4, false>(p, s);
+  return p.rel_bias ? tree_variant<T, D, true>(p, wm, s) : tree_variant<T, D, false>(p, wm, s);
 }
 
 // Warps that share a key range: one per 16 query rows, up to four.
@@ -881,7 +942,7 @@ cudaError_t plan_tree_attention(TreeParams& p, int sms, size_t* ws_floats) {
   const int wm = tree_wm(p), mb = 16 * wm, rows = p.heads / p.c.kv_heads * p.nodes;
   p.row_blocks = (rows + mb - 1) / mb;
   const int items = p.c.batch * p.c.kv_heads * p.row_blocks;
-  const int per_sm = max(1, min(4, kSmSmem / (tree_smem(p, wm) + 1024)));
+  const int per_sm = max(1, min(p.rel_bias && p.c.dtype != 0 ? 3 : 4, kSmSmem / (tree_smem(p, wm) + 1024)));
   const int slots = sms * per_sm, most = (p.c.capacity + p.nodes + kTile - 1) / kTile;
   // Short caches: an item is a few tiles, whole items per CTA need no join.
   p.stream = most > 4;

@@ -89,17 +89,17 @@ constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
 constexpr int kSliceMax = 1 << 17;  // slots per CTA: the bitmap's size
-constexpr int kKeysMax = 8192;      // slots whose keys stay in shared memory
+constexpr int kKeysMax = 16384;     // slots whose keys stay in shared memory
 constexpr int kListMax = 2048;      // moves per CTA and round
 
 struct EvictSmem {
-  uint32_t keys[kKeysMax];
   int hist[kBins];
   int all[kBins];
-  int list_to[kListMax], list_from[kListMax];
   int cluster_eq[kMaxCluster], cluster_hole[kMaxCluster], cluster_fill[kMaxCluster];
-  int warp_a[kEvictWarps], warp_b[kEvictWarps];
+  int warp_a[kEvictWarps], warp_b[kEvictWarps], warp_c[kEvictWarps];
   int found[2];
+  // behind it: list_to[list], list_from[list], bitmap of the slice, keys of
+  // the slice where they fit
 };
 
 __device__ __forceinline__ int ld_cluster(const int* local, uint32_t rank) {
@@ -114,10 +114,14 @@ __device__ __forceinline__ int ld_cluster(const int* local, uint32_t rank) {
 __device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0u : float_order_key(w + 0.f); }
 
 __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid_constant__ EvictParams p, int ranks,
-                                                                     int chunks, int esize) {
+                                                                     int chunks, int esize, int list, int words_max,
+                                                                     int keys_max) {
   extern __shared__ __align__(16) uint8_t raw[];
   EvictSmem& s = *reinterpret_cast<EvictSmem*>(raw);
-  uint32_t* bitmap = reinterpret_cast<uint32_t*>(raw + sizeof(EvictSmem));
+  int* list_to = reinterpret_cast<int*>(raw + sizeof(EvictSmem));
+  int* list_from = list_to + list;
+  uint32_t* bitmap = reinterpret_cast<uint32_t*>(list_from + list);
+  uint32_t* keys = bitmap + words_max;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = ranks > 1 ? (int)cluster_ctarank() : 0;
   const int item = blockIdx.x / ranks, kvh = item % p.c.kv_heads, lb = item / p.c.kv_heads;
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
   // Slots of this CTA and of each of its warps, both multiples of 32 long.
   const int per_warp = ((len + ranks * kEvictWarps - 1) / (ranks * kEvictWarps) + 31) / 32 * 32;
   const int slice = per_warp * kEvictWarps, lo = min(rank * slice, len), hi = min(lo + slice, len);
-  const bool held = slice <= kKeysMax;
+  const bool held = slice <= keys_max;
   const long long safe_from = (long long)p.c.next_pos[b] - p.recent;
   auto key_of = [&](int t) {
     const int at = pos[t];
@@ -166,14 +170,22 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
     const int bits = pass == 2 ? kBits[2] : kBits[0], bins = 1 << bits;
     for (int i = tid; i < kBins; i += kEvictThreads) s.hist[i] = 0;
     __syncthreads();
-    for (int t = lo + tid; t < hi; t += kEvictThreads) {
-      uint32_t k;
-      if (held && pass) k = s.keys[t - lo];
-      else {
-        k = key_of(t);
-        if (held) s.keys[t - lo] = k;
+    constexpr int U = 8;  // keys in flight per thread
+    for (int t0 = lo + tid; t0 < hi; t0 += U * kEvictThreads) {
+      uint32_t k[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kEvictThreads;
+        if (t >= hi) break;
+        k[u] = held && pass ? keys[t - lo] : key_of(t);
       }
-      if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&s.hist[(k >> shift) & (bins - 1)], 1);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kEvictThreads;
+        if (t >= hi) break;
+        if (held && pass == 0) keys[t - lo] = k[u];
+        if (pass == 0 || (k[u] >> (shift + bits)) == prefix) atomicAdd(&s.hist[(k[u] >> shift) & (bins - 1)], 1);
+      }
     }
     meet();
     if (ranks > 1) {
@@ -223,7 +235,7 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
 
   // Equal slots before each warp's first one, over CTAs and warps in slot order.
   const int w_lo = min(lo + warp * per_warp, hi), w_hi = min(w_lo + per_warp, hi);
-  auto key_at = [&](int t) { return held ? s.keys[t - lo] : key_of(t); };
+  auto key_at = [&](int t) { return held ? keys[t - lo] : key_of(t); };
   int eq = 0;
   for (int t = w_lo + lane; t < w_hi; t += 32) eq += key_at(t) == edge;
   eq = __reduce_add_sync(0xffffffffu, eq);
@@ -262,35 +274,35 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
   }
   if (lane == 0) {
     s.warp_b[warp] = holes;
-    s.list_to[warp] = fills;
+    s.warp_c[warp] = fills;
   }
   __syncthreads();
-  const int my_holes = sum_of(s.warp_b, kEvictWarps), my_fills = sum_of(s.list_to, kEvictWarps);
-  const int hole_here = sum_of(s.warp_b, warp), fill_here = sum_of(s.list_to, warp);
+  const int my_holes = sum_of(s.warp_b, kEvictWarps), my_fills = sum_of(s.warp_c, kEvictWarps);
+  const int hole_here = sum_of(s.warp_b, warp), fill_here = sum_of(s.warp_c, warp);
   tell(s.cluster_hole, my_holes);
   tell(s.cluster_fill, my_fills);
   meet();
   const int hole0 = sum_of(s.cluster_hole, rank) + hole_here, fill0 = sum_of(s.cluster_fill, rank) + fill_here;
   const int moves = sum_of(s.cluster_hole, ranks);
 
-  // Rounds of up to kListMax moves per CTA: move m is CTA m % ranks's.
+  // Rounds of up to `list` moves per CTA: move m is CTA m % ranks's.
   uint8_t* kc = (uint8_t*)p.c.k + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
   uint8_t* vc = (uint8_t*)p.c.v + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
-  for (int from = 0; from < moves; from += kListMax * ranks) {
-    const int upto = min(moves, from + kListMax * ranks);
+  for (int from = 0; from < moves; from += list * ranks) {
+    const int upto = min(moves, from + list * ranks);
     int h = hole0, f = fill0;
     for (int t = w_lo; t < w_hi && (h < upto || f < upto); t += 32) {
       const unsigned kept = words[(t - w_lo) / 32], used = w_hi - t >= 32 ? 0xffffffffu : (1u << (w_hi - t)) - 1;
       const unsigned below = t + 32 <= p.budget ? 0xffffffffu : t >= p.budget ? 0u : (1u << (p.budget - t)) - 1;
       const unsigned hm = ~kept & used & below, fm = kept & ~below, lt = (1u << lane) - 1;
       const int hr = h + __popc(hm & lt), fr = f + __popc(fm & lt);
-      auto put = [&](int* list, int m) {
+      auto put = [&](int* to, int m) {
         const int at = (m - from) / ranks;
-        if (ranks > 1) st_cluster_u32(&list[at], (uint32_t)((m - from) % ranks), (uint32_t)(t + lane));
-        else list[at] = t + lane;
+        if (ranks > 1) st_cluster_u32(&to[at], (uint32_t)((m - from) % ranks), (uint32_t)(t + lane));
+        else to[at] = t + lane;
       };
-      if ((hm >> lane & 1) && hr >= from && hr < upto) put(s.list_to, hr);
-      if ((fm >> lane & 1) && fr >= from && fr < upto) put(s.list_from, fr);
+      if ((hm >> lane & 1) && hr >= from && hr < upto) put(list_to, hr);
+      if ((fm >> lane & 1) && fr >= from && fr < upto) put(list_from, fr);
       h += __popc(hm);
       f += __popc(fm);
     }
@@ -304,7 +316,7 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * kEvictThreads;
         if (i >= work) continue;
-        const int m = i / chunks, ch = i - m * chunks, src = s.list_from[m], dst = s.list_to[m];
+        const int m = i / chunks, ch = i - m * chunks, src = list_from[m], dst = list_to[m];
         kv[u] = *reinterpret_cast<const uint4*>(kc + src * p.c.st * esize + ch * 16);
         vv[u] = *reinterpret_cast<const uint4*>(vc + src * p.c.st * esize + ch * 16);
         to[u] = dst * p.c.st * esize + ch * 16;
@@ -320,7 +332,7 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
         *reinterpret_cast<uint4*>(vc + to[u]) = vv[u];
       }
     }
-    if (from + kListMax * ranks < moves) meet();  // the lists are used again
+    if (from + list * ranks < moves) meet();  // the lists are used again
   }
   // Weights and positions that stay in their slots.
   if (apart)
@@ -363,7 +375,9 @@ cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s) {
   while (ranks < kMaxCluster && (cap > ranks * (kSliceMax / 2) || (items * ranks < 2 * op_sm_count(dev) && cap >= ranks * 1024)))
     ranks *= 2;
   const int per_warp = ((cap + ranks * kEvictWarps - 1) / (ranks * kEvictWarps) + 31) / 32 * 32;
-  const int bytes = (int)sizeof(EvictSmem) + per_warp * kEvictWarps / 8;
+  const int slice = per_warp * kEvictWarps, words = slice / 32, keys = slice <= kKeysMax ? slice : 0;
+  const int list = min(kListMax, (min(p.budget, cap) + ranks - 1) / ranks);
+  const int bytes = (int)sizeof(EvictSmem) + (2 * list + words + keys) * 4;
   e = allow_smem<cache_evict_kernel>();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr;
@@ -377,7 +391,7 @@ cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, cache_evict_kernel, p, ranks, chunks, esize);
+  return cudaLaunchKernelEx(&cfg, cache_evict_kernel, p, ranks, chunks, esize, list, words, keys);
 }
 
 }  // namespace mrtdf

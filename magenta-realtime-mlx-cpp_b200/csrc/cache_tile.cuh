@@ -12,11 +12,9 @@
 // few rows bound by memory.
 //
 // Shared-memory rows hold head_dim elements in 16-byte chunks; chunk c of row
-// r sits at chunk c ^ swizzle(r). Key rows use r & 7, so the eight rows of one
-// ldmatrix lie in different banks. bf16 value rows are read by ldmatrix.trans
-// and use the same. float32 value rows are read one word per lane, lane
-// (g, c) at row 2 c (+1), column g: r & 6 puts the four rows' chunk pairs in
-// different banks.
+// r sits at chunk c ^ (r & 7), so the eight rows of one ldmatrix lie in
+// different banks; so do the four rows 2 c (+1) of which float32 value rows are
+// read a word per lane.
 #pragma once
 
 #include "common.cuh"
@@ -25,6 +23,7 @@
 namespace mrtdf {
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -32,6 +31,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
@@ -77,12 +79,8 @@ template <typename T, int D>
 struct Rows {
   static constexpr int kChunks = D * (int)sizeof(T) / 16;  // 16-byte chunks per row
   static constexpr int kBytes = D * (int)sizeof(T);
-  static constexpr bool kF32 = sizeof(T) == 4;
-  __device__ __forceinline__ static uint32_t key_at(int row, int chunk) {
+  __device__ __forceinline__ static uint32_t at(int row, int chunk) {
     return (uint32_t)(row * kBytes + ((chunk ^ (row & 7)) << 4));
-  }
-  __device__ __forceinline__ static uint32_t val_at(int row, int chunk) {
-    return (uint32_t)(row * kBytes + ((chunk ^ (row & (kF32 ? 6 : 7))) << 4));
   }
 };
 
@@ -132,7 +130,7 @@ __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<__nv_bfloat16
 #pragma unroll
     for (int jp = 0; jp < NT / 2; ++jp) {
       uint32_t b[4];
-      ldsm_x4_g(b, keys + R::key_at(16 * jp + (m >> 1) * 8 + r, 2 * ks + (m & 1)));
+      ldsm_x4_g(b, keys + R::at(16 * jp + (m >> 1) * 8 + r, 2 * ks + (m & 1)));
       mma_m16n8k16(s[2 * jp], q.a[ks], b[0], b[1]);
       mma_m16n8k16(s[2 * jp + 1], q.a[ks], b[2], b[3]);
     }
@@ -152,7 +150,7 @@ __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<float, D>& q,
 #pragma unroll
     for (int jp = 0; jp < NT / 2; ++jp) {
       uint32_t b[4], bh[4], bl[4];
-      ldsm_x4_g(b, keys + R::key_at(16 * jp + (m >> 1) * 8 + r, 2 * ks + (m & 1)));
+      ldsm_x4_g(b, keys + R::at(16 * jp + (m >> 1) * 8 + r, 2 * ks + (m & 1)));
 #pragma unroll
       for (int i = 0; i < 4; ++i) split_tf32(b[i], bh[i], bl[i]);
 #pragma unroll
@@ -172,7 +170,8 @@ __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<float, D>& q,
 // o[n][.] += p . value rows of the tile at `vals` (p in the layout of s).
 // bf16: p goes in as two bf16 parts, hi + lo, so that the weights keep 16
 // bits; the second product is free while the tile waits for memory.
-template <int D, int NT>
+// HALF: rows g + 8 do not exist, their weights are taken as zero.
+template <int D, int NT, bool HALF>
 __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint32_t vals, int lane, __nv_bfloat16) {
   using R = Rows<__nv_bfloat16, D>;
   const int m = lane >> 3, r = lane & 7;
@@ -181,6 +180,10 @@ __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (HALF && (i & 1)) {
+        hi[i] = lo[i] = 0u;
+        continue;
+      }
       const float x = p[2 * jp + (i >> 1)][2 * (i & 1)], y = p[2 * jp + (i >> 1)][2 * (i & 1) + 1];
       hi[i] = pack_bf16(x, y);
       lo[i] = pack_bf16(x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u));
@@ -188,7 +191,7 @@ __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint
 #pragma unroll
     for (int np = 0; np < D / 16; ++np) {
       uint32_t b[4];
-      ldsm_x4_t(b, vals + R::val_at(16 * jp + (m & 1) * 8 + r, 2 * np + (m >> 1)));
+      ldsm_x4_t(b, vals + R::at(16 * jp + (m & 1) * 8 + r, 2 * np + (m >> 1)));
       mma_m16n8k16(o[2 * np], hi, b[0], b[1]);
       mma_m16n8k16(o[2 * np + 1], hi, b[2], b[3]);
       mma_m16n8k16(o[2 * np], lo, b[0], b[1]);
@@ -197,7 +200,7 @@ __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint
   }
 }
 
-template <int D, int NT>
+template <int D, int NT, bool HALF>
 __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint32_t vals, int lane, float) {
   using R = Rows<float, D>;
   const int g = lane >> 2, c = lane & 3;
@@ -207,9 +210,9 @@ __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     split_tf32(__float_as_uint(p[j][0]), ah[j][0], al[j][0]);
-    split_tf32(__float_as_uint(p[j][2]), ah[j][1], al[j][1]);
+    split_tf32(HALF ? 0u : __float_as_uint(p[j][2]), ah[j][1], al[j][1]);
     split_tf32(__float_as_uint(p[j][1]), ah[j][2], al[j][2]);
-    split_tf32(__float_as_uint(p[j][3]), ah[j][3], al[j][3]);
+    split_tf32(HALF ? 0u : __float_as_uint(p[j][3]), ah[j][3], al[j][3]);
   }
 #pragma unroll
   for (int n = 0; n < D / 8; ++n) {
@@ -220,7 +223,7 @@ __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint
       uint32_t bh[2], bl[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        split_tf32(lds32(vals + R::val_at(8 * j + 2 * c + h, chunk) + 4 * (g & 3)), bh[h], bl[h]);
+        split_tf32(lds32(vals + R::at(8 * j + 2 * c + h, chunk) + 4 * (g & 3)), bh[h], bl[h]);
       mma_tf32(add, al[j], bh[0], bh[1]);
       mma_tf32(add, ah[j], bl[0], bl[1]);
       mma_tf32(add, ah[j], bh[0], bh[1]);
