@@ -79,11 +79,13 @@ __global__ __launch_bounds__(kMoveThreads) void cache_commit_kernel(const __grid
 // slots [r * slice, (r + 1) * slice). Kept are the `budget` slots that come
 // first by (protected, weight from the largest, slot from the lowest); a
 // weight that is NaN comes last. The threshold is found by three histogram
-// passes over an order-preserving 32-bit key (11, 11, 10 bits) whose counts
-// the cluster adds up over distributed shared memory. Kept slots go into a
-// bitmap; the i-th evicted slot below the budget (a hole) takes the i-th kept
-// slot at or above it. Holes are below the budget and sources at or above it,
-// so every row moves once, in place, in any order.
+// passes over an order-preserving 32-bit key (11, 11, 10 bits); a CTA adds its
+// occupied bins to every CTA's totals over distributed shared memory, one
+// cluster barrier per pass. Short caches (512 slots) count for each slot the
+// slots before it instead. Kept slots go into a bitmap; the i-th evicted slot
+// below the budget (a hole) takes the i-th kept slot at or above it. Holes are
+// below the budget and sources at or above it, so every row moves once, in
+// place, in any order.
 constexpr int kEvictThreads = 256;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kBins = 2048;
@@ -91,42 +93,42 @@ constexpr int kMaxCluster = 8;
 constexpr int kSliceMax = 1 << 17;  // slots per CTA: the bitmap's size
 constexpr int kKeysMax = 16384;     // slots whose keys stay in shared memory
 constexpr int kListMax = 2048;      // moves per CTA and round
+constexpr int kCountMax = 512;      // slots ranked by counting
 
-struct EvictSmem {
+struct alignas(16) EvictSmem {
   int hist[kBins];
-  int all[kBins];
+  int all[2][kBins];  // totals over the cluster; the passes take turns
   int cluster_eq[kMaxCluster], cluster_hole[kMaxCluster], cluster_fill[kMaxCluster];
   int warp_a[kEvictWarps], warp_b[kEvictWarps], warp_c[kEvictWarps];
-  int found[2];
-  // behind it: list_to[list], list_from[list], bitmap of the slice, keys of
-  // the slice where they fit
+  int found[3];
+  // behind it: keys of the slice where they fit (read 16 bytes at a time),
+  // bitmap of the slice, list_to[list], list_from[list]
 };
 
-__device__ __forceinline__ int ld_cluster(const int* local, uint32_t rank) {
+__device__ __forceinline__ void add_cluster(int* local, uint32_t rank, int v) {
   uint32_t ra;
-  int v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(local)), "r"(rank));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(ra) : "memory");
-  return v;
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(ra), "r"(v) : "memory");
 }
 
 // Order of weights: larger first, -0 = +0, NaN last (0).
 __device__ __forceinline__ uint32_t weight_key(float w) { return w != w ? 0u : float_order_key(w + 0.f); }
 
-__global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid_constant__ EvictParams p, int ranks,
-                                                                     int chunks, int esize, int list, int words_max,
-                                                                     int keys_max) {
+__global__ __launch_bounds__(kEvictThreads, 4) void cache_evict_kernel(const __grid_constant__ EvictParams p, int ranks,
+                                                                        int chunks, int esize, int list, int words_max,
+                                                                        int keys_max) {
   extern __shared__ __align__(16) uint8_t raw[];
   EvictSmem& s = *reinterpret_cast<EvictSmem*>(raw);
-  int* list_to = reinterpret_cast<int*>(raw + sizeof(EvictSmem));
+  uint32_t* keys = reinterpret_cast<uint32_t*>(raw + sizeof(EvictSmem));
+  uint32_t* bitmap = keys + keys_max;
+  int* list_to = reinterpret_cast<int*>(bitmap + words_max);
   int* list_from = list_to + list;
-  uint32_t* bitmap = reinterpret_cast<uint32_t*>(list_from + list);
-  uint32_t* keys = bitmap + words_max;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = ranks > 1 ? (int)cluster_ctarank() : 0;
   const int item = blockIdx.x / ranks, kvh = item % p.c.kv_heads, lb = item / p.c.kv_heads;
   const int b = lb % p.c.batch, layer = lb / p.c.batch;
   const int raw_len = p.c.lens[b], cap = p.c.capacity;
+  const long long safe_from = (long long)p.c.next_pos[b] - p.recent;
   const int len = raw_len < 0 || raw_len > cap ? 0 : raw_len;
   if (item == b * p.c.kv_heads && rank == 0 && tid == 0) p.lens_out[b] = raw_len > cap ? raw_len : min(raw_len, p.budget);
   const int64_t row_at = (int64_t)item * cap;
@@ -148,99 +150,109 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
   // Slots of this CTA and of each of its warps, both multiples of 32 long.
   const int per_warp = ((len + ranks * kEvictWarps - 1) / (ranks * kEvictWarps) + 31) / 32 * 32;
   const int slice = per_warp * kEvictWarps, lo = min(rank * slice, len), hi = min(lo + slice, len);
-  const bool held = slice <= keys_max;
-  const long long safe_from = (long long)p.c.next_pos[b] - p.recent;
-  auto key_of = [&](int t) {
-    const int at = pos[t];
-    return at >= safe_from || at < p.sinks ? 0xffffffffu : weight_key(mass[t]);
-  };
+  const bool held = slice <= keys_max, counted = ranks == 1 && len <= kCountMax && held;
+  auto key_of = [&](int at, float w) { return at >= safe_from || at < p.sinks ? 0xffffffffu : weight_key(w); };
   auto meet = [&] {
     if (ranks > 1) cluster_sync();
     else __syncthreads();
   };
 
-  // The key of the budget-th slot, top bits first.
-  uint32_t prefix = 0;
-  int need = p.budget;  // slots still to take among those with this prefix
-  constexpr int kShift[3] = {21, 10, 0};
-  constexpr int kBits[3] = {11, 11, 10};
+  uint32_t edge = 0;      // slots above this key are kept,
+  int need = p.budget;    // `need` of its equals too (the lowest ones),
+  bool some = false;      // which are not all of them
+  if (counted) {
+    for (int t = tid; t < slice; t += kEvictThreads) keys[t] = t < len ? key_of(pos[t], mass[t]) : 0u;
+    __syncthreads();
+  } else {
+    for (int i = tid; i < kBins; i += kEvictThreads) s.hist[i] = s.all[0][i] = s.all[1][i] = 0;
+    meet();  // every CTA's totals are zero
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? kShift[0] : pass == 1 ? kShift[1] : kShift[2];
-    const int bits = pass == 2 ? kBits[2] : kBits[0], bins = 1 << bits;
-    for (int i = tid; i < kBins; i += kEvictThreads) s.hist[i] = 0;
-    __syncthreads();
-    constexpr int U = 8;  // keys in flight per thread
-    for (int t0 = lo + tid; t0 < hi; t0 += U * kEvictThreads) {
-      uint32_t k[U];
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, bins = 1 << bits;
+      constexpr int U = 8;  // keys in flight per thread
+      for (int t0 = lo + tid; t0 < hi; t0 += U * kEvictThreads) {
+        uint32_t k[U];
+        if (held && pass) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u * kEvictThreads;
-        if (t >= hi) break;
-        k[u] = held && pass ? keys[t - lo] : key_of(t);
+          for (int u = 0; u < U; ++u) k[u] = keys[min(t0 + u * kEvictThreads, hi - 1) - lo];
+        } else {
+          int at[U];
+          float w[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int t = min(t0 + u * kEvictThreads, hi - 1);
+            at[u] = pos[t];
+            w[u] = mass[t];
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            k[u] = key_of(at[u], w[u]);
+            if (held && t0 + u * kEvictThreads < hi) keys[t0 + u * kEvictThreads - lo] = k[u];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (t0 + u * kEvictThreads < hi && (pass == 0 || (k[u] >> (shift + bits)) == edge))
+            atomicAdd(&s.hist[(k[u] >> shift) & (bins - 1)], 1);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u * kEvictThreads;
-        if (t >= hi) break;
-        if (held && pass == 0) keys[t - lo] = k[u];
-        if (pass == 0 || (k[u] >> (shift + bits)) == prefix) atomicAdd(&s.hist[(k[u] >> shift) & (bins - 1)], 1);
+      __syncthreads();
+      int* all = s.hist;
+      if (ranks > 1) {
+        all = s.all[pass & 1];
+        for (int i = tid; i < kBins; i += kEvictThreads) {
+          const int n = s.hist[i];
+          if (n)
+            for (int r = 0; r < ranks; ++r) add_cluster(&all[i], r, n);
+        }
+        meet();
       }
-    }
-    meet();
-    if (ranks > 1) {
-      // Each CTA adds up its share of the bins and hands it to all.
-      const int share = kBins / ranks;
-      for (int i = tid; i < share; i += kEvictThreads) {
-        const int bin = rank * share + i;
-        int sum = 0;
-        for (int r = 0; r < ranks; ++r) sum += ld_cluster(&s.hist[bin], r);
-        for (int r = 0; r < ranks; ++r) st_cluster_u32(&s.all[bin], r, (uint32_t)sum);
-      }
-      meet();
-    }
-    const int* all = ranks > 1 ? s.all : s.hist;
-    // Bins from the top: thread i has bins [top - 8 i, top - 8 (i + 1)).
-    constexpr int kPer = kBins / kEvictThreads;
-    int mine = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) mine += all[kBins - 1 - (tid * kPer + i)];
-    int run = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += v;
-    }
-    if (lane == 31) s.warp_a[warp] = run;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) run += s.warp_a[w];
-    int before = run - mine;
-    if (before < need && run >= need) {
+      // Bins from the top: thread i has bins [top - 8 i, top - 8 (i + 1)).
+      constexpr int kPer = kBins / kEvictThreads;
+      const int top = kBins - 1 - tid * kPer;
+      int n[kPer], mine = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int bin = kBins - 1 - (tid * kPer + i), n = all[bin];
-        if (before < need && before + n >= need) {
-          s.found[0] = bin;
-          s.found[1] = need - before;
-        }
-        before += n;
+        n[i] = all[top - i];
+        mine += n[i];
       }
+      int run = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += v;
+      }
+      if (lane == 31) s.warp_a[warp] = run;
+      __syncthreads();
+      // Clear for the passes to come: the histogram and the other totals (the
+      // ones just read are not added to before the next barrier).
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        s.hist[top - i] = 0;
+        if (pass == 1) s.all[0][top - i] = 0;
+      }
+      for (int w = 0; w < warp; ++w) run += s.warp_a[w];
+      int before = run - mine;
+      if (before < need && run >= need) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (before < need && before + n[i] >= need) {
+            s.found[0] = top - i;
+            s.found[1] = need - before;
+            s.found[2] = n[i];
+          }
+          before += n[i];
+        }
+      }
+      __syncthreads();
+      edge = edge << bits | (uint32_t)s.found[0];
+      need = s.found[1];
+      some = need < s.found[2];
+      if (pass == 1 && ranks > 1) meet();  // all[0] is clear everywhere before the last pass adds to it
     }
-    __syncthreads();
-    prefix = prefix << bits | (uint32_t)s.found[0];
-    need = s.found[1];
-    __syncthreads();
   }
-  const uint32_t edge = prefix;  // slots above it are kept, `need` of its equals too
 
-  // Equal slots before each warp's first one, over CTAs and warps in slot order.
   const int w_lo = min(lo + warp * per_warp, hi), w_hi = min(w_lo + per_warp, hi);
-  auto key_at = [&](int t) { return held ? keys[t - lo] : key_of(t); };
-  int eq = 0;
-  for (int t = w_lo + lane; t < w_hi; t += 32) eq += key_at(t) == edge;
-  eq = __reduce_add_sync(0xffffffffu, eq);
-  if (lane == 0) s.warp_a[warp] = eq;
-  __syncthreads();
+  auto key_at = [&](int t) { return held ? keys[t - lo] : key_of(pos[t], mass[t]); };
   auto tell = [&](int* slots, int value) {  // value of this CTA into slots[rank] of every CTA
     if (ranks > 1) {
       if (tid < ranks) st_cluster_u32(&slots[rank], tid, (uint32_t)value);
@@ -253,9 +265,18 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
     for (int i = 0; i < n; ++i) x += v[i];
     return x;
   };
-  tell(s.cluster_eq, sum_of(s.warp_a, kEvictWarps));
-  meet();
-  int eq_before = sum_of(s.cluster_eq, rank) + sum_of(s.warp_a, warp);
+  int eq_before = 0;
+  if (some) {  // equal slots before each warp's first one, over CTAs and warps in slot order
+    int eq = 0;
+    for (int t = w_lo + lane; t < w_hi; t += 32) eq += key_at(t) == edge;
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    if (lane == 0) s.warp_b[warp] = eq;
+    __syncthreads();
+    tell(s.cluster_eq, sum_of(s.warp_b, kEvictWarps));
+    meet();
+    eq_before = sum_of(s.cluster_eq, rank) + sum_of(s.warp_b, warp);
+    __syncthreads();
+  }
 
   // Bitmap of kept slots; holes and fills of each warp.
   int holes = 0, fills = 0;
@@ -263,11 +284,23 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
   for (int t = w_lo; t < w_hi; t += 32) {
     const bool in = t + lane < w_hi;
     const uint32_t k = in ? key_at(t + lane) : 0u;
-    const unsigned same = __ballot_sync(0xffffffffu, in && k == edge);
-    const bool keep = in && (k > edge || (k == edge && eq_before + __popc(same & ((1u << lane) - 1)) < need));
+    bool keep;
+    if (counted) {
+      int ahead = 0;  // slots that come before this one
+#pragma unroll 4
+      for (int j = 0; j < slice; j += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(keys + j);
+        ahead += (v.x > k || (v.x == k && j < t + lane)) + (v.y > k || (v.y == k && j + 1 < t + lane)) +
+                 (v.z > k || (v.z == k && j + 2 < t + lane)) + (v.w > k || (v.w == k && j + 3 < t + lane));
+      }
+      keep = in && ahead < p.budget;
+    } else {
+      const unsigned same = some ? __ballot_sync(0xffffffffu, in && k == edge) : 0u;
+      keep = in && (k > edge || (k == edge && (!some || eq_before + __popc(same & ((1u << lane) - 1)) < need)));
+      eq_before += __popc(same);
+    }
     const unsigned kept = __ballot_sync(0xffffffffu, keep), used = __ballot_sync(0xffffffffu, in);
     const unsigned below = t + 32 <= p.budget ? 0xffffffffu : t >= p.budget ? 0u : (1u << (p.budget - t)) - 1;
-    eq_before += __popc(same);
     holes += __popc(~kept & used & below);
     fills += __popc(kept & ~below);
     if (lane == 0) words[(t - w_lo) / 32] = kept;
@@ -277,17 +310,17 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
     s.warp_c[warp] = fills;
   }
   __syncthreads();
-  const int my_holes = sum_of(s.warp_b, kEvictWarps), my_fills = sum_of(s.warp_c, kEvictWarps);
-  const int hole_here = sum_of(s.warp_b, warp), fill_here = sum_of(s.warp_c, warp);
-  tell(s.cluster_hole, my_holes);
-  tell(s.cluster_fill, my_fills);
+  tell(s.cluster_hole, sum_of(s.warp_b, kEvictWarps));
+  tell(s.cluster_fill, sum_of(s.warp_c, kEvictWarps));
   meet();
-  const int hole0 = sum_of(s.cluster_hole, rank) + hole_here, fill0 = sum_of(s.cluster_fill, rank) + fill_here;
+  const int hole0 = sum_of(s.cluster_hole, rank) + sum_of(s.warp_b, warp);
+  const int fill0 = sum_of(s.cluster_fill, rank) + sum_of(s.warp_c, warp);
   const int moves = sum_of(s.cluster_hole, ranks);
 
   // Rounds of up to `list` moves per CTA: move m is CTA m % ranks's.
   uint8_t* kc = (uint8_t*)p.c.k + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
   uint8_t* vc = (uint8_t*)p.c.v + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
+  const int64_t row_bytes = p.c.st * esize;
   for (int from = 0; from < moves; from += list * ranks) {
     const int upto = min(moves, from + list * ranks);
     int h = hole0, f = fill0;
@@ -295,35 +328,32 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
       const unsigned kept = words[(t - w_lo) / 32], used = w_hi - t >= 32 ? 0xffffffffu : (1u << (w_hi - t)) - 1;
       const unsigned below = t + 32 <= p.budget ? 0xffffffffu : t >= p.budget ? 0u : (1u << (p.budget - t)) - 1;
       const unsigned hm = ~kept & used & below, fm = kept & ~below, lt = (1u << lane) - 1;
-      const int hr = h + __popc(hm & lt), fr = f + __popc(fm & lt);
-      auto put = [&](int* to, int m) {
-        const int at = (m - from) / ranks;
-        if (ranks > 1) st_cluster_u32(&to[at], (uint32_t)((m - from) % ranks), (uint32_t)(t + lane));
-        else to[at] = t + lane;
-      };
-      if ((hm >> lane & 1) && hr >= from && hr < upto) put(list_to, hr);
-      if ((fm >> lane & 1) && fr >= from && fr < upto) put(list_from, fr);
+      // A lane's slot is a hole or a fill, not both.
+      const bool hole = hm >> lane & 1;
+      const int m = hole ? h + __popc(hm & lt) : f + __popc(fm & lt);
+      if (((hm | fm) >> lane & 1) && m >= from && m < upto) {
+        const unsigned at = (unsigned)(m - from) / (unsigned)ranks, to = (unsigned)(m - from) % (unsigned)ranks;
+        int* slot = (hole ? list_to : list_from) + at;
+        if (ranks > 1) st_cluster_u32(slot, to, (uint32_t)(t + lane));
+        else *slot = t + lane;
+      }
       h += __popc(hm);
       f += __popc(fm);
     }
     meet();
-    const int mine = (upto - from - rank + ranks - 1) / ranks;
-    const int work = mine * chunks;
+    // chunks is a power of two; a warp's lanes copy neighbouring chunks.
+    const int mine = (upto - from - rank + ranks - 1) / ranks, work = mine * chunks, log = __ffs(chunks) - 1;
     for (int i0 = tid; i0 < work; i0 += 4 * kEvictThreads) {
       uint4 kv[4], vv[4];
       int64_t to[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * kEvictThreads;
-        if (i >= work) continue;
-        const int m = i / chunks, ch = i - m * chunks, src = list_from[m], dst = list_to[m];
-        kv[u] = *reinterpret_cast<const uint4*>(kc + src * p.c.st * esize + ch * 16);
-        vv[u] = *reinterpret_cast<const uint4*>(vc + src * p.c.st * esize + ch * 16);
-        to[u] = dst * p.c.st * esize + ch * 16;
-        if (ch == 0) {
-          mass_out[dst] = mass[src];
-          pos_out[dst] = pos[src];
-        }
+        const int i = min(i0 + u * kEvictThreads, work - 1);
+        const int m = i >> log, ch = (i & (chunks - 1)) * 16;
+        const int64_t src = list_from[m] * row_bytes + ch;
+        to[u] = list_to[m] * row_bytes + ch;
+        kv[u] = *reinterpret_cast<const uint4*>(kc + src);
+        vv[u] = *reinterpret_cast<const uint4*>(vc + src);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -331,6 +361,11 @@ __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(const __grid
         *reinterpret_cast<uint4*>(kc + to[u]) = kv[u];
         *reinterpret_cast<uint4*>(vc + to[u]) = vv[u];
       }
+    }
+    for (int i = tid; i < mine; i += kEvictThreads) {
+      const int src = list_from[i], dst = list_to[i];
+      mass_out[dst] = mass[src];
+      pos_out[dst] = pos[src];
     }
     if (from + list * ranks < moves) meet();  // the lists are used again
   }
