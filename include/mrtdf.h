@@ -585,9 +585,15 @@ typedef struct mrtdf_q4_args {
   const void* scales; /* (n, k / group) */
   const void* biases; /* (n, k / group) */
   void* out;          /* (m, n), out_stride elements from row to row */
+  void* workspace;    /* mrtdf_q4_linear_workspace bytes, 16-byte aligned; contents do not matter */
+  size_t workspace_bytes;
   int64_t x_stride, out_stride;
   int32_t m, n, k, group, dtype, out_dtype, device;
 } mrtdf_q4_args;
+/* Workspace of a call with these sizes (x as the product takes it: some bytes
+ * per element of x). args' pointers must be set as for the call, workspace
+ * aside. */
+int mrtdf_q4_linear_workspace(const mrtdf_q4_args* args, size_t* bytes);
 int mrtdf_q4_linear(const mrtdf_q4_args* args, void* stream);
 
 /*

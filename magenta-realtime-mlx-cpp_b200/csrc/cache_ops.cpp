@@ -160,6 +160,34 @@ TreeParams tree_params(const mrtdf_cache* cache, const mrtdf_tree_args* a, const
   return p;
 }
 
+Q4Params q4_params(const mrtdf_q4_args* a, const char* op) {
+  if (!a) invalid("q4_linear: args is NULL");
+  if (a->struct_bytes != sizeof(mrtdf_q4_args)) invalid("q4_linear: args.struct_bytes is not sizeof(mrtdf_q4_args)");
+  const int es = dtype_bytes(a->dtype, op);
+  dtype_bytes(a->out_dtype, op);
+  if (a->dtype == MRTDF_DTYPE_FP32 && a->out_dtype != MRTDF_DTYPE_FP32) invalid("q4_linear: float32 x gives float32 out");
+  if (a->group != 32 && a->group != 64 && a->group != 128) invalid("q4_linear: group must be 32, 64 or 128");
+  if (a->m < 1 || a->n < 1 || a->k < 1 || a->k % a->group) invalid("q4_linear: sizes must be positive and k a multiple of the group");
+  if (a->m > kQ4MaxRows || a->k > kQ4MaxIn || a->n > (1 << 24)) out_of_range("q4_linear: at most 64 rows of x, k 2^17, n 2^24");
+  if (!a->x || !a->packed || !a->scales || !a->biases || !a->out) invalid("q4_linear: NULL argument");
+  if (!aligned16(a->x) || !aligned16(a->packed)) invalid("q4_linear: x and packed must be 16-byte aligned");
+  if (a->device < 0) invalid("q4_linear: device is negative");
+  Q4Params p{};
+  p.x = a->x;
+  p.packed = static_cast<const uint8_t*>(a->packed);
+  p.scales = a->scales;
+  p.biases = a->biases;
+  p.out = a->out;
+  p.x_stride = step(a->x_stride, a->m, es, op, "x");
+  p.out_stride = a->out_stride;
+  if (a->m > 1 && a->out_stride < a->n) invalid("q4_linear: out_stride is less than n");
+  p.m = a->m;
+  p.n = a->n;
+  p.k = a->k;
+  p.group = a->group;
+  return p;
+}
+
 }  // namespace
 
 extern "C" {
@@ -281,35 +309,27 @@ int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* a, void*
   });
 }
 
+int mrtdf_q4_linear_workspace(const mrtdf_q4_args* a, size_t* bytes) {
+  return guarded([&] {
+    if (!bytes) invalid("q4_linear_workspace: bytes is NULL");
+    const Q4Params p = q4_params(a, "q4_linear_workspace");
+    cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, op_sm_count(a->device), bytes, nullptr), "q4_linear_workspace");
+  });
+}
+
 int mrtdf_q4_linear(const mrtdf_q4_args* a, void* stream) {
   return guarded([&] {
     const char* op = "q4_linear";
-    if (!a) invalid("q4_linear: args is NULL");
-    if (a->struct_bytes != sizeof(mrtdf_q4_args)) invalid("q4_linear: args.struct_bytes is not sizeof(mrtdf_q4_args)");
-    const int es = dtype_bytes(a->dtype, op);
-    dtype_bytes(a->out_dtype, op);
-    if (a->dtype == MRTDF_DTYPE_FP32 && a->out_dtype != MRTDF_DTYPE_FP32) invalid("q4_linear: float32 x gives float32 out");
-    if (a->group != 32 && a->group != 64 && a->group != 128) invalid("q4_linear: group must be 32, 64 or 128");
-    if (a->m < 1 || a->n < 1 || a->k < 1 || a->k % a->group) invalid("q4_linear: sizes must be positive and k a multiple of the group");
-    if (a->m > kQ4MaxRows || a->k > kQ4MaxIn || a->n > (1 << 24)) out_of_range("q4_linear: at most 64 rows of x, k 2^17, n 2^24");
-    if (!a->x || !a->packed || !a->scales || !a->biases || !a->out) invalid("q4_linear: NULL argument");
-    if (!aligned16(a->x) || !aligned16(a->packed)) invalid("q4_linear: x and packed must be 16-byte aligned");
-    if (a->device < 0) invalid("q4_linear: device is negative");
-    Q4Params p{};
-    p.x = a->x;
-    p.packed = static_cast<const uint8_t*>(a->packed);
-    p.scales = a->scales;
-    p.biases = a->biases;
-    p.out = a->out;
-    p.x_stride = step(a->x_stride, a->m, es, op, "x");
-    p.out_stride = a->out_stride;
-    if (a->m > 1 && a->out_stride < a->n) invalid("q4_linear: out_stride is less than n");
-    p.m = a->m;
-    p.n = a->n;
-    p.k = a->k;
-    p.group = a->group;
+    Q4Params p = q4_params(a, op);
+    size_t need = 0;
+    const int sms = op_sm_count(a->device);
+    cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, &need, nullptr), op);
+    if (!a->workspace || a->workspace_bytes < need)
+      invalid("q4_linear: the workspace is smaller than mrtdf_q4_linear_workspace says (" + std::to_string(need) + " bytes)");
+    if (!aligned16(a->workspace)) invalid("q4_linear: the workspace must be 16-byte aligned");
+    p.ws = a->workspace;
     DeviceScope on(a->device, op);
-    cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, static_cast<cudaStream_t>(stream)), op);
+    cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, nullptr, static_cast<cudaStream_t>(stream)), op);
   });
 }
 

@@ -1,22 +1,35 @@
 // Products with 4-bit weights and one scale and bias per group of columns:
 //   y[m, n] = sum_k x[m, k] w[n, k],  w[n, k] = scale[n, k / G] q[n, k] + bias[n, k / G]
 // with q in 0 .. 15. Per group, with a = q - 8 and X = sum of the group's x,
-//   y += scale * (sum a x) + (bias + 8 scale) * X,
+//   y += scale * (sum a x + 8 X) + bias * X,
 // so the weights are exact small integers in the matrix product and the
-// scales multiply float32 sums: no weight is rounded. The offset 8 keeps the
-// two terms from cancelling where bias is near -8 scale.
+// scales multiply float32 sums: no weight is rounded.
 //
 // For a few rows of x the product is bound by the weight stream (k / 2 bytes
-// per output). A warp takes 16 output rows as the M side of m16n8k16, the rows
-// of x are its eight columns; weights go from global memory through a private
-// cp.async ring to registers and are unpacked there: (w >> s) & 0x000f000f |
-// 0x43004300 is the bf16 pair 128 + q (exact), minus 136 is q - 8 (exact).
-// float32 rows of x are split into three bf16 columns, x = x1 + x2 + x3 with
-// all 24 bits, which the same product multiplies exactly.
+// per output) and, next to it, by the instructions that unpack the weights. A
+// warp takes 16 output rows as the M side of m16n8k16 (fp16), the rows of x
+// are its eight columns; weights go from global memory through a private
+// cp.async ring to registers. fp16 has ten mantissa bits, so two nibbles of a
+// 16-bit half become numbers without a shift: w & 0x000f000f | 0x64006400 is
+// the pair 1024 + q, w & 0x00f000f0 | 0x64006400 the pair 1024 + 16 q (exact).
+//   float32 results: one more instruction each makes them q - 8 (exact).
+//   bf16 results: they stay, the odd columns of x are divided by 16, and the
+//   sums 1024 X_even + 64 X_odd are taken off in float32. That loses seven bits
+//   of float32, nothing in a bf16 result: 5 instructions per 8 weights, not 9.
+// x is brought to fp16 by a power of two per row and group that puts the
+// group's largest |x| into [2^14, 2^15): bf16 x keeps all its bits (smaller
+// ones down to 2^-31 of the largest), float32 x becomes two columns, x = hi + lo
+// with 22 bits. The factor multiplies the group's float32 sum. A kernel of its
+// own does that once; every CTA doing it for itself took as many instructions
+// as the product. The product's weights are on their way meanwhile (programmatic
+// dependent launch).
 //
 // The k index of a product is arbitrary as long as both operands agree: lane
-// (g, c) unpacks whole words of 8 columns from its own rows, and x lies in
-// shared memory in the order in which the lanes ask for it.
+// (g, c) unpacks whole words of 8 columns from its own rows, in the pairs
+// (0, 4), (1, 5), (2, 6), (3, 7), and x lies in shared memory in the order in
+// which the lanes ask for it.
+#include <cuda_fp16.h>
+
 #include "cache_ops.cuh"
 #include "cache_tile.cuh"
 #include "q4.cuh"
@@ -24,234 +37,457 @@
 namespace mrtdf {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kStep = 128;  // columns of a ring stage: 64 bytes of 16 rows
-constexpr int kRing = 5;    // stages per warp
-constexpr int kStageBytes = 16 * kStep / 2;
-constexpr int kChunkElems = 32 * 1024;  // x values (bf16) in shared memory at a time
+constexpr int kMaxWarps = 16;
+constexpr int kStep = 128;  // columns multiplied at a time: 64 bytes of 16 rows
+constexpr int kStepBytes = 16 * kStep / 2;
+// A ring stage has two steps, so that a row gives 128 bytes at a time: in 64-byte
+// pieces 67 MB came in 13 us, in 128-byte pieces in 11 (from L2, no products).
+constexpr int kStageBytes = 2 * kStepBytes;
+constexpr int kRing = 4;  // stages per warp
+constexpr int kSmemMax = 224 * 1024;
 
-// Byte offset of 16-byte chunk `ch` (0 .. 3) of row `row` of a stage. Rows are
+// Byte offset of 16-byte chunk `ch` (0 .. 3) of row `row` of a step. Rows are
 // 64 bytes apart; the swizzle puts the eight rows of one access in different
 // banks.
 __device__ __forceinline__ uint32_t w_at(int row, int ch) {
   return (uint32_t)(row * (kStep / 2) + ((ch ^ (row >> 1 & 3)) << 4));
 }
 
-// Words of a stage that lane (row, c) multiplies for group-in-stage `gi`:
-// WL = G / 32 words, columns gi * G + (c * WL + i) * 8.
+// Words of a step that lane c multiplies for its group `gi`, from row address
+// `row` (of a step, without the chunk) whose swizzle is x: WL = G / 32 words,
+// columns gi * G + (c * WL + i) * 8.
 template <int WL>
-__device__ __forceinline__ void load_words(uint32_t* w, uint32_t stage, int row, int c, int gi) {
+__device__ __forceinline__ void load_words(uint32_t* w, uint32_t row, uint32_t x, int c, int gi) {
   if constexpr (WL == 1) {
-    w[0] = lds32(stage + w_at(row, gi) + 4 * c);
+    w[0] = lds32(row + ((gi << 4) ^ x) + 4 * c);
   } else if constexpr (WL == 2) {
-    const uint32_t a = stage + w_at(row, 2 * gi + (c >> 1)) + 8 * (c & 1);
+    const uint32_t a = row + (((2 * gi + (c >> 1)) << 4) ^ x) + 8 * (c & 1);
     asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
   } else {
-    const uint32_t a = stage + w_at(row, c);
+    const uint32_t a = row + ((c << 4) ^ x);
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                  : "r"(a));
   }
 }
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
 
-// Nibbles s / 4 and s / 4 + 4 of w, minus 8, as a bf16 pair.
-template <int SHIFT>
-__device__ __forceinline__ uint32_t nibbles(uint32_t w) {
-  uint32_t v = (w >> SHIFT) & 0x000f000fu | 0x43004300u;
-  const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));  // 136
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
-  return *reinterpret_cast<const uint32_t*>(&r);
+// The column pairs (0, 4), (1, 5) of w, or with w >> 8 (2, 6), (3, 7): q - 8
+// (EIGHT), or 1024 + q and 1024 + 16 q.
+template <bool EIGHT>
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t& even, uint32_t& odd) {
+  // (w & mask) | magic in one instruction each
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(even) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(odd) : "r"(w), "n"(0x00f000f0), "r"(0x64006400u));
+  if (EIGHT) {
+    const __half2 e = __hadd2(*reinterpret_cast<const __half2*>(&even), __float2half2_rn(-1032.f));
+    const __half2 o = __hfma2(*reinterpret_cast<const __half2*>(&odd), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+    even = *reinterpret_cast<const uint32_t*>(&e);
+    odd = *reinterpret_cast<const uint32_t*>(&o);
+  }
+}
+
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c = a b: the first product of a sum, on zeros that take no registers.
+__device__ __forceinline__ void mma_f16_first(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A scale and its bias, side by side in shared memory.
+__device__ __forceinline__ void load_pair(uint32_t at, float& s, float& b, __nv_bfloat16) {
+  const uint32_t w = lds32(at);
+  s = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void load_pair(uint32_t at, float& s, float& b, float) {
+  uint32_t x, y;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(at));
+  s = __uint_as_float(x);
+  b = __uint_as_float(y);
 }
 
 template <typename T>
-struct Parts;  // bf16 columns per row of x
+struct Parts;  // fp16 columns per row of x
 template <>
 struct Parts<__nv_bfloat16> {
   static constexpr int N = 1;
 };
 template <>
 struct Parts<float> {
-  static constexpr int N = 3;
+  static constexpr int N = 2;
 };
 
-// T: type of x, scales and biases. NT: tiles of eight columns (rows of x x
-// parts). WR: warps with rows of their own; the other kWarps / WR split k.
-template <typename T, typename O, int G, int NT, int WR>
-__global__ __launch_bounds__(kThreads) void q4_linear_kernel(const __grid_constant__ Q4Params p, int rows_per_pass,
-                                                              int chunk) {
-  constexpr int WL = G / 32, GS = kStep / G, WK = kWarps / WR, P = Parts<T>::N, COLS = NT * 8;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wr = warp % WR, wk = warp / WR;
-  const int g = lane >> 2, c = lane & 3;
-  const int m0 = blockIdx.y * rows_per_pass, ms = min(rows_per_pass, p.m - m0);
-  const int row0 = (blockIdx.x * WR + wr) * 16, groups = p.k / G;
-  const uint32_t ring = smem_u32(smem) + warp * (kRing * kStageBytes);
-  // x: column i at i * x_stride bytes; 64 bytes past a multiple of 128, so two
-  // columns of one access lie in different banks. Group sums behind it.
-  const int x_bytes = chunk * 2 + 64;
-  uint8_t* xs = smem + kWarps * kRing * kStageBytes;
-  float* sums = reinterpret_cast<float*>(xs + COLS * x_bytes);  // [group of the chunk][COLS]
+// How a product is laid out over the GPU.
+struct Q4Plan {
+  int split;  // CTAs of a cluster: each has a slab of the columns
+  int tiles;  // row tiles of 16 per cluster (and so per CTA)
+  int warps;  // warps with tiles of their own, taking every warps-th
+  int wk;     // warps per tile: each takes every wk-th stage of the slab
+  int slab;   // steps of 128 columns per CTA
+  int chunk;  // of them, those whose x is in shared memory at a time
+  int part;   // of a chunk, the steps that one barrier stands for
+  int rows;   // rows of x per pass (grid y)
+  int steps;  // all steps
+};
+constexpr int kParts = 4;  // barriers of a chunk
 
-  const int steps = (p.k + kStep - 1) / kStep;
-  // Stage t of this warp: columns (t * WK + wk) * 128.
-  const int mine = (steps - wk + WK - 1) / WK;
-  auto fetch = [&](int t) {
-    const int k0 = (t * WK + wk) * kStep;
-    const uint32_t st = ring + (t % kRing) * kStageBytes;
+// Shared memory of a CTA, in order: rings, x, factors of x, scales, partial
+// sums, barriers.
+template <typename T, int G, int NT>
+struct Q4Smem {
+  static constexpr int COLS = NT * 8;
+  int x_bytes, x, factors, scales, part, bars, bytes;
+  __host__ __device__ explicit Q4Smem(const Q4Plan& q) {
+    x_bytes = q.chunk * kStep * 2 + 64;
+    x = q.warps * q.wk * kRing * kStageBytes;
+    factors = x + COLS * x_bytes;
+    scales = factors + (q.chunk * kStep / G) * COLS * 16;
+    part = scales + (q.chunk * kStep / G) * q.tiles * 16 * 2 * (int)sizeof(T);
+    const int units = q.tiles > q.warps * q.wk ? q.tiles : q.warps * q.wk;
+    bars = (part + units * 16 * (COLS + 1) * 4 + 7) / 8 * 8;
+    bytes = bars + kParts * 8;
+  }
+};
+
+// The prepared x of one pass: [COLS][steps * 128] fp16, then
+// [group][COLS] {factor of the group's sum, what is added to it, X, 0}.
+template <int G, int NT>
+struct Q4Prepared {
+  static constexpr int COLS = NT * 8;
+  static __host__ __device__ int64_t x_bytes(int steps) { return (int64_t)COLS * steps * kStep * 2; }
+  static __host__ __device__ int64_t bytes(int steps) { return x_bytes(steps) + (int64_t)steps * (kStep / G) * COLS * 16; }
+};
+
+__device__ __forceinline__ float ld_cluster_f32(const float* local, uint32_t rank) {
+  uint32_t ra;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ra) : "memory");
+  return v;
+}
+
+// x to fp16: 8 columns (one word of weights) per lane, a group by 4 WL
+// neighbouring lanes; words of one group and index i next to each other for
+// c = 0 .. 3. Columns without a row of x, and columns past k, are zero.
+template <typename T, int G, int NT, bool EIGHT>
+__global__ __launch_bounds__(128) void q4_prepare_kernel(const __grid_constant__ Q4Params p, int steps, int rows) {
+  constexpr int WL = G / 32, P = Parts<T>::N, COLS = NT * 8, V = 8 * (int)sizeof(T) / 16;
+  pdl_launch_dependents();
+  const int words = steps * (kStep / 8), lane = threadIdx.x & 31, m0 = blockIdx.y * rows;
+  uint8_t* out = static_cast<uint8_t*>(p.ws) + blockIdx.y * Q4Prepared<G, NT>::bytes(steps);
+  float4* factor = reinterpret_cast<float4*>(out + Q4Prepared<G, NT>::x_bytes(steps));
+  const int i = blockIdx.x * 128 + threadIdx.x;
+  if (i - lane >= words * (COLS / P)) return;
+  const int m = i / words, wd = i - m * words, kk = wd * 8;
+  float v[8], big = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int idx = lane + 32 * i, row = idx >> 2, ch = idx & 3, n = row0 + row, kb = k0 / 2 + ch * 16;
-      const bool on = n < p.n && kb < p.k / 2;
-      cp_async16_zfill(st + w_at(row, ch), p.packed + (on ? (int64_t)n * (p.k / 2) + kb : 0), on);
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  if (m < rows && m0 + m < p.m && kk < p.k) {
+    const T* src = reinterpret_cast<const T*>(p.x) + (m0 + m) * p.x_stride + kk;
+#pragma unroll
+    for (int e = 0; e < V; ++e) Vec16<T>::unpack(*reinterpret_cast<const uint4*>(src + e * (8 / V)), v + e * (8 / V));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(v[e]));
+#pragma unroll
+  for (int o = 1; o < 4 * WL; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  const uint32_t ex = max(__float_as_uint(big) >> 23, 15u);
+  const float up = __uint_as_float((268u - ex) << 23), down = __uint_as_float((ex - 14u) << 23);
+  const int gr = wd / (4 * WL), in = wd % (4 * WL), to = gr * 4 * WL + (in % WL) * 4 + in / WL;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= up;
+#pragma unroll
+  for (int h = 0; h < P; ++h) {
+    uint32_t w[4];
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = pack_f16(v[e], v[e + 4]);
+      const float2 t2 = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      f[e] = t2.x;
+      f[e + 4] = t2.y;
+    }
+    float even = (f[0] + f[4]) + (f[2] + f[6]), odd = (f[1] + f[5]) + (f[3] + f[7]);
+#pragma unroll
+    for (int o = 1; o < 4 * WL; o <<= 1) {
+      even += __shfl_xor_sync(0xffffffffu, even, o);
+      odd += __shfl_xor_sync(0xffffffffu, odd, o);
+    }
+    if (i < words * (COLS / P)) {
+      if (!EIGHT) {
+        w[1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
+        w[3] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
+      }
+      *reinterpret_cast<uint4*>(out + ((int64_t)(m * P + h) * words + to) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (in == 0) {
+        const float sum = down * (even + odd);
+        factor[gr * COLS + m * P + h] =
+            make_float4(down, EIGHT ? 8.f * sum : -down * (1024.f * even + 64.f * odd), sum, 0.f);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] -= f[e];
+  }
+}
+
+// T: type of x, scales and biases. NT: tiles of eight columns (rows of x x
+// parts). A cluster works on q.tiles row tiles, its CTAs on a slab of the
+// columns each (a CTA reads half of x that way); the slabs' sums meet over
+// distributed shared memory, in rank order.
+template <typename T, typename O, int G, int NT>
+__global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __grid_constant__ Q4Params p,
+                                                                                     const __grid_constant__ Q4Plan q) {
+  constexpr int WL = G / 32, GS = kStep / G, P = Parts<T>::N, COLS = NT * 8, LD = COLS + 1;
+  constexpr bool EIGHT = sizeof(O) == 4;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const Q4Smem<T, G, NT> at(q);
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
+  const int wt = warp % q.warps, wk = warp / q.warps, g = lane >> 2, c = lane & 3;
+  const int rank = q.split > 1 ? (int)cluster_ctarank() : 0, cluster = blockIdx.x / q.split;
+  const int m0 = blockIdx.y * q.rows, ms = min(q.rows, p.m - m0);
+  const int tile0 = cluster * q.tiles, tiles = min(q.tiles, (p.n + 15) / 16 - tile0), stride = q.tiles * 16;
+  const int groups = p.k / G, row_bytes = p.k / 2, n0 = tile0 * 16;
+  const int slab0 = rank * q.slab, slab_end = min(slab0 + q.slab, q.steps);
+  T* sb = reinterpret_cast<T*>(smem + at.scales);  // [group][row], scale and bias side by side
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + at.bars);
+  const uint8_t* prepared = static_cast<const uint8_t*>(p.ws) + blockIdx.y * Q4Prepared<G, NT>::bytes(q.steps);
+  float* part = reinterpret_cast<float*>(smem + at.part);  // [wk][row][COLS + 1]
+
+  const uint32_t ring = smem_u32(smem) + warp * (kRing * kStageBytes);
+  const int fr = lane >> 3, fc = lane & 7;  // a lane copies chunk fc of rows fr, fr + 4, ...
+  const int units_max = q.tiles > q.warps * q.wk ? q.tiles : q.warps * q.wk;
+  for (int i = tid; i < units_max * 16 * LD; i += threads) part[i] = 0.f;
+
+  if (tid == 0) {
+    for (int i = 0; i < kParts; ++i) mbar_init(bars + i, 1);
+    fence_mbar_init();
+  }
+
+  for (int step0 = slab0, round = 0; step0 < slab_end; step0 += q.chunk, ++round) {
+  const int steps = min(q.chunk, slab_end - step0), k0 = step0 * kStep;
+  // This warp's units: its tiles, and of each its stages. Rows past n and
+  // columns past k read a valid address instead: the former are not written,
+  // the latter meet zeros of x.
+  const int my_stages = max(0, ((steps + 1) / 2 - wk + q.wk - 1) / q.wk), my_tiles = max(0, (tiles - wt + q.warps - 1) / q.warps);
+  const int units = my_stages * my_tiles;
+  const int first_col = (k0 + wk * 2 * kStep) / 2 + fc * 16, last_col = row_bytes - 16, col_step = q.wk * kStep;
+  int f_unit = 0, f_step = 0, f_tile = wt, f_col = first_col;  // the unit to fetch next
+  uint32_t f_stage = ring + (fc >> 2) * kStepBytes;
+  const uint8_t* from[4];
+  auto enter = [&] {
+    const int row = n0 + f_tile * 16 + fr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from[i] = p.packed + (int64_t)min(row + 4 * i, p.n - 1) * row_bytes;
+  };
+  enter();
+  auto fetch = [&] {
+    const int col = min(f_col, last_col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cp_async16(f_stage + w_at(fr + 4 * i, fc & 3), from[i] + col);
+    f_stage += kStageBytes;
+    f_col += col_step;
+    if ((++f_unit & (kRing - 1)) == 0) f_stage -= kRing * kStageBytes;
+    if (++f_step == my_stages) {
+      f_step = 0;
+      f_col = first_col;
+      f_tile += q.warps;
+      enter();
     }
   };
 #pragma unroll
   for (int t = 0; t < kRing - 1; ++t) {
-    if (t < mine) fetch(t);
+    if (f_unit < units) fetch();
     cp_async_commit();
   }
 
-  const T* sc0 = reinterpret_cast<const T*>(p.scales) + (int64_t)min(row0 + g, p.n - 1) * groups;
-  const T* sc1 = reinterpret_cast<const T*>(p.scales) + (int64_t)min(row0 + g + 8, p.n - 1) * groups;
-  const T* bi0 = reinterpret_cast<const T*>(p.biases) + (int64_t)min(row0 + g, p.n - 1) * groups;
-  const T* bi1 = reinterpret_cast<const T*>(p.biases) + (int64_t)min(row0 + g + 8, p.n - 1) * groups;
+  if (round) __syncthreads();  // the chunk before is done with
+  const int gn = steps * GS, g0 = k0 / G;
+  if (round == 0) pdl_wait();  // x is prepared
+  if (tid == 0) {
+    // The chunk before was read through the generic proxy.
+    if (round) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    const uint32_t factor_bytes = gn * COLS * 16;
+    for (int i = 0; i < kParts; ++i) {
+      const int first = i * q.part, n = min(q.part, steps - first);
+      if (n <= 0) break;
+      mbar_arrive_expect_tx(bars + i, COLS * n * kStep * 2 + (i == 0 ? factor_bytes : 0));
+      if (i == 0)
+        bulk_g2s(smem + at.factors, prepared + Q4Prepared<G, NT>::x_bytes(q.steps) + (int64_t)g0 * COLS * 16, factor_bytes, bars);
+      for (int col = 0; col < COLS; ++col)
+        bulk_g2s(smem + at.x + col * at.x_bytes + first * kStep * 2,
+                 prepared + ((int64_t)col * q.steps + step0 + first) * (kStep * 2), n * kStep * 2, bars + i);
+    }
+  }
+  // Scales and biases of the chunk's groups, side by side: 16 bytes at a time
+  // where rows and groups allow it.
+  constexpr int E = 16 / (int)sizeof(T);
+  if (groups % E == 0 && g0 % E == 0) {
+    const int vecs = (gn + E - 1) / E, all = tiles * 16 * vecs;
+    for (int i0 = tid; i0 < all; i0 += 4 * threads) {
+      uint4 s[4], b[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = min(i0 + u * threads, all - 1), r = i / vecs;
+        const int64_t from = (int64_t)min(n0 + r, p.n - 1) * groups + min(g0 + (i - r * vecs) * E, groups - E);
+        s[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.scales) + from);
+        b[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.biases) + from);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = min(i0 + u * threads, all - 1), r = i / vecs, first = (i - r * vecs) * E;
+        const T *sv = reinterpret_cast<const T*>(&s[u]), *bv = reinterpret_cast<const T*>(&b[u]);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (first + e < gn) {
+            sb[((first + e) * stride + r) * 2] = sv[e];
+            sb[((first + e) * stride + r) * 2 + 1] = bv[e];
+          }
+      }
+    }
+  } else {
+    for (int i = tid; i < gn * tiles * 16; i += threads) {
+      const int r = i / gn, gr = i - r * gn;
+      const int64_t from = (int64_t)min(n0 + r, p.n - 1) * groups + min(g0 + gr, groups - 1);
+      sb[(gr * stride + r) * 2] = reinterpret_cast<const T*>(p.scales)[from];
+      sb[(gr * stride + r) * 2 + 1] = reinterpret_cast<const T*>(p.biases)[from];
+    }
+  }
+  __syncthreads();  // the scales are there, and the barriers
 
   float y[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j) y[j][0] = y[j][1] = y[j][2] = y[j][3] = 0.f;
-
-  T s0[GS], s1[GS], b0[GS], b1[GS];  // scales of the stage to come
-  auto fetch_scales = [&](int t) {
-    const int gr = (t * WK + wk) * GS;
+  // Shared addresses of this lane's operands in the unit's step.
+  const uint32_t swz = (uint32_t)(g >> 1 & 3) << 4;  // of rows g and g + 8
+  const uint32_t x_first = smem_u32(smem + at.x) + g * at.x_bytes + c * 16 + wk * 2 * GS * (WL * 64);
+  const uint32_t f_first = smem_u32(smem + at.factors) + (wk * 2 * GS * COLS + 2 * c) * 16;
+  const uint32_t s_first = smem_u32(sb) + (wk * 2 * GS * stride + wt * 16 + g) * 2 * (int)sizeof(T);
+  const uint32_t x_step = GS * (WL * 64), fa_step = GS * COLS * 16, skip = 2 * q.wk - 2, s_group = stride * 2 * (int)sizeof(T);
+  uint32_t xa = x_first, fa = f_first, sa = s_first, row = ring + g * (kStep / 2), st = 0;
+  int tile = wt, step = 0, parts = 0;  // parts of x that have arrived
+  for (int t = 0; t < units; ++t) {
+    while (parts * q.part <= min((step * q.wk + wk) * 2 + 1, steps - 1)) mbar_wait_bounded(bars + parts++, round & 1, nullptr);
+    cp_async_wait<kRing - 2>();
+    __syncwarp();
+    if (f_unit < units) fetch();
+    cp_async_commit();
+    const bool odd_end = (step * q.wk + wk) * 2 + 1 >= steps;
 #pragma unroll
-    for (int i = 0; i < GS; ++i) {
-      const int at = min(gr + i, groups - 1);
-      s0[i] = sc0[at];
-      s1[i] = sc1[at];
-      b0[i] = bi0[at];
-      b1[i] = bi1[at];
-    }
-  };
-  fetch_scales(0);
-
-  int t = 0;
-  for (int k0 = 0; k0 < p.k; k0 += chunk) {
-    const int kn = min(chunk, steps * kStep - k0);  // a multiple of 128; columns past k are zero
-    if (k0) __syncthreads();
-    // x into shared memory: 8 columns (one word of weights) per thread, in the
-    // order (0, 4, 1, 5, 2, 6, 3, 7); words of one group and index i next to
-    // each other for c = 0 .. 3.
-    const int words = kn / 8;
-    for (int i = tid; i < words * rows_per_pass; i += kThreads) {
-      const int m = i / words, wd = i - m * words, kk = k0 + wd * 8;
-      float v[8];
+    for (int sub = 0; sub < 2; ++sub) {
+    if (sub && odd_end) break;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (m < ms && kk < p.k) {
-        const T* src = reinterpret_cast<const T*>(p.x) + (m0 + m) * p.x_stride + kk;
+    for (int gi = 0; gi < GS; ++gi) {
+      uint32_t w0[WL], w1[WL];
+      load_words<WL>(w0, row + st + sub * kStepBytes, swz, c, gi);
+      load_words<WL>(w1, row + st + sub * kStepBytes + 8 * (kStep / 2), swz, c, gi);
+      float s0, s1, b0, b1;
+      load_pair(sa + gi * s_group, s0, b0, T());
+      load_pair(sa + gi * s_group + 16 * (int)sizeof(T), s1, b1, T());
+      float acc[NT][4], acd[NT][4];
 #pragma unroll
-        for (int e = 0; e < 8; e += 16 / (int)sizeof(T))
-          Vec16<T>::unpack(*reinterpret_cast<const uint4*>(src + e), v + e);
-      }
-      const int gr = wd / (4 * WL), in = wd - gr * 4 * WL, at = gr * 4 * WL + (in % WL) * 4 + in / WL;
-#pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const uint4 u = make_uint4(pack_bf16(v[0], v[4]), pack_bf16(v[1], v[5]), pack_bf16(v[2], v[6]), pack_bf16(v[3], v[7]));
-        *reinterpret_cast<uint4*>(xs + (m * P + q) * x_bytes + at * 16) = u;
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] -= __uint_as_float(w[e] << 16);
-          v[e + 4] -= __uint_as_float(w[e] & 0xffff0000u);
-        }
-      }
-    }
-    for (int i = tid + words * rows_per_pass * P; i < words * COLS; i += kThreads)  // columns without a row of x
-      *reinterpret_cast<uint4*>(xs + (i / words) * x_bytes + (i % words) * 16) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    for (int i = tid; i < kn / G * COLS; i += kThreads) {
-      const int col = i % COLS, gr = i / COLS;
-      float sum = 0.f;
-#pragma unroll 4
-      for (int w = 0; w < 4 * WL; ++w) {
-        float v[8];
-        Vec16<__nv_bfloat16>::unpack(*reinterpret_cast<const uint4*>(xs + col * x_bytes + (gr * 4 * WL + w) * 16), v);
-        sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-      }
-      sums[gr * COLS + col] = sum;
-    }
-    __syncthreads();
-
-    for (; t < mine && (t * WK + wk) * kStep < k0 + kn; ++t) {
-      cp_async_wait<kRing - 2>();
-      __syncwarp();
-      if (t + kRing - 1 < mine) fetch(t + kRing - 1);
-      cp_async_commit();
-      float fs0[GS], fs1[GS], fb0[GS], fb1[GS];
-#pragma unroll
-      for (int i = 0; i < GS; ++i) {
-        fs0[i] = to_f(s0[i]);
-        fs1[i] = to_f(s1[i]);
-        fb0[i] = fmaf(8.f, fs0[i], to_f(b0[i]));
-        fb1[i] = fmaf(8.f, fs1[i], to_f(b1[i]));
-      }
-      if (t + 1 < mine) fetch_scales(t + 1);
-      const uint32_t st = ring + (t % kRing) * kStageBytes;
-      const int at = (t * WK + wk) * kStep - k0;  // first column of the stage in the chunk
-#pragma unroll
-      for (int gi = 0; gi < GS; ++gi) {
-        uint32_t w0[WL], w1[WL];
-        load_words<WL>(w0, st, g, c, gi);
-        load_words<WL>(w1, st, g + 8, c, gi);
-        float acc[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < WL; ++i) {
-          const uint32_t a0[4] = {nibbles<0>(w0[i]), nibbles<0>(w1[i]), nibbles<4>(w0[i]), nibbles<4>(w1[i])};
-          const uint32_t a1[4] = {nibbles<8>(w0[i]), nibbles<8>(w1[i]), nibbles<12>(w0[i]), nibbles<12>(w1[i])};
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            const uint4 b = *reinterpret_cast<const uint4*>(xs + (j * 8 + g) * x_bytes +
-                                                            ((at / G + gi) * 4 * WL + i * 4 + c) * 16);
-            mma_m16n8k16(acc[j], a0, b.x, b.y);
-            mma_m16n8k16(acc[j], a1, b.z, b.w);
-          }
-        }
+      for (int i = 0; i < WL; ++i) {
+        uint32_t a0[4], a1[4];
+        unpack<EIGHT>(w0[i], a0[0], a0[2]);
+        unpack<EIGHT>(w1[i], a0[1], a0[3]);
+        unpack<EIGHT>(w0[i] >> 8, a1[0], a1[2]);
+        unpack<EIGHT>(w1[i] >> 8, a1[1], a1[3]);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const float2 x2 = *reinterpret_cast<const float2*>(sums + (at / G + gi) * COLS + j * 8 + 2 * c);
-          y[j][0] += fs0[gi] * acc[j][0] + fb0[gi] * x2.x;
-          y[j][1] += fs0[gi] * acc[j][1] + fb0[gi] * x2.y;
-          y[j][2] += fs1[gi] * acc[j][2] + fb1[gi] * x2.x;
-          y[j][3] += fs1[gi] * acc[j][3] + fb1[gi] * x2.y;
+          const uint4 b = lds128(xa + j * 8 * at.x_bytes + gi * (WL * 64) + i * 64);
+          if (i == 0) {
+            mma_f16_first(acc[j], a0, b.x, b.y);
+            mma_f16_first(acd[j], a1, b.z, b.w);
+          } else {
+            mma_f16(acc[j], a0, b.x, b.y);
+            mma_f16(acd[j], a1, b.z, b.w);
+          }
         }
       }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint4 u = lds128(fa + (gi * COLS + j * 8) * 16), v = lds128(fa + (gi * COLS + j * 8) * 16 + 16);
+        const float fu = __uint_as_float(u.x), ou = __uint_as_float(u.y), xu = __uint_as_float(u.z);
+        const float fv = __uint_as_float(v.x), ov = __uint_as_float(v.y), xv = __uint_as_float(v.z);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] += acd[j][e];
+        y[j][0] = fmaf(s0, fmaf(fu, acc[j][0], ou), fmaf(b0, xu, y[j][0]));
+        y[j][1] = fmaf(s0, fmaf(fv, acc[j][1], ov), fmaf(b0, xv, y[j][1]));
+        y[j][2] = fmaf(s1, fmaf(fu, acc[j][2], ou), fmaf(b1, xu, y[j][2]));
+        y[j][3] = fmaf(s1, fmaf(fv, acc[j][3], ov), fmaf(b1, xv, y[j][3]));
+      }
+    }
+    xa += x_step;
+    fa += fa_step;
+    sa += GS * s_group;
+    }
+    st = (st + kStageBytes) & (kRing * kStageBytes - 1);
+    xa += skip * x_step;
+    fa += skip * fa_step;
+    sa += skip * GS * s_group;
+    if (++step == my_stages) {  // the tile is done
+      float* to = part + ((wk * q.warps + tile) * 16 + g) * LD + 2 * c;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          to[8 * (e >> 1) * LD + j * 8 + (e & 1)] += y[j][e];
+          y[j][e] = 0.f;
+        }
+      step = 0;
+      tile += q.warps;
+      xa = x_first;
+      fa = f_first;
+      sa = s_first + (tile - wt) * 32 * (int)sizeof(T);
     }
   }
   cp_async_wait<0>();
-  __syncthreads();
+  // No copy is still landing when the chunk is left (or the CTA).
+  while (parts < kParts && parts * q.part < steps) mbar_wait_bounded(bars + parts++, round & 1, nullptr);
+  }
 
-  // Sums of the k splits and of the parts, in a fixed order; x's space.
-  float* part = reinterpret_cast<float*>(xs);  // [wk][WR * 16][COLS + 1]
-  constexpr int LD = COLS + 1;
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      part[(wk * WR * 16 + wr * 16 + g + 8 * (e >> 1)) * LD + j * 8 + 2 * c + (e & 1)] = y[j][e];
-  __syncthreads();
-  for (int i = tid; i < ms * WR * 16; i += kThreads) {
-    const int r = i % (WR * 16), m = i / (WR * 16), n = blockIdx.x * WR * 16 + r;
+  // Sums of the warps that share tiles (then each has one), of the slabs and
+  // of the parts, in a fixed order.
+  if (q.wk > 1) {
+    __syncthreads();
+    for (int i = tid; i < tiles * 16 * COLS; i += threads) {
+      const int cell = i / COLS * LD + i % COLS;
+      float sum = part[cell];
+      for (int w = 1; w < q.wk; ++w) sum += part[w * q.warps * 16 * LD + cell];
+      part[cell] = sum;
+    }
+  }
+  if (q.split > 1) cluster_sync();
+  else __syncthreads();
+  for (int i = rank * threads + tid; i < ms * tiles * 16; i += q.split * threads) {
+    const int m = i / (tiles * 16), r = i - m * (tiles * 16), n = n0 + r;
     if (n >= p.n) continue;
     float sum = 0.f;
+    for (int o = 0; o < q.split; ++o)
 #pragma unroll
-    for (int w = 0; w < WK; ++w)
-#pragma unroll
-      for (int q = 0; q < P; ++q) sum += part[(w * WR * 16 + r) * LD + m * P + q];
+      for (int h = 0; h < P; ++h) {
+        const float* from = part + r * LD + m * P + h;
+        sum += q.split > 1 ? ld_cluster_f32(from, o) : *from;
+      }
     reinterpret_cast<O*>(p.out)[(m0 + m) * p.out_stride + n] = from_f<O>(sum);
   }
+  if (q.split > 1) cluster_sync();  // nobody leaves while its sums are read
 }
 
 // One warp per group: scale = (max - min) / 15 and bias = min, both rounded to
@@ -292,62 +528,85 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const __grid_constant_
   }
 }
 
-template <typename T, typename O, int G, int NT, int WR>
-cudaError_t q4_run(const Q4Params& p, cudaStream_t s) {
-  constexpr int COLS = NT * 8, WK = kWarps / WR, P = Parts<T>::N;
-  const int rows = COLS / P;  // rows of x per pass
-  const int per = p.m < rows ? p.m : rows;
-  const int unit = kStep * WK;
-  const int padded = (p.k + kStep - 1) / kStep * kStep;
-  int chunk = kChunkElems / COLS / unit * unit;  // columns of x held at a time
-  static_assert(kChunkElems / COLS >= kStep * WK, "a chunk has a stage for every warp");
-  if (chunk > padded) chunk = padded;
-  int body = COLS * (chunk * 2 + 64) + chunk / G * COLS * 4;
-  const int tail = WK * WR * 16 * (COLS + 1) * 4;
-  const int bytes = kWarps * kRing * kStageBytes + (body > tail ? body : tail);
-  constexpr auto K = q4_linear_kernel<T, O, G, NT, WR>;
-  cudaError_t e = allow_smem<K>();
-  if (e != cudaSuccess) return e;
-  const dim3 grid((p.n + WR * 16 - 1) / (WR * 16), (p.m + rows - 1) / rows);
-  K<<<grid, kThreads, bytes, s>>>(p, per, chunk);
-  return cudaGetLastError();
+// The layout on a GPU of `sms` multiprocessors: one CTA per SM, row tiles spread
+// evenly over pairs of CTAs (1025 tiles are 74 pairs of 14), a slab of the
+// columns for each of a pair where there are eight steps or more; fewer tiles
+// or columns at a time where the shared memory asks for it.
+template <typename T, int G, int NT>
+Q4Plan q4_plan(const Q4Params& p, int sms) {
+  const int tiles = (p.n + 15) / 16;
+  Q4Plan q{};
+  q.steps = (p.k + kStep - 1) / kStep;
+  q.rows = min(p.m, NT * 8 / Parts<T>::N);
+  q.split = q.steps >= 8 ? 2 : 1;
+  q.slab = (q.steps + q.split - 1) / q.split;
+  q.chunk = q.slab;
+  const int clusters = max(1, sms / q.split);
+  q.tiles = (tiles + clusters - 1) / clusters;
+  for (;;) {
+    const int per_warp = (q.tiles + kMaxWarps - 1) / kMaxWarps;
+    q.warps = (q.tiles + per_warp - 1) / per_warp;
+    q.wk = max(1, min(kMaxWarps / q.warps, (q.chunk + 1) / 2));
+    q.part = (q.chunk + kParts - 1) / kParts;
+    const Q4Smem<T, G, NT> at(q);
+    if (at.bytes <= kSmemMax || (q.tiles == 1 && q.chunk == 1)) return q;
+    if (q.tiles == 1 || (q.chunk > 1 && at.scales - at.x > kSmemMax / 2)) q.chunk = (q.chunk + 1) / 2;
+    else q.tiles = (q.tiles + 1) / 2;
+  }
 }
 
-// Rows per CTA: as many as still give every SM a CTA (x is read once per CTA).
 template <typename T, typename O, int G, int NT>
-cudaError_t q4_rows(const Q4Params& p, cudaStream_t s) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+cudaError_t q4_run(const Q4Params& p, int sms, size_t* ws_bytes, cudaStream_t s) {
+  const Q4Plan q = q4_plan<T, G, NT>(p, sms);
+  const int passes = (p.m + q.rows - 1) / q.rows;
+  if (ws_bytes) {
+    *ws_bytes = (size_t)passes * Q4Prepared<G, NT>::bytes(q.steps);
+    return cudaSuccess;
+  }
+  constexpr auto K = q4_linear_kernel<T, O, G, NT>;
+  cudaError_t e = allow_smem<K>();
   if (e != cudaSuccess) return e;
-  const int n = op_sm_count(dev);
-  if (p.n > 64 * n) return q4_run<T, O, G, NT, 4>(p, s);
-  if (p.n > 32 * n) return q4_run<T, O, G, NT, 2>(p, s);
-  return q4_run<T, O, G, NT, 1>(p, s);
+  const int words = q.steps * (kStep / 8) * (NT * 8 / Parts<T>::N);
+  q4_prepare_kernel<T, G, NT, sizeof(O) == 4><<<dim3((words + 127) / 128, passes), 128, 0, s>>>(p, q.steps, q.rows);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = q.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(((p.n + 15) / 16 + q.tiles - 1) / q.tiles * q.split, passes);
+  cfg.blockDim = dim3(q.warps * q.wk * 32);
+  cfg.dynamicSmemBytes = Q4Smem<T, G, NT>(q).bytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = q.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, K, p, q);
 }
 
 template <typename T, typename O, int G>
-cudaError_t q4_tiles(const Q4Params& p, cudaStream_t s) {
+cudaError_t q4_tiles(const Q4Params& p, int sms, size_t* ws, cudaStream_t s) {
   const int cols = p.m * Parts<T>::N;
-  if (cols <= 8) return q4_rows<T, O, G, 1>(p, s);
-  if (cols <= 16) return q4_rows<T, O, G, 2>(p, s);
-  if constexpr (Parts<T>::N == 3) {
-    if (cols <= 24) return q4_rows<T, O, G, 3>(p, s);
-  }
-  return q4_rows<T, O, G, 4>(p, s);
+  if (cols <= 8) return q4_run<T, O, G, 1>(p, sms, ws, s);
+  if (cols <= 16) return q4_run<T, O, G, 2>(p, sms, ws, s);
+  return q4_run<T, O, G, 4>(p, sms, ws, s);
 }
 
 template <typename T, typename O>
-cudaError_t q4_group(const Q4Params& p, cudaStream_t s) {
-  if (p.group == 32) return q4_tiles<T, O, 32>(p, s);
-  if (p.group == 64) return q4_tiles<T, O, 64>(p, s);
-  return q4_tiles<T, O, 128>(p, s);
+cudaError_t q4_group(const Q4Params& p, int sms, size_t* ws, cudaStream_t s) {
+  if (p.group == 32) return q4_tiles<T, O, 32>(p, sms, ws, s);
+  if (p.group == 64) return q4_tiles<T, O, 64>(p, sms, ws, s);
+  return q4_tiles<T, O, 128>(p, sms, ws, s);
 }
 
 }  // namespace
 
-cudaError_t launch_q4_linear(const Q4Params& p, int dtype, int out_dtype, cudaStream_t s) {
-  if (dtype == 0) return q4_group<float, float>(p, s);
-  return out_dtype == 0 ? q4_group<__nv_bfloat16, float>(p, s) : q4_group<__nv_bfloat16, __nv_bfloat16>(p, s);
+cudaError_t launch_q4_linear(const Q4Params& p, int dtype, int out_dtype, int sms, size_t* ws_bytes, cudaStream_t s) {
+  if (dtype == 0) return q4_group<float, float>(p, sms, ws_bytes, s);
+  return out_dtype == 0 ? q4_group<__nv_bfloat16, float>(p, sms, ws_bytes, s)
+                        : q4_group<__nv_bfloat16, __nv_bfloat16>(p, sms, ws_bytes, s);
 }
 
 cudaError_t launch_q4_quantize(const Q4PackParams& p, int dtype, cudaStream_t s) {

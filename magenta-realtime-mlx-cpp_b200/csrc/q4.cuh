@@ -15,6 +15,7 @@ struct Q4Params {
   const uint8_t* packed;   // (n, k / 2): column 2 j in the low half of byte j
   const void* scales;      // (n, k / group)
   const void* biases;      // (n, k / group)
+  void* ws;                // x as the product takes it
   void* out;               // (m, n), row stride out_stride elements
   int64_t x_stride, out_stride;
   int m, n, k, group;
@@ -30,7 +31,9 @@ struct Q4PackParams {
 };
 
 // dtype (of x, scales, biases) and out_dtype: MRTDF_DTYPE_*.
-cudaError_t launch_q4_linear(const Q4Params& p, int dtype, int out_dtype, cudaStream_t s);
+// With ws_bytes: only the size of the workspace that the call needs, on a GPU of
+// `sms` multiprocessors.
+cudaError_t launch_q4_linear(const Q4Params& p, int dtype, int out_dtype, int sms, size_t* ws_bytes, cudaStream_t s);
 cudaError_t launch_q4_quantize(const Q4PackParams& p, int dtype, cudaStream_t s);
 
 }  // namespace mrtdf

@@ -18,7 +18,7 @@ _TREE = struct.Struct("@Q" + "Q4q" * 4 + "QQQQQiiif0Q")
 _MASS = struct.Struct("@Q" + "Q4q" * 2 + "QQQQQiiiiff0Q")
 _COMMIT = struct.Struct("@Q" + "Q4q" * 2 + "QQQii0Q")
 _EVICT = struct.Struct("@QQQQQiii0Q")
-_Q4 = struct.Struct("@QQQQQQqq7i0Q")
+_Q4 = struct.Struct("@QQQQQQQQqq7i0Q")
 _PACK = struct.Struct("@QQQQQq5i0Q")
 
 
@@ -52,7 +52,8 @@ class Call:
         self.commit = dict(size=_COMMIT.size, k_new=rows(), v_new=rows(), path=256, lens_out=512, next_pos_out=0, nodes=8,
                            path_len=4)
         self.evict = dict(size=_EVICT.size, mass=256, mass_out=256, pos_out=256, lens_out=512, budget=64, recent=8, sinks=1)
-        self.q4 = dict(size=_Q4.size, x=256, packed=256, scales=256, biases=256, out=256, x_stride=128, out_stride=64, m=2,
+        self.q4 = dict(size=_Q4.size, x=256, packed=256, scales=256, biases=256, out=256, workspace=256, workspace_bytes=1 << 20,
+                       x_stride=128, out_stride=64, m=2,
                        n=64, k=128, group=32, dtype=1, out_dtype=1, device=0)
         self.pack = dict(size=_PACK.size, w=256, packed=256, scales=256, biases=256, w_stride=128, n=4, k=128, group=32,
                          dtype=1, device=0)
@@ -110,7 +111,7 @@ def test_cache_fields_are_checked(ops, what, field, value):
     ("evict", "lens_out", 0, 1), ("evict", "lens_out", 256, 1), ("evict", "budget", 0, 1), ("evict", "recent", -1, 1),
     ("evict", "recent", 64, 1), ("evict", "sinks", -1, 1),
     ("q4", "size", 1, 1), ("q4", "x", 0, 1), ("q4", "x", 264, 1), ("q4", "packed", 0, 1), ("q4", "packed", 260, 1),
-    ("q4", "scales", 0, 1), ("q4", "biases", 0, 1), ("q4", "out", 0, 1), ("q4", "x_stride", 129, 1), ("q4", "out_stride", 63, 1),
+    ("q4", "workspace", 0, 1), ("q4", "workspace", 264, 1), ("q4", "workspace_bytes", 64, 1), ("q4", "scales", 0, 1), ("q4", "biases", 0, 1), ("q4", "out", 0, 1), ("q4", "x_stride", 129, 1), ("q4", "out_stride", 63, 1),
     ("q4", "m", 0, 1), ("q4", "m", 65, 7), ("q4", "n", 0, 1), ("q4", "k", 0, 1), ("q4", "k", 120, 1), ("q4", "k", 1 << 18, 7),
     ("q4", "group", 16, 1), ("q4", "dtype", 3, 1), ("q4", "dtype", 0, 1), ("q4", "out_dtype", 5, 1), ("q4", "device", -1, 1),
     ("pack", "size", 1, 1), ("pack", "w", 0, 1), ("pack", "group", 0, 1), ("pack", "k", 100, 1), ("pack", "w_stride", 100, 1),
