@@ -590,8 +590,8 @@ typedef struct mrtdf_q4_args {
   int64_t x_stride, out_stride;
   int32_t m, n, k, group, dtype, out_dtype, device;
 } mrtdf_q4_args;
-/* Workspace of a call with these sizes (x as the product takes it: some bytes
- * per element of x). args' pointers must be set as for the call, workspace
+/* Workspace of a call with these sizes (x as the product takes it, some bytes
+ * per element of x; 0 where x is small). args' pointers must be set as for the call, workspace
  * aside. */
 int mrtdf_q4_linear_workspace(const mrtdf_q4_args* args, size_t* bytes);
 int mrtdf_q4_linear(const mrtdf_q4_args* args, void* stream);

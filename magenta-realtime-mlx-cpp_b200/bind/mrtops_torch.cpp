@@ -408,10 +408,13 @@ PyObject* q4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     m.device = d.index();
     size_t need = 0;
     check(mrtdf_q4_linear_workspace(&m, &need));
-    const int64_t bytes[1] = {(int64_t)need};
-    at::Tensor ws = fresh(bytes, at::kByte, d);
-    m.workspace = ws.data_ptr();
-    m.workspace_bytes = need;
+    at::Tensor ws;
+    if (need) {
+      const int64_t bytes[1] = {(int64_t)need};
+      ws = fresh(bytes, at::kByte, d);
+      m.workspace = ws.data_ptr();
+      m.workspace_bytes = need;
+    }
     check(mrtdf_q4_linear(&m, stream_of(d)));
     return a[4] == Py_None ? wrap(out) : given(a[4]);
   });

@@ -16,149 +16,12 @@
 // keys; WM warps share a key range with 16 rows each, and the 4 / WM key
 // groups stream their own 16 * WM keys of each tile through a private
 // cp.async ring, so a group waits for nobody until its item ends.
-#include "cache_ops.cuh"
-#include "cache_tile.cuh"
+#include "cache_sched.cuh"
 
 namespace mrtdf {
 namespace {
 
-constexpr int kTile = 64;      // keys per CTA tile
-constexpr int kThreads = 128;  // four warps
 constexpr int kStages = 3;
-
-// ---- schedule ----------------------------------------------------------------
-// A sequence's tiles: ceil((len + nodes) / 64), at least one. A length outside
-// [0, capacity] makes the sequence empty (len -1 here).
-__device__ __forceinline__ int checked_len(const CacheView& c, int b) {
-  const int l = c.lens[b];
-  return l < 0 || l > c.capacity ? -1 : l;
-}
-__device__ __forceinline__ int tiles_of(int len, int extra) { return (max(len, 0) + extra + kTile - 1) / kTile; }
-
-// lens[b] and first[b] = tiles of all items before sequence b's, for b <= B.
-// All 128 threads; ends with a barrier.
-__device__ void build_schedule(const CacheView& c, int batch, int items, int extra, int* lens, int* first) {
-  __shared__ int warp_sum[kThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, per = (batch + kThreads - 1) / kThreads;
-  int sum = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b < batch) {
-      const int l = checked_len(c, b);
-      lens[b] = l;
-      sum += tiles_of(l, extra) * items;
-    }
-  }
-  int run = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += v;
-  }
-  if (lane == 31) warp_sum[tid >> 5] = run;
-  __syncthreads();
-  run -= sum;
-  for (int w = 0; w < (tid >> 5); ++w) run += warp_sum[w];
-  for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b < batch) {
-      first[b] = run;
-      run += tiles_of(lens[b], extra) * items;
-      if (b == batch - 1) first[batch] = run;
-    }
-  }
-  __syncthreads();
-}
-
-// Position in the list of tiles: sequence-major, then outer, inner (an item is
-// one pair of them), then tile.
-struct Cursor {
-  int w, b, outer, inner, tile, tiles, len;
-  __device__ __forceinline__ void seek(int at, const int* lens, const int* first, int batch, int inners, int extra) {
-    w = at;
-    int lo = 0, hi = batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first[mid] <= at) lo = mid;
-      else hi = mid - 1;
-    }
-    b = lo;
-    len = lens[b];
-    tiles = tiles_of(len, extra);
-    const int rem = at - first[b], item = rem / tiles;
-    tile = rem - item * tiles;
-    outer = item / inners;
-    inner = item - outer * inners;
-  }
-  // True when the next tile is another item's.
-  __device__ __forceinline__ bool next(const int* lens, int batch, int outers, int inners, int extra) {
-    ++w;
-    if (++tile < tiles) return false;
-    tile = 0;
-    if (++inner == inners) {
-      inner = 0;
-      if (++outer == outers) {
-        outer = 0;
-        if (++b < batch) {
-          len = lens[b];
-          tiles = tiles_of(len, extra);
-        }
-      }
-    }
-    return true;
-  }
-};
-
-// CTA c of g takes tiles [share(c), share(c + 1)) of `total`.
-__device__ __forceinline__ int share(int c, int g, int total) { return (int)((long long)c * total / g); }
-// The CTA whose run holds tile w.
-__device__ __forceinline__ int owner(int w, int g, int total) {
-  return (int)((((long long)w + 1) * g - 1) / total);
-}
-// CTAs that take part: a run has two tiles or more, or there is one tile each.
-__device__ __forceinline__ int active(int grid, int total) { return max(1, min(grid, total / 2)); }
-
-// ---- the tree ------------------------------------------------------------------
-// seen[i]: bit j set when node j is node i or an ancestor; 0 for a node that is
-// absent (its chain holds a parent outside [-1, i)). One warp; pointer
-// doubling: after k rounds a node knows 2^k links of its chain.
-__device__ void node_masks(unsigned long long* seen, const int32_t* parents, int nodes, bool there, int lane) {
-  constexpr int kRoot = -1, kAbsent = -2;
-  unsigned long long m[2];
-  int up[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = lane + 32 * h;
-    const int p = i < nodes ? (parents ? parents[i] : i - 1) : kAbsent;
-    up[h] = p < kRoot || p >= i ? kAbsent : p;
-    m[h] = 1ull << i;
-  }
-#pragma unroll
-  for (int round = 0; round < 6; ++round) {
-    unsigned long long om[2];
-    int ou[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int from = up[h] & 31;
-      const unsigned long long a = __shfl_sync(0xffffffffu, m[0], from), b = __shfl_sync(0xffffffffu, m[1], from);
-      const int c = __shfl_sync(0xffffffffu, up[0], from), d = __shfl_sync(0xffffffffu, up[1], from);
-      om[h] = up[h] >= 32 ? b : a;
-      ou[h] = up[h] >= 32 ? d : c;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (up[h] >= 0) {
-        m[h] |= om[h];
-        up[h] = ou[h];
-      }
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = lane + 32 * h;
-    seen[i] = there && i < nodes && up[h] == kRoot ? m[h] : 0ull;
-  }
-  __syncwarp();
-}
 
 template <int WM>
 __device__ __forceinline__ void group_sync(int group) {
@@ -182,11 +45,6 @@ __device__ __forceinline__ float2 val2(uint32_t vals, int row, int n, int c, flo
   const uint32_t at = vals + Rows<float, D>::at(row, 2 * n + (c >> 1)) + 8 * (c & 1);
   return make_float2(__uint_as_float(lds32(at)), __uint_as_float(lds32(at + 4)));
 }
-
-__device__ __forceinline__ void store2(__nv_bfloat16* p, float a, float b) {
-  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
-}
-__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 
 // Shared memory of the attention kernel.
 template <typename T, int D, int WM>
@@ -235,7 +93,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   unsigned long long* seen = seen_all + warp * kOpMaxNodes;
   const int batch = p.c.batch, blocks = p.row_blocks, items = p.c.kv_heads * blocks, nodes = p.nodes;
   const int heads_per = p.heads / p.c.kv_heads, rows = heads_per * nodes;
-  build_schedule(p.c, batch, items, nodes, lens, first);
+  build_schedule<false>(p.c, batch, items, nodes, lens, first);
 
   // This CTA's run of tiles.
   const int total = first[batch];
@@ -255,7 +113,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
     auto start = [&](int i) {
       if (i == all) return total;
       const int b = i / items;
-      return first[b] + (i - b * items) * tiles_of(lens[b], nodes);
+      return first[b] + (i - b * items) * tiles_of<false>(lens[b], nodes);
     };
     w0 = start(i0);
     w1 = start(i1);
@@ -274,7 +132,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   const int r0 = gt / CH, ch = gt % CH;
   const uint32_t x0 = (uint32_t)((ch ^ (r0 & 7)) << 4);
   const int64_t row_step = (int64_t)RS * p.c.st;
-  Cursor ahead;
+  Cursor<false> ahead;
   const T *kb = nullptr, *vb = nullptr;  // this lane's chunk of row 0 of ahead's item
   auto enter = [&] {
     const int64_t at = ahead.b * p.c.sb + ahead.outer * p.c.sh + ch * (16 / (int)sizeof(T));
@@ -315,7 +173,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   };
 
   ahead.seek(w0, lens, first, batch, blocks, nodes);
-  Cursor cur = ahead;
+  Cursor<false> cur = ahead;
   enter();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
@@ -618,58 +476,6 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   pdl_launch_dependents();
 }
 
-// Joins the partial rows of items that several CTAs worked on: a warp per row.
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_constant__ TreeParams p, int mb) {
-  extern __shared__ __align__(16) int sched[];
-  int *lens = sched, *first = sched + p.c.batch;
-  const int items = p.c.kv_heads * p.row_blocks, nodes = p.nodes;
-  build_schedule(p.c, p.c.batch, items, nodes, lens, first);
-  const int b = blockIdx.x / items, item = blockIdx.x % items, total = first[p.c.batch];
-  const int parts = active(p.grid, total), tiles = tiles_of(lens[b], nodes), w = first[b] + item * tiles;
-  const int c0 = owner(w, parts, total), c1 = owner(w + tiles - 1, parts, total);
-  pdl_wait();
-  if (c0 == c1) return;
-  const int lane = threadIdx.x & 31, r = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5);
-  const int heads_per = p.heads / p.c.kv_heads, row = (item % p.row_blocks) * mb + r;
-  if (r >= mb || row >= heads_per * nodes) return;
-  auto part = [&](int c) { return p.ws + (int64_t)(c * 2 + (c == c0)) * mb * (D + 2); };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part(c)[mb * D + r]);
-  m = warp_max(m);
-  const float u = m == -INFINITY ? 0.f : m;
-  constexpr int V = D / 32;
-  float acc[V] = {}, sum = 0.f;
-  for (int cb = c0; cb <= c1; cb += 32) {
-    const int mine = cb + lane;
-    float wt = 0.f;
-    if (mine <= c1) {
-      wt = ex2((part(mine)[mb * D + r] - u) * kLog2e);
-      const float l = part(mine)[mb * D + mb + r];
-      sum += l == 0.f ? 0.f : l * wt;
-    }
-    const int n = min(32, c1 - cb + 1);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float f = __shfl_sync(0xffffffffu, wt, i);
-      const float* src = part(cb + i) + r * D + lane * V;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float v = src[k];
-        if (!(f == 0.f)) acc[k] += v * f;
-      }
-    }
-  }
-  sum = warp_sum(sum);
-  const int hd = row / nodes, n = row - hd * nodes, head = (item / p.row_blocks) * heads_per + hd;
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + n * p.out.sn + lane * V;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int k = 0; k < V; k += 2)
-    store2(dst + k, sum == 0.f ? 0.f : acc[k] * inv, sum == 0.f ? 0.f : acc[k + 1] * inv);
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + head) * nodes + n] = sum == 0.f ? -INFINITY : m + logf(sum);
-}
-
 // ---- collected weight ------------------------------------------------------------
 // mass_out[t] = decay mass[t] + sum over the accepted path's rows (head, i) of
 // exp(x_t - lse) for cached rows t < len, and for the path's own rows, which
@@ -734,13 +540,13 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   const int batch = p.c.batch, kv = p.c.kv_heads, items = p.c.layers * kv, extra = p.path_len;
   const int heads_per = p.heads / p.c.kv_heads;
-  build_schedule(p.c, batch, items, extra, lens, first);
+  build_schedule<false>(p.c, batch, items, extra, lens, first);
   const int total = first[batch], parts = active(p.grid, total);
   if ((int)blockIdx.x >= parts) return;
   const int w0 = share(blockIdx.x, parts, total), w1 = share(blockIdx.x + 1, parts, total);
   const uint32_t ring = smem_u32(smem) + warp * (16 * R::kBytes);
 
-  Cursor cur;
+  Cursor<false> cur;
   cur.seek(w0, lens, first, batch, kv, extra);
   while (cur.w < w1) {
     // One item's run of tiles [t0, t1): layer, sequence, kv head.
@@ -903,7 +709,7 @@ cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, p, 16 * WM);
+  return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D, false>, p, 16 * WM);
 }
 
 template <typename T, int D, bool BIAS>
@@ -935,11 +741,18 @@ int tree_smem(const TreeParams& p, int wm) {
 }
 
 constexpr int kSmSmem = 227 * 1024;
+// Rows and capacity above which the tcgen05 kernel takes bf16 calls.
+constexpr int kTcRows = 16, kTcCapacity = 256;
 
 }  // namespace
 
 cudaError_t plan_tree_attention(TreeParams& p, int sms, size_t* ws_floats) {
   const int wm = tree_wm(p), mb = 16 * wm, rows = p.heads / p.c.kv_heads * p.nodes;
+  p.tc = rows > kTcRows && p.c.capacity > kTcCapacity && tree_attention_tc_takes(p);
+  if (p.tc) {
+    plan_tree_attention_tc(p, sms, ws_floats);
+    return cudaSuccess;
+  }
   p.row_blocks = (rows + mb - 1) / mb;
   const int items = p.c.batch * p.c.kv_heads * p.row_blocks;
   const int per_sm = max(1, min(p.rel_bias && p.c.dtype != 0 ? 3 : 4, kSmSmem / (tree_smem(p, wm) + 1024)));
@@ -952,6 +765,7 @@ cudaError_t plan_tree_attention(TreeParams& p, int sms, size_t* ws_floats) {
 }
 
 cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t s) {
+  if (p.tc) return launch_tree_attention_tc(p, s);
   const int wm = tree_wm(p);
   if (p.c.dtype == 0) return p.c.head_dim == 64 ? tree_variant<float, 64>(p, wm, s) : tree_variant<float, 128>(p, wm, s);
   return p.c.head_dim == 64 ? tree_variant<__nv_bfloat16, 64>(p, wm, s) : tree_variant<__nv_bfloat16, 128>(p, wm, s);

@@ -1,0 +1,549 @@
+// Attention of a drafted tree over a KV cache (bf16) on the 5th-generation
+// tensor cores, for trees and head groups of more than a few rows. The
+// mathematics is that of cache_attn.cu.
+//
+// The rows of one kv head (nodes x its query heads) are the M side of
+// tcgen05.mma, 128 at a time. With 128 rows a tile of 64 keys takes 512 clocks
+// of products (head_dim 128) and its 32 KB of K and V come in 1400 at the
+// memory's rate, so padding to 128 rows costs nothing while the cache is read
+// from HBM; mma.sync, which a quarter of the rate is left of, took 4 times
+// that at 96 rows.
+//
+// CTA of 320 threads, one per SM, over an equal run of the key tiles of all
+// items (cache_sched.cuh); roles and hand-over as in enc_attn_tc.cu:
+//   warps 0-7  softmax: two threads per query row, each with 32 of a tile's
+//              64 key columns, a running maximum and an accumulator of its own
+//              (rows that do not exist skip the work: their weights are zero
+//              from the start);
+//   warp 8     TMA producer: K and V tiles through a ring, 128-byte swizzle,
+//              over the items of the run without a stop;
+//   warp 9     MMA issuer: S = Q K^T into one of two TMEM buffers, then
+//              O_h += P_h V for the two key halves h, weights as two bf16
+//              parts (16 bits of a weight; the second product is hidden too).
+// A maximum is raised only when a tile exceeds it by 8 units of its scale.
+// The drafted rows are a tile of their own behind the cached ones.
+//
+// Values that no row sees must not meet the products, where 0 x NaN is NaN:
+// rows behind the length are zeroed in the last cached tile, and in the drafted
+// tile single values that are not finite, which the rows that do see them take
+// from global memory at the end.
+#include <cuda.h>
+
+#include "cache_sched.cuh"
+#include "tcgen05.cuh"
+
+namespace mrtdf {
+namespace {
+
+using namespace tcg;
+typedef __nv_bfloat16 bf16;
+
+constexpr int kRows = 128;
+constexpr int kSoft = 256;              // softmax threads
+constexpr int kTcThreads = kSoft + 64;  // and the TMA and MMA warps
+constexpr int kSub = 64 * 128;          // 64 rows of 128 bytes (64 columns)
+constexpr int kPBytes = kRows * 128;    // one part of the weights of a tile
+constexpr float kLazy = 8.f;
+
+template <int D>
+struct TcCfg {
+  static constexpr int kSubs = D / 64;  // 64-column parts of a row
+  static constexpr int kStagesKv = D == 64 ? 4 : 3;
+  static constexpr int kQBytes = kRows * D * 2, kKvBytes = kSub * kSubs;
+  static constexpr int kOffQ = 0, kOffKv = kQBytes, kOffP = kOffKv + kStagesKv * 2 * kKvBytes;
+  static constexpr int kOffBar = kOffP + 2 * 2 * kPBytes;  // two buffers of two parts
+  static constexpr int kOffSched = kOffBar + 256;
+  static int smem(int batch) { return kOffSched + (2 * batch + 1) * 4 + 1024; }
+  static constexpr uint32_t kTmem = D == 64 ? 256 : 512;  // S 2 x 64, O 2 x D columns
+};
+// kind::f16, D f32, A / B bf16, M 128, N 64, K-major; PV: B MN-major.
+constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+constexpr uint32_t kIdescPv = kIdesc | (1u << 16);
+
+struct TcMaps {
+  CUtensorMap k, v, kn, vn;
+};
+
+__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ uint32_t sw128(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+
+template <int D, bool BIAS>
+__global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __grid_constant__ TcMaps maps,
+                                                                       const __grid_constant__ TreeParams p) {
+  using C = TcCfg<D>;
+  constexpr int NS = C::kStagesKv, SUBS = C::kSubs;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t *q_full = bar, *o_done = bar + 1, *drain = bar + 2, *kv_full = bar + 3, *kv_empty = bar + 3 + NS;
+  uint64_t *s_full = bar + 3 + 2 * NS, *s_empty = s_full + 2, *p_full = s_full + 4, *p_empty = s_full + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 8);
+  int* lens = reinterpret_cast<int*>(smem + C::kOffSched);
+  int* first = lens + p.c.batch;
+  __shared__ int abort_flag;
+  __shared__ unsigned long long seen[kOpMaxNodes], poison;
+  __shared__ float xm[2][kRows], xl[2][kRows];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int batch = p.c.batch, blocks = p.row_blocks, items = p.c.kv_heads * blocks, nodes = p.nodes;
+  const int heads_per = p.heads / p.c.kv_heads, rows = heads_per * nodes;
+
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 32) {
+    mbar_init(q_full, kSoft);
+    mbar_init(o_done, 1);
+    mbar_init(drain, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(kv_full + i, 1);
+      mbar_init(kv_empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(s_empty + i, kSoft);
+      mbar_init(p_full + i, kSoft);
+      mbar_init(p_empty + i, 1);
+    }
+    fence_mbar_init();
+    abort_flag = 0;
+  }
+  // Weights of rows that do not exist stay zero.
+  for (int i = tid; i < 4 * kPBytes / 16; i += kTcThreads)
+    reinterpret_cast<uint4*>(smem + C::kOffP)[i] = make_uint4(0, 0, 0, 0);
+  fence_async();
+  tc_fence_before();
+  build_schedule<true>(p.c, batch, items, nodes, lens, first);  // ends with a barrier
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int total = first[batch], parts = active(p.grid, total);
+  const bool idle = (int)blockIdx.x >= parts;
+  const int w0 = idle ? 0 : share(blockIdx.x, parts, total), w1 = idle ? 0 : share(blockIdx.x + 1, parts, total);
+  Cursor<true> cur;
+  cur.seek(w0, lens, first, batch, blocks, nodes);
+
+  auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
+    if (*(volatile int*)&abort_flag) return false;
+    if (mbar_wait_bounded(b, parity, nullptr)) return true;
+    *(volatile int*)&abort_flag = 1;
+    return false;
+  };
+
+  if (idle) {
+  } else if (warp == kSoft / 32) {
+    // ---- TMA producer ----
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; cur.w < w1; ++i) {
+        const int st = i % NS;
+        if (i >= NS && !wait(kv_empty + st, (uint32_t)((i / NS - 1) & 1))) break;
+        uint8_t* ks = smem + C::kOffKv + st * 2 * C::kKvBytes;
+        const bool fresh = cur.tile + 1 == cur.tiles;  // the drafted rows
+        mbar_arrive_expect_tx(kv_full + st, 2 * C::kKvBytes);
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) {
+          const int row = fresh ? 0 : cur.tile * kTile;
+          tma_load_4d(ks + u * kSub, fresh ? &maps.kn : &maps.k, u * 64, row, cur.outer, cur.b, kv_full + st);
+          tma_load_4d(ks + C::kKvBytes + u * kSub, fresh ? &maps.vn : &maps.v, u * 64, row, cur.outer, cur.b, kv_full + st);
+        }
+        issued = i + 1;
+        cur.next(lens, batch, p.c.kv_heads, blocks, nodes);
+      }
+      // No copy may still be landing when the CTA exits.
+      for (int i = max(0, issued - NS); i < issued; ++i) mbar_wait_bounded(kv_full + i % NS, (uint32_t)((i / NS) & 1), nullptr);
+    }
+  } else if (warp == kSoft / 32 + 1) {
+    // ---- MMA issuer ----
+    if (lane == 0) {
+      const uint32_t aq = smem_u32(smem + C::kOffQ);
+      bool ok = true;
+      auto issue_s = [&](int i) -> bool {
+        const int st = i % NS, sb = i & 1;
+        if (!wait(kv_full + st, (uint32_t)((i / NS) & 1))) return false;
+        if (i >= 2 && !wait(s_empty + sb, (uint32_t)(((i >> 1) - 1) & 1))) return false;
+        tc_fence_after();
+        const uint32_t ak = smem_u32(smem + C::kOffKv + st * 2 * C::kKvBytes);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma(tmem + (uint32_t)(sb * 64), smem_desc_sw128(aq + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
+               smem_desc_sw128(ak + (kk >> 2) * kSub + (kk & 3) * 32), kIdesc, kk != 0);
+        mma_commit(s_full + sb);
+        return true;
+      };
+      int i = 0;
+      for (int seg = 0; ok && cur.w < w1; ++seg) {
+        const int n = min(cur.tiles - cur.tile, w1 - cur.w);  // tiles of the item's run
+        if (!(ok = wait(q_full, (uint32_t)(seg & 1)))) break;
+        ok = issue_s(i);
+        for (int t = 0; ok && t < n; ++t, ++i) {
+          if (t + 1 < n && !(ok = issue_s(i + 1))) break;
+          const int st = i % NS, pb = i & 1;
+          if (!(ok = wait(p_full + pb, (uint32_t)((i >> 1) & 1)))) break;
+          tc_fence_after();
+          const uint32_t ap = smem_u32(smem + C::kOffP + pb * 2 * kPBytes);
+          const uint32_t av = smem_u32(smem + C::kOffKv + st * 2 * C::kKvBytes + C::kKvBytes);
+          // Slices 0, 1 of 16 keys go to O_0, slices 2, 3 to O_1.
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+              for (int u = 0; u < SUBS; ++u)
+                umma(tmem + 128 + (uint32_t)((kk >> 1) * D + u * 64), smem_desc_sw128(ap + part * kPBytes + kk * 32),
+                     smem_desc_sw128(av + u * kSub + kk * 2048), kIdescPv, (part || t != 0 || (kk & 1)) ? 1u : 0u);
+          mma_commit(p_empty + pb);
+          mma_commit(kv_empty + st);
+        }
+        if (ok) mma_commit(o_done);
+        // To the next item.
+        cur.w += n - 1;
+        cur.tile += n - 1;
+        cur.next(lens, batch, p.c.kv_heads, blocks, nodes);
+      }
+      // Every product issued so far has retired before TMEM is released.
+      mma_commit(drain);
+      mbar_wait_bounded(drain, 0, nullptr);
+    }
+  } else {
+    // ---- softmax ----
+    const int row = tid & (kRows - 1), half = tid >> 7;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const int c0 = half * 32;
+    const uint32_t ocol = 128u + (uint32_t)(half * D);
+    constexpr bool POW2 = !BIAS;
+    const float unit = POW2 ? p.scale * kLog2e : p.scale;
+    auto weight = [](float x) { return ex2(POW2 ? x : x * kLog2e); };
+    auto soft_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory"); };
+    bool ok = true;
+    int i = 0, masks_of = -1;
+    for (int seg = 0; cur.w < w1; ++seg) {
+      const int n = min(cur.tiles - cur.tile, w1 - cur.w), first_tile = cur.tile, kvh = cur.outer, b = cur.b;
+      const int len = max(cur.len, 0), row0 = cur.inner * kRows, here = min(kRows, rows - row0);
+      const bool last = first_tile + n == cur.tiles, live = (warp & 3) * 32 < here;
+      // The item's rows: into shared memory, and this thread's own.
+      if (masks_of != b) {
+        masks_of = b;
+        if (warp == 0) node_masks(seen, p.parents ? p.parents + b * nodes : nullptr, nodes, cur.len >= 0, lane);
+      }
+      if (tid == 0) poison = 0;
+      for (int x = tid; x < kRows * (D / 8); x += kSoft) {
+        const int r = x / (D / 8), ch = x % (D / 8);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < here) {
+          const int hd = (row0 + r) / nodes, nd = row0 + r - hd * nodes;
+          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(p.q.ptr) + b * p.q.sb +
+                                              (kvh * heads_per + hd) * p.q.sh + nd * p.q.sn + ch * 8);
+        }
+        *reinterpret_cast<uint4*>(smem + C::kOffQ + (ch >> 3) * (kRows * 128) + sw128(r, ch & 7)) = v;
+      }
+      fence_async();
+      arrive(q_full);
+      soft_sync();  // the masks
+      const int hd = (row0 + row) / nodes, nd = row0 + row - hd * nodes, head = kvh * heads_per + hd;
+      const unsigned long long see = row < here ? seen[nd] : 0ull;
+      const int next = p.c.next_pos ? p.c.next_pos[b] : len, at = (int)((unsigned)next + (unsigned)(see ? __popcll(see) - 1 : 0));
+      const float* tab = BIAS ? p.rel_bias + (row < here ? (int64_t)head * p.rel_len : 0) : nullptr;
+      const float far = BIAS ? tab[p.rel_len - 1] : 0.f;
+      const int32_t* ps = BIAS && p.c.pos ? p.c.pos + (int64_t)(b * p.c.kv_heads + kvh) * p.c.capacity : nullptr;
+
+      float m = -INFINITY, l = 0.f;
+      for (int t = 0; t < n; ++t, ++i) {
+        const int tile = first_tile + t, sb = i & 1, pb = i & 1, st = i % NS;
+        const bool fresh = tile + 1 == cur.tiles;
+        const int key0 = tile * kTile + c0, valid = fresh ? nodes - c0 : len - key0;  // columns of mine that exist
+        // Positions of this half's keys, one per lane.
+        int mine = 0;
+        bool near = false;
+        if (BIAS) {
+          const int k = key0 + lane;
+          if (fresh) {
+            const unsigned long long s = c0 + lane < nodes ? seen[c0 + lane] : 0ull;
+            mine = (int)((unsigned)next + (unsigned)(s ? __popcll(s) - 1 : 0));
+          } else {
+            mine = ps ? ps[min(k, max(len - 1, 0))] : k;
+          }
+          near = __any_sync(0xffffffffu, lane < valid && (int)((unsigned)next - (unsigned)mine) < p.rel_len - 1);
+        }
+        if (ok) ok = wait(s_full + sb, (uint32_t)((i >> 1) & 1));
+        // The TMEM accesses below are .sync.aligned: decide warp-uniformly.
+        ok = __all_sync(0xffffffffu, ok) != 0;
+        if (ok) {
+          tc_fence_after();
+          float x[32];
+          if (live) {
+            tmem_ld16(tmem + lane_base + (uint32_t)(sb * 64 + c0), reinterpret_cast<uint32_t*>(x));
+            tmem_ld16(tmem + lane_base + (uint32_t)(sb * 64 + c0 + 16), reinterpret_cast<uint32_t*>(x) + 16);
+            tmem_wait_ld();
+          }
+          tc_fence_before();
+          arrive(s_empty + sb);
+          // Values that must not meet the products.
+          if (fresh || (tile + 1) * kTile > len) {
+            if ((ok = __all_sync(0xffffffffu, wait(kv_full + st, (uint32_t)((i / NS) & 1))) != 0)) {
+              uint8_t* vs = smem + C::kOffKv + st * 2 * C::kKvBytes + C::kKvBytes;
+              for (int x4 = tid; x4 < kTile * (D / 8); x4 += kSoft) {
+                const int r = x4 / (D / 8), ch = x4 % (D / 8);
+                uint4* v4 = reinterpret_cast<uint4*>(vs + (ch >> 3) * kSub + sw128(r, ch & 7));
+                if (!fresh) {
+                  if (tile * kTile + r >= len) *v4 = make_uint4(0, 0, 0, 0);
+                } else {
+                  uint4 v = *v4;
+                  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+                  bool bad = false;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, bad = true;
+                    if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, bad = true;
+                  }
+                  if (bad) {
+                    *v4 = v;
+                    if (r < nodes) atomicOr(&poison, 1ull << r);
+                  }
+                }
+              }
+            }
+          }
+          if (live && ok) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] *= unit;
+            if (BIAS) {
+              if (near) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const int pos = __shfl_sync(0xffffffffu, mine, e);
+                  x[e] += __ldg(tab + min(max((int)((unsigned)at - (unsigned)pos), 0), p.rel_len - 1));
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] += far;
+              }
+            }
+            if (fresh) {
+              const uint32_t bits = (uint32_t)(see >> c0);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(bits >> e & 1)) x[e] = -INFINITY;
+            } else if (valid < 32 || !see) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (e >= valid || !see) x[e] = -INFINITY;
+            }
+            float mt = x[0];
+#pragma unroll
+            for (int e = 1; e < 32; ++e) mt = fmaxf(mt, x[e]);
+            float alpha = 1.f;
+            bool scale = false;
+            if (mt > m + kLazy) {  // also the first tile with a key (m = -inf)
+              if (m != -INFINITY) {
+                alpha = weight(m - mt);
+                scale = true;
+              }
+              m = mt;
+              l *= alpha;
+            }
+            if (__any_sync(0xffffffffu, scale)) {
+              // O holds products made with the old maximum: scale it once the
+              // last of them has retired (an earlier tile of this item).
+              ok = __all_sync(0xffffffffu, wait(p_empty + ((i - 1) & 1), (uint32_t)(((i - 1) >> 1) & 1))) != 0;
+              if (ok) {
+                tc_fence_after();
+#pragma unroll
+                for (int cc = 0; cc < D; cc += 16) {
+                  uint32_t o[16];
+                  tmem_ld16(tmem + lane_base + ocol + (uint32_t)cc, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                  tmem_st16(tmem + lane_base + ocol + (uint32_t)cc, o);
+                }
+                tmem_wait_st();
+              }
+            }
+            if (ok && i >= 2) ok = __all_sync(0xffffffffu, wait(p_empty + pb, (uint32_t)(((i >> 1) - 1) & 1))) != 0;
+            if (ok) {
+              uint8_t* ph = smem + C::kOffP + pb * 2 * kPBytes;
+              const float u = m == -INFINITY ? 0.f : m;
+              float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int cc = 0; cc < 32; cc += 8) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float a = weight(x[cc + 2 * e] - u), d = weight(x[cc + 2 * e + 1] - u);
+                  sum[e] += a + d;
+                  hi[e] = pack_bf16(a, d);
+                  lo[e] = pack_bf16(a - __uint_as_float(hi[e] << 16), d - __uint_as_float(hi[e] & 0xffff0000u));
+                }
+                const uint32_t to = sw128(row, (c0 + cc) >> 3);
+                *reinterpret_cast<uint4*>(ph + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(ph + kPBytes + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              }
+              l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+          }
+          tc_fence_before();
+          fence_async();
+          arrive(p_full + pb);
+        }
+      }
+      if (ok) ok = wait(o_done, (uint32_t)(seg & 1));
+      ok = __all_sync(0xffffffffu, ok) != 0;
+      // Join the halves; every softmax thread passes here once per item.
+      xm[half][row] = m;
+      xl[half][row] = l;
+      soft_sync();
+      const float m0 = xm[0][row], m1 = xm[1][row], mx = fmaxf(m0, m1), u = mx == -INFINITY ? 0.f : mx;
+      const float a0 = weight(m0 - u), a1 = weight(m1 - u), sum = xl[0][row] * a0 + xl[1][row] * a1;
+      const float mn = POW2 ? mx * kLn2 : mx;
+      const bool whole = first_tile == 0 && last, empty = !see || sum == 0.f;
+      const unsigned long long bad = last ? poison & see : 0ull;
+      if (live) {
+        tc_fence_after();
+        const float inv = !ok ? NAN : empty ? 0.f : whole ? 1.f / sum : 1.f;
+        float* part = p.ws + (int64_t)(blockIdx.x * 2 + (first_tile == 0)) * kRows * (D + 2) + row * D;
+        bf16* out = row < here ? reinterpret_cast<bf16*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + nd * p.out.sn
+                               : nullptr;
+        // Columns [half * D / 2, + D / 2) of this row.
+#pragma unroll
+        for (int cc = 0; cc < D / 2; cc += 16) {
+          const int col = half * (D / 2) + cc;
+          float o0[16], o1[16];
+          tmem_ld16(tmem + lane_base + 128u + (uint32_t)col, reinterpret_cast<uint32_t*>(o0));
+          tmem_ld16(tmem + lane_base + 128u + (uint32_t)(D + col), reinterpret_cast<uint32_t*>(o1));
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o0[e] = empty && ok ? 0.f : (o0[e] * a0 + o1[e] * a1) * inv;
+          for (unsigned long long s = bad; s; s &= s - 1) {
+            const int j = __ffsll((long long)s) - 1;
+            const bf16* vr = reinterpret_cast<const bf16*>(p.v_new.ptr) + b * p.v_new.sb + kvh * p.v_new.sh + j * p.v_new.sn + col;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float v = to_f(vr[e]);
+              if (!(fabsf(v) < INFINITY)) o0[e] += v;
+            }
+          }
+          if (row < here) {
+            if (whole) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = pack_bf16(o0[2 * e], o0[2 * e + 1]);
+              *reinterpret_cast<uint4*>(out + col) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(out + col + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) store2(part + col + e, o0[e], o0[e + 1]);
+            }
+          }
+        }
+        if (row < here && half == 0) {
+          if (whole) {
+            if (p.lse) p.lse[((int64_t)b * p.heads + head) * nodes + nd] = !ok ? NAN : empty ? -INFINITY : mn + logf(sum);
+          } else {
+            float* stat = p.ws + (int64_t)(blockIdx.x * 2 + (first_tile == 0)) * kRows * (D + 2) + kRows * D;
+            stat[row] = empty ? -INFINITY : mn;
+            stat[kRows + row] = !ok ? NAN : empty ? 0.f : sum;
+          }
+        }
+      }
+      tc_fence_before();
+      soft_sync();  // xm, xl, seen and poison are used again
+      cur.w += n - 1;
+      cur.tile += n - 1;
+      cur.next(lens, batch, p.c.kv_heads, blocks, nodes);
+    }
+  }
+  pdl_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+  }
+}
+
+// A tensor map of (head_dim, rows, heads, batch) rows: boxes of 64 columns x 64
+// rows, 128-byte swizzle, zeros outside. Strides of dimensions of one element
+// are set to a row's bytes.
+bool make_map(CUtensorMap* m, const void* base, int d, int64_t rows, int heads, int batch, int64_t sn, int64_t sh, int64_t sb) {
+  auto fn = encode_tiled_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
+  const cuuint64_t row = (cuuint64_t)d * 2;
+  const cuuint64_t strides[3] = {sn ? (cuuint64_t)sn * 2 : row, sh ? (cuuint64_t)sh * 2 : row, sb ? (cuuint64_t)sb * 2 : row};
+  const cuuint32_t box[4] = {64, 64, 1, 1}, step[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BIAS>
+cudaError_t tc_run(const TreeParams& p, cudaStream_t s) {
+  TcMaps maps;
+  const CacheView& c = p.c;
+  if (!make_map(&maps.k, c.k, D, c.capacity, c.kv_heads, c.batch, c.st, c.sh, c.sb) ||
+      !make_map(&maps.v, c.v, D, c.capacity, c.kv_heads, c.batch, c.st, c.sh, c.sb) ||
+      !make_map(&maps.kn, p.k_new.ptr, D, p.nodes, c.kv_heads, c.batch, p.k_new.sn, p.k_new.sh, p.k_new.sb) ||
+      !make_map(&maps.vn, p.v_new.ptr, D, p.nodes, c.kv_heads, c.batch, p.v_new.sn, p.v_new.sh, p.v_new.sb))
+    return cudaErrorInvalidValue;
+  constexpr auto K = tree_attn_tc_kernel<D, BIAS>;
+  constexpr int kMost = 220 * 1024;
+  static_assert(TcCfg<D>::kOffSched + (2 * kOpMaxBatch + 1) * 4 + 1024 <= kMost, "fits");
+  cudaError_t e = allow_smem<K, kMost>();
+  if (e != cudaSuccess) return e;
+  K<<<p.grid, kTcThreads, TcCfg<D>::smem(c.batch), s>>>(maps, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(c.batch * c.kv_heads * p.row_blocks, kRows / 4);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (2 * c.batch + 1) * 4;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tree_join_kernel<bf16, D, true>, p, kRows);
+}
+
+}  // namespace
+
+// Strides that a tensor map takes: not zero where there is more than one
+// element (an expanded tensor).
+bool tree_attention_tc_takes(const TreeParams& p) {
+  const CacheView& c = p.c;
+  auto fits = [&](int64_t stride, int64_t extent) { return extent <= 1 || stride > 0; };
+  return c.dtype != 0 && fits(c.st, c.capacity) && fits(c.sh, c.kv_heads) && fits(c.sb, c.batch) &&
+         fits(p.k_new.sn, p.nodes) && fits(p.k_new.sh, c.kv_heads) && fits(p.k_new.sb, c.batch) && fits(p.v_new.sn, p.nodes) &&
+         fits(p.v_new.sh, c.kv_heads) && fits(p.v_new.sb, c.batch);
+}
+
+void plan_tree_attention_tc(TreeParams& p, int sms, size_t* ws_floats) {
+  const int rows = p.heads / p.c.kv_heads * p.nodes;
+  p.row_blocks = (rows + kRows - 1) / kRows;
+  const long long items = (long long)p.c.batch * p.c.kv_heads * p.row_blocks, most = (p.c.capacity + kTile - 1) / kTile + 1;
+  p.stream = 1;
+  p.grid = (int)min((long long)sms, max(1ll, items * most / 2));
+  *ws_floats = (size_t)p.grid * 2 * kRows * (p.c.head_dim + 2);
+}
+
+cudaError_t launch_tree_attention_tc(const TreeParams& p, cudaStream_t s) {
+  if (p.c.head_dim == 64) return p.rel_bias ? tc_run<64, true>(p, s) : tc_run<64, false>(p, s);
+  return p.rel_bias ? tc_run<128, true>(p, s) : tc_run<128, false>(p, s);
+}
+
+}  // namespace mrtdf

@@ -324,10 +324,12 @@ int mrtdf_q4_linear(const mrtdf_q4_args* a, void* stream) {
     size_t need = 0;
     const int sms = op_sm_count(a->device);
     cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, &need, nullptr), op);
-    if (!a->workspace || a->workspace_bytes < need)
-      invalid("q4_linear: the workspace is smaller than mrtdf_q4_linear_workspace says (" + std::to_string(need) + " bytes)");
-    if (!aligned16(a->workspace)) invalid("q4_linear: the workspace must be 16-byte aligned");
-    p.ws = a->workspace;
+    if (need) {
+      if (!a->workspace || a->workspace_bytes < need)
+        invalid("q4_linear: the workspace is smaller than mrtdf_q4_linear_workspace says (" + std::to_string(need) + " bytes)");
+      if (!aligned16(a->workspace)) invalid("q4_linear: the workspace must be 16-byte aligned");
+      p.ws = a->workspace;
+    }
     DeviceScope on(a->device, op);
     cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, nullptr, static_cast<cudaStream_t>(stream)), op);
   });

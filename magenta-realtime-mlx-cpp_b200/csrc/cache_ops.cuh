@@ -10,10 +10,10 @@
 
 namespace mrtdf {
 
-// Lets kernel `K` use up to kOpMaxSmem bytes of dynamic shared memory on the
-// current device; the attribute is set once per device.
+// Lets kernel `K` use up to `BYTES` of dynamic shared memory (next to a little
+// static) on the current device; the attribute is set once per device.
 constexpr int kOpMaxSmem = 226 * 1024;
-template <auto K>
+template <auto K, int BYTES = kOpMaxSmem>
 cudaError_t allow_smem() {
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -21,7 +21,7 @@ cudaError_t allow_smem() {
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, kOpMaxSmem);
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
@@ -59,6 +59,7 @@ struct TreeParams {
   float scale;
   int grid;       // CTAs of the attention kernel
   int row_blocks; // blocks of query rows per (sequence, kv head)
+  int tc;         // 1: the tcgen05 kernel
   int stream;     // 1: equal runs of key tiles per CTA, joined afterwards; 0: whole items
 };
 
@@ -100,6 +101,10 @@ int op_sm_count(int device);
 // of `sms` multiprocessors; gives the floats of workspace the launch needs.
 cudaError_t plan_tree_attention(TreeParams& p, int sms, size_t* ws_floats);
 cudaError_t launch_tree_attention(const TreeParams& p, cudaStream_t s);
+// The tcgen05 kernel's part of the two (cache_attn_tc.cu).
+bool tree_attention_tc_takes(const TreeParams& p);
+void plan_tree_attention_tc(TreeParams& p, int sms, size_t* ws_floats);
+cudaError_t launch_tree_attention_tc(const TreeParams& p, cudaStream_t s);
 cudaError_t launch_cache_mass(MassParams& p, cudaStream_t s);
 cudaError_t launch_cache_commit(const CommitParams& p, cudaStream_t s);
 cudaError_t launch_cache_evict(const EvictParams& p, cudaStream_t s);

@@ -1,0 +1,212 @@
+// How the attention over a cache is spread over the GPU, shared by its kernels
+// (cache_attn.cu, cache_attn_tc.cu): a list of key tiles of all (sequence, kv
+// head, row block) items, equal runs of it per CTA, the drafted tree's masks,
+// and the join of items that several CTAs worked on.
+#pragma once
+
+#include "cache_ops.cuh"
+#include "cache_tile.cuh"
+
+namespace mrtdf {
+
+constexpr int kTile = 64;      // keys per CTA tile
+constexpr int kThreads = 128;  // four warps
+
+// ---- schedule ----------------------------------------------------------------
+// A sequence's tiles: ceil((len + nodes) / 64), or with APART the drafted rows
+// in a tile of their own behind ceil(len / 64); at least one. A length outside
+// [0, capacity] makes the sequence empty (len -1 here).
+__device__ __forceinline__ int checked_len(const CacheView& c, int b) {
+  const int l = c.lens[b];
+  return l < 0 || l > c.capacity ? -1 : l;
+}
+template <bool APART>
+__device__ __forceinline__ int tiles_of(int len, int extra) {
+  return (max(len, 0) + (APART ? kTile : extra) + kTile - 1) / kTile;
+}
+
+// lens[b] and first[b] = tiles of all items before sequence b's, for b <= B.
+// All threads of the block; the first 128 do the work; ends with a barrier.
+template <bool APART>
+__device__ void build_schedule(const CacheView& c, int batch, int items, int extra, int* lens, int* first) {
+  __shared__ int warp_sum[kThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, per = (batch + kThreads - 1) / kThreads;
+  int sum = 0;
+  for (int i = 0; i < per && tid < kThreads; ++i) {
+    const int b = tid * per + i;
+    if (b < batch) {
+      const int l = checked_len(c, b);
+      lens[b] = l;
+      sum += tiles_of<APART>(l, extra) * items;
+    }
+  }
+  int run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
+  }
+  if (lane == 31 && tid < kThreads) warp_sum[tid >> 5] = run;
+  __syncthreads();
+  run -= sum;
+  for (int w = 0; w < (tid >> 5) && tid < kThreads; ++w) run += warp_sum[w];
+  for (int i = 0; i < per && tid < kThreads; ++i) {
+    const int b = tid * per + i;
+    if (b < batch) {
+      first[b] = run;
+      run += tiles_of<APART>(lens[b], extra) * items;
+      if (b == batch - 1) first[batch] = run;
+    }
+  }
+  __syncthreads();
+}
+
+// Position in the list of tiles: sequence-major, then outer, inner (an item is
+// one pair of them), then tile.
+template <bool APART>
+struct Cursor {
+  int w, b, outer, inner, tile, tiles, len;
+  __device__ __forceinline__ void seek(int at, const int* lens, const int* first, int batch, int inners, int extra) {
+    w = at;
+    int lo = 0, hi = batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    len = lens[b];
+    tiles = tiles_of<APART>(len, extra);
+    const int rem = at - first[b], item = rem / tiles;
+    tile = rem - item * tiles;
+    outer = item / inners;
+    inner = item - outer * inners;
+  }
+  // True when the next tile is another item's.
+  __device__ __forceinline__ bool next(const int* lens, int batch, int outers, int inners, int extra) {
+    ++w;
+    if (++tile < tiles) return false;
+    tile = 0;
+    if (++inner == inners) {
+      inner = 0;
+      if (++outer == outers) {
+        outer = 0;
+        if (++b < batch) {
+          len = lens[b];
+          tiles = tiles_of<APART>(len, extra);
+        }
+      }
+    }
+    return true;
+  }
+};
+
+// CTA c of g takes tiles [share(c), share(c + 1)) of `total`.
+__device__ __forceinline__ int share(int c, int g, int total) { return (int)((long long)c * total / g); }
+// The CTA whose run holds tile w.
+__device__ __forceinline__ int owner(int w, int g, int total) {
+  return (int)((((long long)w + 1) * g - 1) / total);
+}
+// CTAs that take part: a run has two tiles or more, or there is one tile each.
+__device__ __forceinline__ int active(int grid, int total) { return max(1, min(grid, total / 2)); }
+
+// ---- the tree ------------------------------------------------------------------
+// seen[i]: bit j set when node j is node i or an ancestor; 0 for a node that is
+// absent (its chain holds a parent outside [-1, i)). One warp; pointer
+// doubling: after k rounds a node knows 2^k links of its chain.
+__device__ inline void node_masks(unsigned long long* seen, const int32_t* parents, int nodes, bool there, int lane) {
+  constexpr int kRoot = -1, kAbsent = -2;
+  unsigned long long m[2];
+  int up[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = lane + 32 * h;
+    const int p = i < nodes ? (parents ? parents[i] : i - 1) : kAbsent;
+    up[h] = p < kRoot || p >= i ? kAbsent : p;
+    m[h] = 1ull << i;
+  }
+#pragma unroll
+  for (int round = 0; round < 6; ++round) {
+    unsigned long long om[2];
+    int ou[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int from = up[h] & 31;
+      const unsigned long long a = __shfl_sync(0xffffffffu, m[0], from), b = __shfl_sync(0xffffffffu, m[1], from);
+      const int c = __shfl_sync(0xffffffffu, up[0], from), d = __shfl_sync(0xffffffffu, up[1], from);
+      om[h] = up[h] >= 32 ? b : a;
+      ou[h] = up[h] >= 32 ? d : c;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (up[h] >= 0) {
+        m[h] |= om[h];
+        up[h] = ou[h];
+      }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = lane + 32 * h;
+    seen[i] = there && i < nodes && up[h] == kRoot ? m[h] : 0ull;
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ void store2(__nv_bfloat16* p, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+
+// Joins the partial rows of items that several CTAs worked on: a warp per row.
+template <typename T, int D, bool APART>
+__global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_constant__ TreeParams p, int mb) {
+  extern __shared__ __align__(16) int sched[];
+  int *lens = sched, *first = sched + p.c.batch;
+  const int items = p.c.kv_heads * p.row_blocks, nodes = p.nodes;
+  build_schedule<APART>(p.c, p.c.batch, items, nodes, lens, first);
+  const int b = blockIdx.x / items, item = blockIdx.x % items, total = first[p.c.batch];
+  const int parts = active(p.grid, total), tiles = tiles_of<APART>(lens[b], nodes), w = first[b] + item * tiles;
+  const int c0 = owner(w, parts, total), c1 = owner(w + tiles - 1, parts, total);
+  pdl_wait();
+  if (c0 == c1) return;
+  const int lane = threadIdx.x & 31, r = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5);
+  const int heads_per = p.heads / p.c.kv_heads, row = (item % p.row_blocks) * mb + r;
+  if (r >= mb || row >= heads_per * nodes) return;
+  auto part = [&](int c) { return p.ws + (int64_t)(c * 2 + (c == c0)) * mb * (D + 2); };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part(c)[mb * D + r]);
+  m = warp_max(m);
+  const float u = m == -INFINITY ? 0.f : m;
+  constexpr int V = D / 32;
+  float acc[V] = {}, sum = 0.f;
+  for (int cb = c0; cb <= c1; cb += 32) {
+    const int mine = cb + lane;
+    float wt = 0.f;
+    if (mine <= c1) {
+      wt = ex2((part(mine)[mb * D + r] - u) * kLog2e);
+      const float l = part(mine)[mb * D + mb + r];
+      sum += l == 0.f ? 0.f : l * wt;
+    }
+    const int n = min(32, c1 - cb + 1);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float f = __shfl_sync(0xffffffffu, wt, i);
+      const float* src = part(cb + i) + r * D + lane * V;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float v = src[k];
+        if (!(f == 0.f)) acc[k] += v * f;
+      }
+    }
+  }
+  sum = warp_sum(sum);
+  const int hd = row / nodes, n = row - hd * nodes, head = (item / p.row_blocks) * heads_per + hd;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + n * p.out.sn + lane * V;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int k = 0; k < V; k += 2)
+    store2(dst + k, sum == 0.f ? 0.f : acc[k] * inv, sum == 0.f ? 0.f : acc[k + 1] * inv);
+  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + head) * nodes + n] = sum == 0.f ? -INFINITY : m + logf(sum);
+}
+
+}  // namespace mrtdf

@@ -183,24 +183,18 @@ __device__ __forceinline__ float ld_cluster_f32(const float* local, uint32_t ran
   return v;
 }
 
-// x to fp16: 8 columns (one word of weights) per lane, a group by 4 WL
-// neighbouring lanes; words of one group and index i next to each other for
-// c = 0 .. 3. Columns without a row of x, and columns past k, are zero.
-template <typename T, int G, int NT, bool EIGHT>
-__global__ __launch_bounds__(128) void q4_prepare_kernel(const __grid_constant__ Q4Params p, int steps, int rows) {
-  constexpr int WL = G / 32, P = Parts<T>::N, COLS = NT * 8, V = 8 * (int)sizeof(T) / 16;
-  pdl_launch_dependents();
-  const int words = steps * (kStep / 8), lane = threadIdx.x & 31, m0 = blockIdx.y * rows;
-  uint8_t* out = static_cast<uint8_t*>(p.ws) + blockIdx.y * Q4Prepared<G, NT>::bytes(steps);
-  float4* factor = reinterpret_cast<float4*>(out + Q4Prepared<G, NT>::x_bytes(steps));
-  const int i = blockIdx.x * 128 + threadIdx.x;
-  if (i - lane >= words * (COLS / P)) return;
-  const int m = i / words, wd = i - m * words, kk = wd * 8;
+// x to fp16: 8 columns from kk on (one word of weights) per lane, a group by
+// 4 WL neighbouring lanes, all lanes of a warp together. put(h, words) gets the
+// lane's eight values of part h, sums(h, {factor, addend, X, 0}) the group's.
+// Rows that do not exist (m < 0) and columns past k are zero.
+template <typename T, int G, bool EIGHT, typename Put, typename Sums>
+__device__ __forceinline__ void bring_x(const Q4Params& p, int m, int kk, Put&& put, Sums&& sums) {
+  constexpr int WL = G / 32, P = Parts<T>::N, V = 8 * (int)sizeof(T) / 16;
   float v[8], big = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  if (m < rows && m0 + m < p.m && kk < p.k) {
-    const T* src = reinterpret_cast<const T*>(p.x) + (m0 + m) * p.x_stride + kk;
+  if (m >= 0 && kk < p.k) {
+    const T* src = reinterpret_cast<const T*>(p.x) + m * p.x_stride + kk;
 #pragma unroll
     for (int e = 0; e < V; ++e) Vec16<T>::unpack(*reinterpret_cast<const uint4*>(src + e * (8 / V)), v + e * (8 / V));
   }
@@ -210,7 +204,6 @@ __global__ __launch_bounds__(128) void q4_prepare_kernel(const __grid_constant__
   for (int o = 1; o < 4 * WL; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
   const uint32_t ex = max(__float_as_uint(big) >> 23, 15u);
   const float up = __uint_as_float((268u - ex) << 23), down = __uint_as_float((ex - 14u) << 23);
-  const int gr = wd / (4 * WL), in = wd % (4 * WL), to = gr * 4 * WL + (in % WL) * 4 + in / WL;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] *= up;
 #pragma unroll
@@ -230,28 +223,51 @@ __global__ __launch_bounds__(128) void q4_prepare_kernel(const __grid_constant__
       even += __shfl_xor_sync(0xffffffffu, even, o);
       odd += __shfl_xor_sync(0xffffffffu, odd, o);
     }
-    if (i < words * (COLS / P)) {
-      if (!EIGHT) {
-        w[1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
-        w[3] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
-      }
-      *reinterpret_cast<uint4*>(out + ((int64_t)(m * P + h) * words + to) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-      if (in == 0) {
-        const float sum = down * (even + odd);
-        factor[gr * COLS + m * P + h] =
-            make_float4(down, EIGHT ? 8.f * sum : -down * (1024.f * even + 64.f * odd), sum, 0.f);
-      }
+    if (!EIGHT) {
+      w[1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
+      w[3] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
     }
+    put(h, make_uint4(w[0], w[1], w[2], w[3]));
+    const float sum = down * (even + odd);
+    sums(h, make_float4(down, EIGHT ? 8.f * sum : -down * (1024.f * even + 64.f * odd), sum, 0.f));
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] -= f[e];
   }
+}
+// Where word wd of a row lies: words of one group and index i next to each
+// other for c = 0 .. 3.
+template <int WL>
+__device__ __forceinline__ int word_at(int wd) {
+  const int in = wd % (4 * WL);
+  return wd - in + (in % WL) * 4 + in / WL;
+}
+
+template <typename T, int G, int NT, bool EIGHT>
+__global__ __launch_bounds__(128) void q4_prepare_kernel(const __grid_constant__ Q4Params p, int steps, int rows) {
+  constexpr int WL = G / 32, P = Parts<T>::N, COLS = NT * 8;
+  pdl_launch_dependents();
+  const int words = steps * (kStep / 8), lane = threadIdx.x & 31, m0 = blockIdx.y * rows, all = words * (COLS / P);
+  uint8_t* out = static_cast<uint8_t*>(p.ws) + blockIdx.y * Q4Prepared<G, NT>::bytes(steps);
+  float4* factor = reinterpret_cast<float4*>(out + Q4Prepared<G, NT>::x_bytes(steps));
+  const int i = blockIdx.x * 128 + threadIdx.x;
+  if (i - lane >= all) return;
+  const int m = i / words, wd = i - m * words;
+  bring_x<T, G, EIGHT>(
+      p, i < all && m < rows && m0 + m < p.m ? m0 + m : -1, wd * 8,
+      [&](int h, uint4 w) {
+        if (i < all) *reinterpret_cast<uint4*>(out + ((int64_t)(m * P + h) * words + word_at<WL>(wd)) * 16) = w;
+      },
+      [&](int h, float4 f) {
+        if (i < all && wd % (4 * WL) == 0) factor[wd / (4 * WL) * COLS + m * P + h] = f;
+      });
 }
 
 // T: type of x, scales and biases. NT: tiles of eight columns (rows of x x
 // parts). A cluster works on q.tiles row tiles, its CTAs on a slab of the
 // columns each (a CTA reads half of x that way); the slabs' sums meet over
-// distributed shared memory, in rank order.
-template <typename T, typename O, int G, int NT>
+// distributed shared memory, in rank order. FUSED: x is small and every CTA
+// brings its slab to fp16 itself (2 x 1024: 7 us, 10 with a launch for it).
+template <typename T, typename O, int G, int NT, bool FUSED>
 __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __grid_constant__ Q4Params p,
                                                                                      const __grid_constant__ Q4Plan q) {
   constexpr int WL = G / 32, GS = kStep / G, P = Parts<T>::N, COLS = NT * 8, LD = COLS + 1;
@@ -275,7 +291,7 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
   const int units_max = q.tiles > q.warps * q.wk ? q.tiles : q.warps * q.wk;
   for (int i = tid; i < units_max * 16 * LD; i += threads) part[i] = 0.f;
 
-  if (tid == 0) {
+  if (!FUSED && tid == 0) {
     for (int i = 0; i < kParts; ++i) mbar_init(bars + i, 1);
     fence_mbar_init();
   }
@@ -319,8 +335,8 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
 
   if (round) __syncthreads();  // the chunk before is done with
   const int gn = steps * GS, g0 = k0 / G;
-  if (round == 0) pdl_wait();  // x is prepared
-  if (tid == 0) {
+  if (!FUSED && round == 0) pdl_wait();  // x is prepared
+  if (!FUSED && tid == 0) {
     // The chunk before was read through the generic proxy.
     if (round) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     const uint32_t factor_bytes = gn * COLS * 16;
@@ -369,7 +385,26 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
       sb[(gr * stride + r) * 2 + 1] = reinterpret_cast<const T*>(p.biases)[from];
     }
   }
-  __syncthreads();  // the scales are there, and the barriers
+  if (FUSED) {
+    const int words = steps * (kStep / 8), all = words * q.rows, spare = COLS - q.rows * P;
+    float4* factor = reinterpret_cast<float4*>(smem + at.factors);
+    for (int i0 = tid; i0 - lane < all; i0 += threads) {
+      const int m = i0 / words, wd = i0 - m * words;
+      bring_x<T, G, EIGHT>(
+          p, i0 < all && m < ms ? m0 + m : -1, k0 + wd * 8,
+          [&](int h, uint4 w) {
+            if (i0 < all) *reinterpret_cast<uint4*>(smem + at.x + (m * P + h) * at.x_bytes + word_at<WL>(wd) * 16) = w;
+          },
+          [&](int h, float4 f) {
+            if (i0 < all && wd % (4 * WL) == 0) factor[wd / (4 * WL) * COLS + m * P + h] = f;
+          });
+    }
+    for (int i = tid; i < words * spare; i += threads)  // columns without a row of x
+      *reinterpret_cast<uint4*>(smem + at.x + (COLS - spare + i / words) * at.x_bytes + (i % words) * 16) = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < gn * spare; i += threads)
+      factor[i / spare * COLS + COLS - spare + i % spare] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __syncthreads();  // the scales are there, and the barriers (or x)
 
   float y[NT][4];
 #pragma unroll
@@ -383,7 +418,7 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
   uint32_t xa = x_first, fa = f_first, sa = s_first, row = ring + g * (kStep / 2), st = 0;
   int tile = wt, step = 0, parts = 0;  // parts of x that have arrived
   for (int t = 0; t < units; ++t) {
-    while (parts * q.part <= min((step * q.wk + wk) * 2 + 1, steps - 1)) mbar_wait_bounded(bars + parts++, round & 1, nullptr);
+    while (!FUSED && parts * q.part <= min((step * q.wk + wk) * 2 + 1, steps - 1)) mbar_wait_bounded(bars + parts++, round & 1, nullptr);
     cp_async_wait<kRing - 2>();
     __syncwarp();
     if (f_unit < units) fetch();
@@ -459,7 +494,7 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
   }
   cp_async_wait<0>();
   // No copy is still landing when the chunk is left (or the CTA).
-  while (parts < kParts && parts * q.part < steps) mbar_wait_bounded(bars + parts++, round & 1, nullptr);
+  while (!FUSED && parts < kParts && parts * q.part < steps) mbar_wait_bounded(bars + parts++, round & 1, nullptr);
   }
 
   // Sums of the warps that share tiles (then each has one), of the slabs and
@@ -530,7 +565,7 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const __grid_constant_
 
 // The layout on a GPU of `sms` multiprocessors: one CTA per SM, row tiles spread
 // evenly over pairs of CTAs (1025 tiles are 74 pairs of 14), a slab of the
-// columns for each of a pair where there are eight steps or more; fewer tiles
+// columns for each of a pair where there are 16 steps or more; fewer tiles
 // or columns at a time where the shared memory asks for it.
 template <typename T, int G, int NT>
 Q4Plan q4_plan(const Q4Params& p, int sms) {
@@ -538,7 +573,7 @@ Q4Plan q4_plan(const Q4Params& p, int sms) {
   Q4Plan q{};
   q.steps = (p.k + kStep - 1) / kStep;
   q.rows = min(p.m, NT * 8 / Parts<T>::N);
-  q.split = q.steps >= 8 ? 2 : 1;
+  q.split = q.steps >= 16 ? 2 : 1;
   q.slab = (q.steps + q.split - 1) / q.split;
   q.chunk = q.slab;
   const int clusters = max(1, sms / q.split);
@@ -555,35 +590,48 @@ Q4Plan q4_plan(const Q4Params& p, int sms) {
   }
 }
 
-template <typename T, typename O, int G, int NT>
-cudaError_t q4_run(const Q4Params& p, int sms, size_t* ws_bytes, cudaStream_t s) {
-  const Q4Plan q = q4_plan<T, G, NT>(p, sms);
-  const int passes = (p.m + q.rows - 1) / q.rows;
-  if (ws_bytes) {
-    *ws_bytes = (size_t)passes * Q4Prepared<G, NT>::bytes(q.steps);
-    return cudaSuccess;
-  }
-  constexpr auto K = q4_linear_kernel<T, O, G, NT>;
+template <typename T, typename O, int G, int NT, bool FUSED>
+cudaError_t q4_launch(const Q4Params& p, const Q4Plan& q, int passes, cudaStream_t s) {
+  constexpr auto K = q4_linear_kernel<T, O, G, NT, FUSED>;
   cudaError_t e = allow_smem<K>();
   if (e != cudaSuccess) return e;
-  const int words = q.steps * (kStep / 8) * (NT * 8 / Parts<T>::N);
-  q4_prepare_kernel<T, G, NT, sizeof(O) == 4><<<dim3((words + 127) / 128, passes), 128, 0, s>>>(p, q.steps, q.rows);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = q.split;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  int n = 0;
+  if (!FUSED) {
+    const int words = q.steps * (kStep / 8) * (NT * 8 / Parts<T>::N);
+    q4_prepare_kernel<T, G, NT, sizeof(O) == 4><<<dim3((words + 127) / 128, passes), 128, 0, s>>>(p, q.steps, q.rows);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (q.split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = q.split;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(((p.n + 15) / 16 + q.tiles - 1) / q.tiles * q.split, passes);
   cfg.blockDim = dim3(q.warps * q.wk * 32);
   cfg.dynamicSmemBytes = Q4Smem<T, G, NT>(q).bytes;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = q.split > 1 ? 2 : 1;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, K, p, q);
+}
+
+template <typename T, typename O, int G, int NT>
+cudaError_t q4_run(const Q4Params& p, int sms, size_t* ws_bytes, cudaStream_t s) {
+  const Q4Plan q = q4_plan<T, G, NT>(p, sms);
+  const int passes = (p.m + q.rows - 1) / q.rows;
+  // Words of x per CTA: up to two per thread it takes them itself.
+  const bool fused = q.slab * (kStep / 8) * q.rows <= 1024;
+  if (ws_bytes) {
+    *ws_bytes = fused ? 0 : (size_t)passes * Q4Prepared<G, NT>::bytes(q.steps);
+    return cudaSuccess;
+  }
+  return fused ? q4_launch<T, O, G, NT, true>(p, q, passes, s) : q4_launch<T, O, G, NT, false>(p, q, passes, s);
 }
 
 template <typename T, typename O, int G>

@@ -53,8 +53,8 @@ class Call:
                            path_len=4)
         self.evict = dict(size=_EVICT.size, mass=256, mass_out=256, pos_out=256, lens_out=512, budget=64, recent=8, sinks=1)
         self.q4 = dict(size=_Q4.size, x=256, packed=256, scales=256, biases=256, out=256, workspace=256, workspace_bytes=1 << 20,
-                       x_stride=128, out_stride=64, m=2,
-                       n=64, k=128, group=32, dtype=1, out_dtype=1, device=0)
+                       x_stride=16384, out_stride=64, m=16,
+                       n=64, k=16384, group=32, dtype=1, out_dtype=1, device=0)
         self.pack = dict(size=_PACK.size, w=256, packed=256, scales=256, biases=256, w_stride=128, n=4, k=128, group=32,
                          dtype=1, device=0)
 
