@@ -3,11 +3,12 @@
 // mathematics is that of cache_attn.cu.
 //
 // The rows of one kv head (nodes x its query heads) are the M side of
-// tcgen05.mma, 128 at a time. With 128 rows a tile of 64 keys takes 512 clocks
-// of products (head_dim 128) and its 32 KB of K and V come in 1400 at the
-// memory's rate, so padding to 128 rows costs nothing while the cache is read
-// from HBM; mma.sync, which a quarter of the rate is left of, took 4 times
-// that at 96 rows.
+// tcgen05.mma, 128 at a time. With 128 rows a tile of 64 keys takes some 800
+// clocks of products (head_dim 128) and its 32 KB of K and V come in 1400 at
+// the memory's rate, so padding to 128 rows costs nothing while the cache is
+// read from HBM. The A operands (the queries, and the weights in the place of
+// the scores they came from) are in TMEM: read from shared memory, 64 columns at
+// a time, they alone kept the products at a third of their rate.
 //
 // CTA of 320 threads, one per SM, over an equal run of the key tiles of all
 // items (cache_sched.cuh); roles and hand-over as in enc_attn_tc.cu:
@@ -20,6 +21,7 @@
 //   warp 9     MMA issuer: S = Q K^T into one of two TMEM buffers, then
 //              O_h += P_h V for the two key halves h, weights as two bf16
 //              parts (16 bits of a weight; the second product is hidden too).
+//              V is an MN-major operand of 64-column parts kSub bytes apart.
 // A maximum is raised only when a tile exceeds it by 8 units of its scale.
 // The drafted rows are a tile of their own behind the cached ones.
 //
@@ -42,34 +44,39 @@ constexpr int kRows = 128;
 constexpr int kSoft = 256;              // softmax threads
 constexpr int kTcThreads = kSoft + 64;  // and the TMA and MMA warps
 constexpr int kSub = 64 * 128;          // 64 rows of 128 bytes (64 columns)
-constexpr int kPBytes = kRows * 128;    // one part of the weights of a tile
 constexpr float kLazy = 8.f;
 
 template <int D>
 struct TcCfg {
   static constexpr int kSubs = D / 64;  // 64-column parts of a row
-  static constexpr int kStagesKv = D == 64 ? 4 : 3;
-  static constexpr int kQBytes = kRows * D * 2, kKvBytes = kSub * kSubs;
-  static constexpr int kOffQ = 0, kOffKv = kQBytes, kOffP = kOffKv + kStagesKv * 2 * kKvBytes;
-  static constexpr int kOffBar = kOffP + 2 * 2 * kPBytes;  // two buffers of two parts
+  static constexpr int kStagesKv = D == 64 ? 8 : 6;
+  static constexpr int kKvBytes = kSub * kSubs;
+  static constexpr int kOffBar = kStagesKv * 2 * kKvBytes;
   static constexpr int kOffSched = kOffBar + 256;
   static int smem(int batch) { return kOffSched + (2 * batch + 1) * 4 + 1024; }
-  static constexpr uint32_t kTmem = D == 64 ? 256 : 512;  // S 2 x 64, O 2 x D columns
 };
-// kind::f16, D f32, A / B bf16, M 128, N 64, K-major; PV: B MN-major.
-constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(64 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-constexpr uint32_t kIdescPv = kIdesc | (1u << 16);
+// TMEM columns: the scores of a tile, then its weights (per key half 16 columns
+// of high parts, 16 of low ones), twice; O_0 and O_1; the queries.
+constexpr uint32_t kTmem = 512, kColO = 128;
+template <int D>
+constexpr uint32_t kColQ = kColO + 2 * D;
+// kind::f16, D f32, A / B bf16, M 128, K-major B of 64 rows; PV: B MN-major.
+constexpr uint32_t idesc(int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+constexpr uint32_t kMnMajorB = 1u << 16;
 
 struct TcMaps {
   CUtensorMap k, v, kn, vn;
 };
 
-__device__ __forceinline__ void umma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A in TMEM (row = lane, two bf16 per column), B in shared memory.
+__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
@@ -87,8 +94,8 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t *q_full = bar, *o_done = bar + 1, *drain = bar + 2, *kv_full = bar + 3, *kv_empty = bar + 3 + NS;
-  uint64_t *s_full = bar + 3 + 2 * NS, *s_empty = s_full + 2, *p_full = s_full + 4, *p_empty = s_full + 6;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 8);
+  uint64_t *s_full = bar + 3 + 2 * NS, *p_full = s_full + 2, *p_empty = s_full + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
   int* lens = reinterpret_cast<int*>(smem + C::kOffSched);
   int* first = lens + p.c.batch;
   __shared__ int abort_flag;
@@ -100,7 +107,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   const int heads_per = p.heads / p.c.kv_heads, rows = heads_per * nodes;
 
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmem)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmem)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -114,17 +121,12 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(s_empty + i, kSoft);
       mbar_init(p_full + i, kSoft);
       mbar_init(p_empty + i, 1);
     }
     fence_mbar_init();
     abort_flag = 0;
   }
-  // Weights of rows that do not exist stay zero.
-  for (int i = tid; i < 4 * kPBytes / 16; i += kTcThreads)
-    reinterpret_cast<uint4*>(smem + C::kOffP)[i] = make_uint4(0, 0, 0, 0);
-  fence_async();
   tc_fence_before();
   build_schedule<true>(p.c, batch, items, nodes, lens, first);  // ends with a barrier
   tc_fence_after();
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       for (int i = 0; cur.w < w1; ++i) {
         const int st = i % NS;
         if (i >= NS && !wait(kv_empty + st, (uint32_t)((i / NS - 1) & 1))) break;
-        uint8_t* ks = smem + C::kOffKv + st * 2 * C::kKvBytes;
+        uint8_t* ks = smem + st * 2 * C::kKvBytes;
         const bool fresh = cur.tile + 1 == cur.tiles;  // the drafted rows
         mbar_arrive_expect_tx(kv_full + st, 2 * C::kKvBytes);
 #pragma unroll
@@ -169,18 +171,20 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   } else if (warp == kSoft / 32 + 1) {
     // ---- MMA issuer ----
     if (lane == 0) {
-      const uint32_t aq = smem_u32(smem + C::kOffQ);
+      // Descriptors differ in the start address alone (units of 16 bytes, which
+      // do not carry out of their field): one add per product.
+      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem));
+      const uint64_t dv0 = (dk0 & ~((uint64_t)0x3fff << 16)) | (uint64_t)(kSub / 16) << 16;  // LBO: the next 64 columns
       bool ok = true;
       auto issue_s = [&](int i) -> bool {
         const int st = i % NS, sb = i & 1;
         if (!wait(kv_full + st, (uint32_t)((i / NS) & 1))) return false;
-        if (i >= 2 && !wait(s_empty + sb, (uint32_t)(((i >> 1) - 1) & 1))) return false;
+        if (i >= 2 && !wait(p_empty + sb, (uint32_t)(((i >> 1) - 1) & 1))) return false;
         tc_fence_after();
-        const uint32_t ak = smem_u32(smem + C::kOffKv + st * 2 * C::kKvBytes);
+        const uint64_t dk = dk0 + (uint64_t)(st * 2 * C::kKvBytes / 16);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma(tmem + (uint32_t)(sb * 64), smem_desc_sw128(aq + (kk >> 2) * (kRows * 128) + (kk & 3) * 32),
-               smem_desc_sw128(ak + (kk >> 2) * kSub + (kk & 3) * 32), kIdesc, kk != 0);
+          umma(tmem + (uint32_t)(sb * 64), tmem + kColQ<D> + kk * 8, dk + ((kk >> 2) * kSub + (kk & 3) * 32) / 16, idesc(64), kk != 0);
         mma_commit(s_full + sb);
         return true;
       };
@@ -194,17 +198,14 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
           const int st = i % NS, pb = i & 1;
           if (!(ok = wait(p_full + pb, (uint32_t)((i >> 1) & 1)))) break;
           tc_fence_after();
-          const uint32_t ap = smem_u32(smem + C::kOffP + pb * 2 * kPBytes);
-          const uint32_t av = smem_u32(smem + C::kOffKv + st * 2 * C::kKvBytes + C::kKvBytes);
+          const uint64_t dv = dv0 + (uint64_t)((st * 2 + 1) * C::kKvBytes / 16);
           // Slices 0, 1 of 16 keys go to O_0, slices 2, 3 to O_1.
 #pragma unroll
           for (int part = 0; part < 2; ++part)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-              for (int u = 0; u < SUBS; ++u)
-                umma(tmem + 128 + (uint32_t)((kk >> 1) * D + u * 64), smem_desc_sw128(ap + part * kPBytes + kk * 32),
-                     smem_desc_sw128(av + u * kSub + kk * 2048), kIdescPv, (part || t != 0 || (kk & 1)) ? 1u : 0u);
+              umma(tmem + kColO + (uint32_t)((kk >> 1) * D), tmem + (uint32_t)(pb * 64 + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8),
+                   dv + kk * 2048 / 16, idesc(D) | kMnMajorB, (part || t != 0 || (kk & 1)) ? 1u : 0u);
           mma_commit(p_empty + pb);
           mma_commit(kv_empty + st);
         }
@@ -223,9 +224,11 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     const int row = tid & (kRows - 1), half = tid >> 7;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int c0 = half * 32;
-    const uint32_t ocol = 128u + (uint32_t)(half * D);
+    const uint32_t ocol = kColO + (uint32_t)(half * D);
     constexpr bool POW2 = !BIAS;
-    const float unit = POW2 ? p.scale * kLog2e : p.scale;
+    // Not zero: it multiplies -inf.
+    const float unit = fmaxf(fabsf(POW2 ? p.scale * kLog2e : p.scale), 1e-30f);
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale is the queries'
     auto weight = [](float x) { return ex2(POW2 ? x : x * kLog2e); };
     auto soft_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory"); };
     bool ok = true;
@@ -240,20 +243,29 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         if (warp == 0) node_masks(seen, p.parents ? p.parents + b * nodes : nullptr, nodes, cur.len >= 0, lane);
       }
       if (tid == 0) poison = 0;
-      for (int x = tid; x < kRows * (D / 8); x += kSoft) {
-        const int r = x / (D / 8), ch = x % (D / 8);
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < here) {
-          const int hd = (row0 + r) / nodes, nd = row0 + r - hd * nodes;
-          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(p.q.ptr) + b * p.q.sb +
-                                              (kvh * heads_per + hd) * p.q.sh + nd * p.q.sn + ch * 8);
+      const int hd = (row0 + row) / nodes, nd = row0 + row - hd * nodes, head = kvh * heads_per + hd;
+      {
+        // Columns [half * D / 2, + D / 2) of this row's query.
+        const bf16* q = reinterpret_cast<const bf16*>(p.q.ptr) + b * p.q.sb + head * p.q.sh + nd * p.q.sn + half * (D / 2);
+#pragma unroll
+        for (int cc = 0; cc < D / 4; cc += 16) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row < here) v = *reinterpret_cast<const uint4*>(q + 2 * (cc + e));
+            w[e] = v.x ^ flip;
+            w[e + 1] = v.y ^ flip;
+            w[e + 2] = v.z ^ flip;
+            w[e + 3] = v.w ^ flip;
+          }
+          tmem_st16(tmem + lane_base + kColQ<D> + (uint32_t)(half * (D / 4) + cc), w);
         }
-        *reinterpret_cast<uint4*>(smem + C::kOffQ + (ch >> 3) * (kRows * 128) + sw128(r, ch & 7)) = v;
+        tmem_wait_st();
       }
-      fence_async();
+      tc_fence_before();
       arrive(q_full);
       soft_sync();  // the masks
-      const int hd = (row0 + row) / nodes, nd = row0 + row - hd * nodes, head = kvh * heads_per + hd;
       const unsigned long long see = row < here ? seen[nd] : 0ull;
       const int next = p.c.next_pos ? p.c.next_pos[b] : len, at = (int)((unsigned)next + (unsigned)(see ? __popcll(see) - 1 : 0));
       const float* tab = BIAS ? p.rel_bias + (row < here ? (int64_t)head * p.rel_len : 0) : nullptr;
@@ -289,12 +301,11 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
             tmem_ld16(tmem + lane_base + (uint32_t)(sb * 64 + c0 + 16), reinterpret_cast<uint32_t*>(x) + 16);
             tmem_wait_ld();
           }
-          tc_fence_before();
-          arrive(s_empty + sb);
           // Values that must not meet the products.
-          if (fresh || (tile + 1) * kTile > len) {
+          const bool cleaned = fresh || (tile + 1) * kTile > len;
+          if (cleaned) {
             if ((ok = __all_sync(0xffffffffu, wait(kv_full + st, (uint32_t)((i / NS) & 1))) != 0)) {
-              uint8_t* vs = smem + C::kOffKv + st * 2 * C::kKvBytes + C::kKvBytes;
+              uint8_t* vs = smem + st * 2 * C::kKvBytes + C::kKvBytes;
               for (int x4 = tid; x4 < kTile * (D / 8); x4 += kSoft) {
                 const int r = x4 / (D / 8), ch = x4 % (D / 8);
                 uint4* v4 = reinterpret_cast<uint4*>(vs + (ch >> 3) * kSub + sw128(r, ch & 7));
@@ -318,9 +329,9 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
             }
           }
           if (live && ok) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] *= unit;
             if (BIAS) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] *= unit;
               if (near) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
@@ -345,6 +356,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
             float mt = x[0];
 #pragma unroll
             for (int e = 1; e < 32; ++e) mt = fmaxf(mt, x[e]);
+            if (!BIAS) mt *= unit;  // x itself is scaled where its weight is taken
             float alpha = 1.f;
             bool scale = false;
             if (mt > m + kLazy) {  // also the first tile with a key (m = -inf)
@@ -373,30 +385,27 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
                 tmem_wait_st();
               }
             }
-            if (ok && i >= 2) ok = __all_sync(0xffffffffu, wait(p_empty + pb, (uint32_t)(((i >> 1) - 1) & 1))) != 0;
             if (ok) {
-              uint8_t* ph = smem + C::kOffP + pb * 2 * kPBytes;
               const float u = m == -INFINITY ? 0.f : m;
               float sum[4] = {0.f, 0.f, 0.f, 0.f};
+              uint32_t hi[16], lo[16];
 #pragma unroll
-              for (int cc = 0; cc < 32; cc += 8) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float a = weight(x[cc + 2 * e] - u), d = weight(x[cc + 2 * e + 1] - u);
-                  sum[e] += a + d;
-                  hi[e] = pack_bf16(a, d);
-                  lo[e] = pack_bf16(a - __uint_as_float(hi[e] << 16), d - __uint_as_float(hi[e] & 0xffff0000u));
-                }
-                const uint32_t to = sw128(row, (c0 + cc) >> 3);
-                *reinterpret_cast<uint4*>(ph + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(ph + kPBytes + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              for (int e = 0; e < 16; ++e) {
+                const float a = weight(BIAS ? x[2 * e] - u : fmaf(x[2 * e], unit, -u));
+                const float d = weight(BIAS ? x[2 * e + 1] - u : fmaf(x[2 * e + 1], unit, -u));
+                sum[e & 3] += a + d;
+                hi[e] = pack_bf16(a, d);
+                lo[e] = pack_bf16(a - __uint_as_float(hi[e] << 16), d - __uint_as_float(hi[e] & 0xffff0000u));
               }
+              // Into the place of this half's scores.
+              tmem_st16(tmem + lane_base + (uint32_t)(pb * 64 + c0), hi);
+              tmem_st16(tmem + lane_base + (uint32_t)(pb * 64 + c0 + 16), lo);
+              tmem_wait_st();
               l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
           }
           tc_fence_before();
-          fence_async();
+          if (cleaned) fence_async();
           arrive(p_full + pb);
         }
       }
@@ -422,8 +431,8 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         for (int cc = 0; cc < D / 2; cc += 16) {
           const int col = half * (D / 2) + cc;
           float o0[16], o1[16];
-          tmem_ld16(tmem + lane_base + 128u + (uint32_t)col, reinterpret_cast<uint32_t*>(o0));
-          tmem_ld16(tmem + lane_base + 128u + (uint32_t)(D + col), reinterpret_cast<uint32_t*>(o1));
+          tmem_ld16(tmem + lane_base + kColO + (uint32_t)col, reinterpret_cast<uint32_t*>(o0));
+          tmem_ld16(tmem + lane_base + kColO + (uint32_t)(D + col), reinterpret_cast<uint32_t*>(o1));
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 16; ++e) o0[e] = empty && ok ? 0.f : (o0[e] * a0 + o1[e] * a1) * inv;
@@ -471,7 +480,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
   }
 }
 
