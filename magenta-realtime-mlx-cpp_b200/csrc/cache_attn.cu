@@ -464,7 +464,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
           const int r = wm * 16 + g + 8 * h;
 #pragma unroll
           for (int i = 0; i < ND; ++i)
-            store2(part + r * D + 8 * i + 2 * c, h ? o[i][2] : o[i][0], h ? o[i][3] : o[i][1]);
+            store2(part + ((2 * i + (c >> 1)) * MB + r) * 4 + 2 * (c & 1), h ? o[i][2] : o[i][0], h ? o[i][3] : o[i][1]);
           if (c == 0) {
             part[MB * D + r] = h ? m1 : m0;
             part[MB * D + MB + r] = h ? l1 : l0;
@@ -703,7 +703,7 @@ cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.c.batch * p.c.kv_heads * p.row_blocks, (16 * WM + 3) / 4);
+  cfg.gridDim = join_grid(p, 16 * WM, D);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (2 * p.c.batch + 1) * 4;
   cfg.stream = s;

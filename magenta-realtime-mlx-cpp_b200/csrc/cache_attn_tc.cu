@@ -12,15 +12,16 @@
 //
 // CTA of 320 threads, one per SM, over an equal run of the key tiles of all
 // items (cache_sched.cuh); roles and hand-over as in enc_attn_tc.cu:
-//   warps 0-7  softmax: two threads per query row, each with 32 of a tile's
-//              64 key columns, a running maximum and an accumulator of its own
-//              (rows that do not exist skip the work: their weights are zero
-//              from the start);
+//   warps 0-7  softmax: two groups of four warps take turns at the tiles, a
+//              thread per query row, each group with a running maximum and an
+//              accumulator of its own, so that one's exponentials overlap the
+//              other's products (rows that do not exist skip the work: their
+//              queries are zero, their scores stay zero bits);
 //   warp 8     TMA producer: K and V tiles through a ring, 128-byte swizzle,
 //              over the items of the run without a stop;
-//   warp 9     MMA issuer: S = Q K^T into one of two TMEM buffers, then
-//              O_h += P_h V for the two key halves h, weights as two bf16
-//              parts (16 bits of a weight; the second product is hidden too).
+//   warp 9     MMA issuer: S = Q K^T into one of three TMEM buffers, three
+//              tiles ahead, then O_g += P V for the tile's group g, weights as two bf16 parts (16 bits of a
+//              weight; the second product is hidden too).
 //              V is an MN-major operand of 64-column parts kSub bytes apart.
 // A maximum is raised only when a tile exceeds it by 8 units of its scale.
 // The drafted rows are a tile of their own behind the cached ones.
@@ -55,9 +56,10 @@ struct TcCfg {
   static constexpr int kOffSched = kOffBar + 256;
   static int smem(int batch) { return kOffSched + (2 * batch + 1) * 4 + 1024; }
 };
-// TMEM columns: the scores of a tile, then its weights (per key half 16 columns
-// of high parts, 16 of low ones), twice; O_0 and O_1; the queries.
-constexpr uint32_t kTmem = 512, kColO = 128;
+// TMEM columns: the scores of a tile, then its weights (32 columns of high
+// parts, 32 of low ones), three times; O_0 and O_1; the queries.
+constexpr int kBufs = 3;
+constexpr uint32_t kTmem = 512, kColO = kBufs * 64;
 template <int D>
 constexpr uint32_t kColQ = kColO + 2 * D;
 // kind::f16, D f32, A / B bf16, M 128, K-major B of 64 rows; PV: B MN-major.
@@ -94,8 +96,8 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t *q_full = bar, *o_done = bar + 1, *drain = bar + 2, *kv_full = bar + 3, *kv_empty = bar + 3 + NS;
-  uint64_t *s_full = bar + 3 + 2 * NS, *p_full = s_full + 2, *p_empty = s_full + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
+  uint64_t *s_full = bar + 3 + 2 * NS, *p_full = s_full + kBufs, *p_empty = p_full + kBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_empty + kBufs);
   int* lens = reinterpret_cast<int*>(smem + C::kOffSched);
   int* first = lens + p.c.batch;
   __shared__ int abort_flag;
@@ -119,9 +121,9 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       mbar_init(kv_full + i, 1);
       mbar_init(kv_empty + i, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBufs; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, kSoft);
+      mbar_init(p_full + i, kSoft / 2);
       mbar_init(p_empty + i, 1);
     }
     fence_mbar_init();
@@ -177,9 +179,9 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       const uint64_t dv0 = (dk0 & ~((uint64_t)0x3fff << 16)) | (uint64_t)(kSub / 16) << 16;  // LBO: the next 64 columns
       bool ok = true;
       auto issue_s = [&](int i) -> bool {
-        const int st = i % NS, sb = i & 1;
+        const int st = i % NS, sb = i % kBufs;
         if (!wait(kv_full + st, (uint32_t)((i / NS) & 1))) return false;
-        if (i >= 2 && !wait(p_empty + sb, (uint32_t)(((i >> 1) - 1) & 1))) return false;
+        if (i >= kBufs && !wait(p_empty + sb, (uint32_t)((i / kBufs - 1) & 1))) return false;
         tc_fence_after();
         const uint64_t dk = dk0 + (uint64_t)(st * 2 * C::kKvBytes / 16);
 #pragma unroll
@@ -192,22 +194,21 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       for (int seg = 0; ok && cur.w < w1; ++seg) {
         const int n = min(cur.tiles - cur.tile, w1 - cur.w);  // tiles of the item's run
         if (!(ok = wait(q_full, (uint32_t)(seg & 1)))) break;
-        ok = issue_s(i);
+        for (int t = 0; ok && t < min(n, kBufs); ++t) ok = issue_s(i + t);
         for (int t = 0; ok && t < n; ++t, ++i) {
-          if (t + 1 < n && !(ok = issue_s(i + 1))) break;
-          const int st = i % NS, pb = i & 1;
-          if (!(ok = wait(p_full + pb, (uint32_t)((i >> 1) & 1)))) break;
+          const int st = i % NS, pb = i % kBufs, og = i & 1;
+          if (!(ok = wait(p_full + pb, (uint32_t)((i / kBufs) & 1)))) break;
           tc_fence_after();
           const uint64_t dv = dv0 + (uint64_t)((st * 2 + 1) * C::kKvBytes / 16);
-          // Slices 0, 1 of 16 keys go to O_0, slices 2, 3 to O_1.
 #pragma unroll
           for (int part = 0; part < 2; ++part)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma(tmem + kColO + (uint32_t)((kk >> 1) * D), tmem + (uint32_t)(pb * 64 + (kk >> 1) * 32 + part * 16 + (kk & 1) * 8),
-                   dv + kk * 2048 / 16, idesc(D) | kMnMajorB, (part || t != 0 || (kk & 1)) ? 1u : 0u);
+              umma(tmem + kColO + (uint32_t)(og * D), tmem + (uint32_t)(pb * 64 + part * 32 + kk * 8), dv + kk * 2048 / 16,
+                   idesc(D) | kMnMajorB, (part || t >= 2 || kk) ? 1u : 0u);
           mma_commit(p_empty + pb);
           mma_commit(kv_empty + st);
+          if (t + kBufs < n) ok = issue_s(i + kBufs);  // once these products have retired
         }
         if (ok) mma_commit(o_done);
         // To the next item.
@@ -223,8 +224,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     // ---- softmax ----
     const int row = tid & (kRows - 1), half = tid >> 7;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const int c0 = half * 32;
-    const uint32_t ocol = kColO + (uint32_t)(half * D);
+    const uint32_t ocol = kColO + (uint32_t)(half * D);  // half: the group, too
     constexpr bool POW2 = !BIAS;
     // Not zero: it multiplies -inf.
     const float unit = fmaxf(fabsf(POW2 ? p.scale * kLog2e : p.scale), 1e-30f);
@@ -238,180 +238,184 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       const int len = max(cur.len, 0), row0 = cur.inner * kRows, here = min(kRows, rows - row0);
       const bool last = first_tile + n == cur.tiles, live = (warp & 3) * 32 < here;
       // The item's rows: into shared memory, and this thread's own.
+      const int hd = (row0 + row) / nodes, nd = row0 + row - hd * nodes, head = kvh * heads_per + hd;
+      // Columns [half * D / 2, + D / 2) of this row's query.
+      const bf16* q = reinterpret_cast<const bf16*>(p.q.ptr) + b * p.q.sb + head * p.q.sh + nd * p.q.sn + half * (D / 2);
+      uint4 qv[D / 16];
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) qv[e] = row < here ? *reinterpret_cast<const uint4*>(q + 8 * e) : make_uint4(0, 0, 0, 0);
+      const int next = p.c.next_pos ? p.c.next_pos[b] : len;
       if (masks_of != b) {
         masks_of = b;
         if (warp == 0) node_masks(seen, p.parents ? p.parents + b * nodes : nullptr, nodes, cur.len >= 0, lane);
       }
       if (tid == 0) poison = 0;
-      const int hd = (row0 + row) / nodes, nd = row0 + row - hd * nodes, head = kvh * heads_per + hd;
-      {
-        // Columns [half * D / 2, + D / 2) of this row's query.
-        const bf16* q = reinterpret_cast<const bf16*>(p.q.ptr) + b * p.q.sb + head * p.q.sh + nd * p.q.sn + half * (D / 2);
 #pragma unroll
-        for (int cc = 0; cc < D / 4; cc += 16) {
-          uint32_t w[16];
+      for (int cc = 0; cc < D / 16; cc += 4) {
+        uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row < here) v = *reinterpret_cast<const uint4*>(q + 2 * (cc + e));
-            w[e] = v.x ^ flip;
-            w[e + 1] = v.y ^ flip;
-            w[e + 2] = v.z ^ flip;
-            w[e + 3] = v.w ^ flip;
-          }
-          tmem_st16(tmem + lane_base + kColQ<D> + (uint32_t)(half * (D / 4) + cc), w);
+        for (int e = 0; e < 4; ++e) {
+          w[4 * e] = qv[cc + e].x ^ flip;
+          w[4 * e + 1] = qv[cc + e].y ^ flip;
+          w[4 * e + 2] = qv[cc + e].z ^ flip;
+          w[4 * e + 3] = qv[cc + e].w ^ flip;
         }
-        tmem_wait_st();
+        tmem_st16(tmem + lane_base + kColQ<D> + (uint32_t)(half * (D / 4) + 4 * cc), w);
       }
+      tmem_wait_st();
       tc_fence_before();
       arrive(q_full);
       soft_sync();  // the masks
       const unsigned long long see = row < here ? seen[nd] : 0ull;
-      const int next = p.c.next_pos ? p.c.next_pos[b] : len, at = (int)((unsigned)next + (unsigned)(see ? __popcll(see) - 1 : 0));
+      const int at = (int)((unsigned)next + (unsigned)(see ? __popcll(see) - 1 : 0));
       const float* tab = BIAS ? p.rel_bias + (row < here ? (int64_t)head * p.rel_len : 0) : nullptr;
       const float far = BIAS ? tab[p.rel_len - 1] : 0.f;
       const int32_t* ps = BIAS && p.c.pos ? p.c.pos + (int64_t)(b * p.c.kv_heads + kvh) * p.c.capacity : nullptr;
 
       float m = -INFINITY, l = 0.f;
-      for (int t = 0; t < n; ++t, ++i) {
-        const int tile = first_tile + t, sb = i & 1, pb = i & 1, st = i % NS;
+      for (int t = (half ^ i) & 1; t < n; t += 2) {
+        const int it = i + t, tile = first_tile + t, st = it % NS;
         const bool fresh = tile + 1 == cur.tiles;
-        const int key0 = tile * kTile + c0, valid = fresh ? nodes - c0 : len - key0;  // columns of mine that exist
-        // Positions of this half's keys, one per lane.
-        int mine = 0;
+        const int key0 = tile * kTile, valid = fresh ? nodes : len - key0;  // columns that exist
+        // Positions of the keys, two per lane.
+        int mine[2] = {0, 0};
         bool near = false;
         if (BIAS) {
-          const int k = key0 + lane;
-          if (fresh) {
-            const unsigned long long s = c0 + lane < nodes ? seen[c0 + lane] : 0ull;
-            mine = (int)((unsigned)next + (unsigned)(s ? __popcll(s) - 1 : 0));
-          } else {
-            mine = ps ? ps[min(k, max(len - 1, 0))] : k;
-          }
-          near = __any_sync(0xffffffffu, lane < valid && (int)((unsigned)next - (unsigned)mine) < p.rel_len - 1);
-        }
-        if (ok) ok = wait(s_full + sb, (uint32_t)((i >> 1) & 1));
-        // The TMEM accesses below are .sync.aligned: decide warp-uniformly.
-        ok = __all_sync(0xffffffffu, ok) != 0;
-        if (ok) {
-          tc_fence_after();
-          float x[32];
-          if (live) {
-            tmem_ld16(tmem + lane_base + (uint32_t)(sb * 64 + c0), reinterpret_cast<uint32_t*>(x));
-            tmem_ld16(tmem + lane_base + (uint32_t)(sb * 64 + c0 + 16), reinterpret_cast<uint32_t*>(x) + 16);
-            tmem_wait_ld();
-          }
-          // Values that must not meet the products.
-          const bool cleaned = fresh || (tile + 1) * kTile > len;
-          if (cleaned) {
-            if ((ok = __all_sync(0xffffffffu, wait(kv_full + st, (uint32_t)((i / NS) & 1))) != 0)) {
-              uint8_t* vs = smem + st * 2 * C::kKvBytes + C::kKvBytes;
-              for (int x4 = tid; x4 < kTile * (D / 8); x4 += kSoft) {
-                const int r = x4 / (D / 8), ch = x4 % (D / 8);
-                uint4* v4 = reinterpret_cast<uint4*>(vs + (ch >> 3) * kSub + sw128(r, ch & 7));
-                if (!fresh) {
-                  if (tile * kTile + r >= len) *v4 = make_uint4(0, 0, 0, 0);
-                } else {
-                  uint4 v = *v4;
-                  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-                  bool bad = false;
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, bad = true;
-                    if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, bad = true;
-                  }
-                  if (bad) {
-                    *v4 = v;
-                    if (r < nodes) atomicOr(&poison, 1ull << r);
-                  }
-                }
-              }
-            }
-          }
-          if (live && ok) {
-            if (BIAS) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] *= unit;
-              if (near) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const int pos = __shfl_sync(0xffffffffu, mine, e);
-                  x[e] += __ldg(tab + min(max((int)((unsigned)at - (unsigned)pos), 0), p.rel_len - 1));
-                }
-              } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] += far;
-              }
-            }
+          for (int h = 0; h < 2; ++h) {
+            const int k = 32 * h + lane;
             if (fresh) {
-              const uint32_t bits = (uint32_t)(see >> c0);
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(bits >> e & 1)) x[e] = -INFINITY;
-            } else if (valid < 32 || !see) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (e >= valid || !see) x[e] = -INFINITY;
+              const unsigned long long s = k < nodes ? seen[k] : 0ull;
+              mine[h] = (int)((unsigned)next + (unsigned)(s ? __popcll(s) - 1 : 0));
+            } else {
+              mine[h] = ps ? ps[min(key0 + k, max(len - 1, 0))] : key0 + k;
             }
-            float mt = x[0];
+            near |= k < valid && (int)((unsigned)next - (unsigned)mine[h]) < p.rel_len - 1;
+          }
+          near = __any_sync(0xffffffffu, near);
+        }
+        const int buf = it % kBufs;
+        if (ok) ok = wait(s_full + buf, (uint32_t)((it / kBufs) & 1));
+        // The TMEM accesses below are .sync.aligned: decide warp-uniformly.
+        if (!(ok = __all_sync(0xffffffffu, ok) != 0)) break;
+        tc_fence_after();
+        const uint32_t scores = tmem + lane_base + (uint32_t)(buf * 64);
+        float x[64];
+        if (live) {
 #pragma unroll
-            for (int e = 1; e < 32; ++e) mt = fmaxf(mt, x[e]);
-            if (!BIAS) mt *= unit;  // x itself is scaled where its weight is taken
-            float alpha = 1.f;
-            bool scale = false;
-            if (mt > m + kLazy) {  // also the first tile with a key (m = -inf)
-              if (m != -INFINITY) {
-                alpha = weight(m - mt);
-                scale = true;
+          for (int e = 0; e < 64; e += 16) tmem_ld16(scores + (uint32_t)e, reinterpret_cast<uint32_t*>(x) + e);
+          tmem_wait_ld();
+        }
+        // Values that must not meet the products.
+        const bool cleaned = fresh || (tile + 1) * kTile > len;
+        if (cleaned) {
+          if (!(ok = __all_sync(0xffffffffu, wait(kv_full + st, (uint32_t)((it / NS) & 1))) != 0)) break;
+          uint8_t* vs = smem + st * 2 * C::kKvBytes + C::kKvBytes;
+          for (int x4 = row; x4 < kTile * (D / 8); x4 += kRows) {
+            const int r = x4 / (D / 8), ch = x4 % (D / 8);
+            uint4* v4 = reinterpret_cast<uint4*>(vs + (ch >> 3) * kSub + sw128(r, ch & 7));
+            if (!fresh) {
+              if (key0 + r >= len) *v4 = make_uint4(0, 0, 0, 0);
+            } else {
+              uint4 v = *v4;
+              uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+              bool bad = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u, bad = true;
+                if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu, bad = true;
               }
-              m = mt;
-              l *= alpha;
-            }
-            if (__any_sync(0xffffffffu, scale)) {
-              // O holds products made with the old maximum: scale it once the
-              // last of them has retired (an earlier tile of this item).
-              ok = __all_sync(0xffffffffu, wait(p_empty + ((i - 1) & 1), (uint32_t)(((i - 1) >> 1) & 1))) != 0;
-              if (ok) {
-                tc_fence_after();
-#pragma unroll
-                for (int cc = 0; cc < D; cc += 16) {
-                  uint32_t o[16];
-                  tmem_ld16(tmem + lane_base + ocol + (uint32_t)cc, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                  tmem_st16(tmem + lane_base + ocol + (uint32_t)cc, o);
-                }
-                tmem_wait_st();
+              if (bad) {
+                *v4 = v;
+                if (r < nodes) atomicOr(&poison, 1ull << r);
               }
-            }
-            if (ok) {
-              const float u = m == -INFINITY ? 0.f : m;
-              float sum[4] = {0.f, 0.f, 0.f, 0.f};
-              uint32_t hi[16], lo[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float a = weight(BIAS ? x[2 * e] - u : fmaf(x[2 * e], unit, -u));
-                const float d = weight(BIAS ? x[2 * e + 1] - u : fmaf(x[2 * e + 1], unit, -u));
-                sum[e & 3] += a + d;
-                hi[e] = pack_bf16(a, d);
-                lo[e] = pack_bf16(a - __uint_as_float(hi[e] << 16), d - __uint_as_float(hi[e] & 0xffff0000u));
-              }
-              // Into the place of this half's scores.
-              tmem_st16(tmem + lane_base + (uint32_t)(pb * 64 + c0), hi);
-              tmem_st16(tmem + lane_base + (uint32_t)(pb * 64 + c0 + 16), lo);
-              tmem_wait_st();
-              l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
           }
-          tc_fence_before();
-          if (cleaned) fence_async();
-          arrive(p_full + pb);
+          fence_async();
         }
+        if (live) {
+          if (BIAS) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) x[e] *= unit;
+            if (near) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) {
+                const int pos = __shfl_sync(0xffffffffu, mine[e >> 5], e & 31);
+                x[e] += __ldg(tab + min(max((int)((unsigned)at - (unsigned)pos), 0), p.rel_len - 1));
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) x[e] += far;
+            }
+          }
+          if (fresh) {
+            const uint32_t bits[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (!(bits[e >> 5] >> (e & 31) & 1)) x[e] = -INFINITY;
+          } else if (valid < kTile || !see) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (e >= valid || !see) x[e] = -INFINITY;
+          }
+          float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int e = 4; e < 64; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          if (!BIAS) mt *= unit;  // x itself is scaled where its weight is taken
+          float alpha = 1.f;
+          bool scale = false;
+          if (mt > m + kLazy) {  // also the first tile with a key (m = -inf)
+            if (m != -INFINITY) {
+              alpha = weight(m - mt);
+              scale = true;
+            }
+            m = mt;
+            l *= alpha;
+          }
+          if (__any_sync(0xffffffffu, scale)) {
+            // O holds products made with the old maximum: scale it once the
+            // last of them (this group's tile before) has retired.
+            if (!(ok = __all_sync(0xffffffffu, wait(p_empty + (it - 2) % kBufs, (uint32_t)(((it - 2) / kBufs) & 1))) != 0)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int cc = 0; cc < D; cc += 16) {
+              uint32_t o[16];
+              tmem_ld16(tmem + lane_base + ocol + (uint32_t)cc, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st16(tmem + lane_base + ocol + (uint32_t)cc, o);
+            }
+            tmem_wait_st();
+          }
+          const float u = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          // Into the place of the scores.
+#pragma unroll
+          for (int cc = 0; cc < 64; cc += 32) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float a = weight(BIAS ? x[cc + 2 * e] - u : fmaf(x[cc + 2 * e], unit, -u));
+              const float d = weight(BIAS ? x[cc + 2 * e + 1] - u : fmaf(x[cc + 2 * e + 1], unit, -u));
+              sum[e & 3] += a + d;
+              hi[e] = pack_bf16(a, d);
+              lo[e] = pack_bf16(a - __uint_as_float(hi[e] << 16), d - __uint_as_float(hi[e] & 0xffff0000u));
+            }
+            tmem_st16(scores + (uint32_t)(cc / 2), hi);
+            tmem_st16(scores + (uint32_t)(32 + cc / 2), lo);
+          }
+          tmem_wait_st();
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        tc_fence_before();
+        arrive(p_full + buf);
       }
+      i += n;
       if (ok) ok = wait(o_done, (uint32_t)(seg & 1));
       ok = __all_sync(0xffffffffu, ok) != 0;
-      // Join the halves; every softmax thread passes here once per item.
+      // Join the groups; every softmax thread passes here once per item.
       xm[half][row] = m;
       xl[half][row] = l;
       soft_sync();
@@ -423,7 +427,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       if (live) {
         tc_fence_after();
         const float inv = !ok ? NAN : empty ? 0.f : whole ? 1.f / sum : 1.f;
-        float* part = p.ws + (int64_t)(blockIdx.x * 2 + (first_tile == 0)) * kRows * (D + 2) + row * D;
+        float* part = p.ws + (int64_t)(blockIdx.x * 2 + (first_tile == 0)) * kRows * (D + 2) + row * 4;
         bf16* out = row < here ? reinterpret_cast<bf16*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + nd * p.out.sn
                                : nullptr;
         // Columns [half * D / 2, + D / 2) of this row.
@@ -435,7 +439,11 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
           tmem_ld16(tmem + lane_base + kColO + (uint32_t)(D + col), reinterpret_cast<uint32_t*>(o1));
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o0[e] = empty && ok ? 0.f : (o0[e] * a0 + o1[e] * a1) * inv;
+          for (int e = 0; e < 16; ++e) {
+            // A group that had no tile has no accumulator either.
+            const float both = (m0 == -INFINITY ? 0.f : o0[e] * a0) + (m1 == -INFINITY ? 0.f : o1[e] * a1);
+            o0[e] = empty && ok ? 0.f : both * inv;
+          }
           for (unsigned long long s = bad; s; s &= s - 1) {
             const int j = __ffsll((long long)s) - 1;
             const bf16* vr = reinterpret_cast<const bf16*>(p.v_new.ptr) + b * p.v_new.sb + kvh * p.v_new.sh + j * p.v_new.sn + col;
@@ -454,7 +462,8 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
               *reinterpret_cast<uint4*>(out + col + 8) = make_uint4(w[4], w[5], w[6], w[7]);
             } else {
 #pragma unroll
-              for (int e = 0; e < 16; e += 2) store2(part + col + e, o0[e], o0[e + 1]);
+              for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<float4*>(part + (col + e) * kRows) = make_float4(o0[e], o0[e + 1], o0[e + 2], o0[e + 3]);
             }
           }
         }
@@ -520,7 +529,7 @@ cudaError_t tc_run(const TreeParams& p, cudaStream_t s) {
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(c.batch * c.kv_heads * p.row_blocks, kRows / 4);
+  cfg.gridDim = join_grid(p, kRows, D);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = (2 * c.batch + 1) * 4;
   cfg.stream = s;

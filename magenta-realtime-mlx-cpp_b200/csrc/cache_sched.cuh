@@ -157,7 +157,12 @@ __device__ __forceinline__ void store2(__nv_bfloat16* p, float a, float b) {
 }
 __device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 
-// Joins the partial rows of items that several CTAs worked on: a warp per row.
+// Joins the partial rows of items that several CTAs worked on. A CTA's two
+// partial blocks of mb rows hold [head_dim / 4][row][4] sums, then the rows'
+// maxima (natural units) and sums of weights. A thread per row and four columns.
+inline dim3 join_grid(const TreeParams& p, int mb, int d) {
+  return dim3(p.c.batch * p.c.kv_heads * p.row_blocks, (mb * d / 4 + kThreads - 1) / kThreads);
+}
 template <typename T, int D, bool APART>
 __global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_constant__ TreeParams p, int mb) {
   extern __shared__ __align__(16) int sched[];
@@ -169,44 +174,36 @@ __global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_consta
   const int c0 = owner(w, parts, total), c1 = owner(w + tiles - 1, parts, total);
   pdl_wait();
   if (c0 == c1) return;
-  const int lane = threadIdx.x & 31, r = blockIdx.y * (kThreads / 32) + (threadIdx.x >> 5);
+  const int at = blockIdx.y * kThreads + threadIdx.x, r = at % mb, quad = at / mb;
   const int heads_per = p.heads / p.c.kv_heads, row = (item % p.row_blocks) * mb + r;
-  if (r >= mb || row >= heads_per * nodes) return;
+  if (quad >= D / 4 || row >= heads_per * nodes) return;
+  // The first CTA began with the item (its block 1), the others went on with it.
   auto part = [&](int c) { return p.ws + (int64_t)(c * 2 + (c == c0)) * mb * (D + 2); };
   float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, part(c)[mb * D + r]);
-  m = warp_max(m);
-  const float u = m == -INFINITY ? 0.f : m;
-  constexpr int V = D / 32;
-  float acc[V] = {}, sum = 0.f;
-  for (int cb = c0; cb <= c1; cb += 32) {
-    const int mine = cb + lane;
-    float wt = 0.f;
-    if (mine <= c1) {
-      wt = ex2((part(mine)[mb * D + r] - u) * kLog2e);
-      const float l = part(mine)[mb * D + mb + r];
-      sum += l == 0.f ? 0.f : l * wt;
-    }
-    const int n = min(32, c1 - cb + 1);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float f = __shfl_sync(0xffffffffu, wt, i);
-      const float* src = part(cb + i) + r * D + lane * V;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float v = src[k];
-        if (!(f == 0.f)) acc[k] += v * f;
-      }
-    }
+  for (int c = c0; c <= c1; ++c) m = fmaxf(m, part(c)[mb * D + r]);
+  const float u = m == -INFINITY ? 0.f : m;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const float* src = part(c);
+    const float f = ex2((src[mb * D + r] - u) * kLog2e), l = src[mb * D + mb + r];
+    const float4 v = *reinterpret_cast<const float4*>(src + (quad * mb + r) * 4);
+    if (f == 0.f) continue;  // an empty part's sums may be anything
+    sum += l * f;
+    acc.x += v.x * f;
+    acc.y += v.y * f;
+    acc.z += v.z * f;
+    acc.w += v.w * f;
   }
-  sum = warp_sum(sum);
   const int hd = row / nodes, n = row - hd * nodes, head = (item / p.row_blocks) * heads_per + hd;
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + n * p.out.sn + lane * V;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int k = 0; k < V; k += 2)
-    store2(dst + k, sum == 0.f ? 0.f : acc[k] * inv, sum == 0.f ? 0.f : acc[k + 1] * inv);
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.heads + head) * nodes + n] = sum == 0.f ? -INFINITY : m + logf(sum);
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + n * p.out.sn + quad * 4;
+  const bool empty = sum == 0.f;
+  const float inv = empty ? 0.f : 1.f / sum;
+  store2(dst, empty ? 0.f : acc.x * inv, empty ? 0.f : acc.y * inv);
+  store2(dst + 2, empty ? 0.f : acc.z * inv, empty ? 0.f : acc.w * inv);
+  if (p.lse && quad == 0) p.lse[((int64_t)b * p.heads + head) * nodes + n] = empty ? -INFINITY : m + logf(sum);
 }
 
 }  // namespace mrtdf
