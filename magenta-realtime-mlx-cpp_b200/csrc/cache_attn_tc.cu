@@ -10,16 +10,17 @@
 // the scores they came from) are in TMEM: read from shared memory, 64 columns at
 // a time, they alone kept the products at a third of their rate.
 //
-// CTA of 320 threads, one per SM, over an equal run of the key tiles of all
+// CTA of 576 threads, one per SM, over an equal run of the key tiles of all
 // items (cache_sched.cuh); roles and hand-over as in enc_attn_tc.cu:
-//   warps 0-7  softmax: two groups of four warps take turns at the tiles, a
-//              thread per query row, each group with a running maximum and an
-//              accumulator of its own, so that one's exponentials overlap the
-//              other's products (rows that do not exist skip the work: their
+//   warps 0-15 softmax: two groups of eight warps take turns at the tiles, each
+//              with a running maximum and an accumulator of its own, so that
+//              one's exponentials overlap the other's products; two threads per
+//              query row, each with 32 of the 64 columns, who tell each other
+//              their maxima (rows that do not exist skip the work: their
 //              queries are zero, their scores stay zero bits);
-//   warp 8     TMA producer: K and V tiles through a ring, 128-byte swizzle,
+//   warp 16    TMA producer: K and V tiles through a ring, 128-byte swizzle,
 //              over the items of the run without a stop;
-//   warp 9     MMA issuer: S = Q K^T into one of three TMEM buffers, three
+//   warp 17    MMA issuer: S = Q K^T into one of three TMEM buffers, three
 //              tiles ahead, then O_g += P V for the tile's group g, weights as two bf16 parts (16 bits of a
 //              weight; the second product is hidden too).
 //              V is an MN-major operand of 64-column parts kSub bytes apart.
@@ -42,7 +43,7 @@ using namespace tcg;
 typedef __nv_bfloat16 bf16;
 
 constexpr int kRows = 128;
-constexpr int kSoft = 256;              // softmax threads
+constexpr int kSoft = 512;              // softmax threads
 constexpr int kTcThreads = kSoft + 64;  // and the TMA and MMA warps
 constexpr int kSub = 64 * 128;          // 64 rows of 128 bytes (64 columns)
 constexpr float kLazy = 8.f;
@@ -72,14 +73,32 @@ struct TcMaps {
   CUtensorMap k, v, kn, vn;
 };
 
-// A in TMEM (row = lane, two bf16 per column), B in shared memory.
-__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A in TMEM (row = lane, two bf16 per column), B in shared memory. One lane of
+// the warp issues; the operands are the same in all of them, so they can be
+// kept in uniform registers (a single lane's branch has to move five operands
+// there for every product, 80 clocks each).
+__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ bool elected() {
+  uint32_t e;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -102,7 +121,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   int* first = lens + p.c.batch;
   __shared__ int abort_flag;
   __shared__ unsigned long long seen[kOpMaxNodes], poison;
-  __shared__ float xm[2][kRows], xl[2][kRows];
+  __shared__ float xm[2][kRows], xl[4][kRows], tops[2][2][2][kRows];  // tops: [slot][group][half][row]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int batch = p.c.batch, blocks = p.row_blocks, items = p.c.kv_heads * blocks, nodes = p.nodes;
@@ -123,7 +142,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, kSoft / 2);
+      mbar_init(p_full + i, kSoft / 2);  // one group
       mbar_init(p_empty + i, 1);
     }
     fence_mbar_init();
@@ -172,64 +191,82 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     }
   } else if (warp == kSoft / 32 + 1) {
     // ---- MMA issuer ----
-    if (lane == 0) {
-      // Descriptors differ in the start address alone (units of 16 bytes, which
-      // do not carry out of their field): one add per product.
-      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem));
-      const uint64_t dv0 = (dk0 & ~((uint64_t)0x3fff << 16)) | (uint64_t)(kSub / 16) << 16;  // LBO: the next 64 columns
-      bool ok = true;
-      auto issue_s = [&](int i) -> bool {
-        const int st = i % NS, sb = i % kBufs;
-        if (!wait(kv_full + st, (uint32_t)((i / NS) & 1))) return false;
-        if (i >= kBufs && !wait(p_empty + sb, (uint32_t)((i / kBufs - 1) & 1))) return false;
-        tc_fence_after();
-        const uint64_t dk = dk0 + (uint64_t)(st * 2 * C::kKvBytes / 16);
+    // The whole warp goes through it with the same values.
+    auto all = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    auto wait_all = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
+    const uint32_t tm = (uint32_t)all((int)tmem);
+    // Descriptors differ in the start address alone (units of 16 bytes, which
+    // do not carry out of their field): one add per product.
+    const uint64_t dk0 = smem_desc_sw128(smem_u32(smem));
+    const uint64_t dv0 = (dk0 & ~((uint64_t)0x3fff << 16)) | (uint64_t)(kSub / 16) << 16;  // LBO: the next 64 columns
+    const uint32_t k_lo = (uint32_t)all((int)(uint32_t)dk0), k_hi = (uint32_t)(dk0 >> 32);
+    const uint32_t v_lo = (uint32_t)all((int)(uint32_t)dv0), v_hi = (uint32_t)(dv0 >> 32);
+    bool ok = true;
+    auto issue_s = [&](int i) -> bool {
+      const int st = i % NS, sb = i % kBufs;
+      if (!wait_all(kv_full + st, (uint32_t)((i / NS) & 1))) return false;
+      if (i >= kBufs && !wait_all(p_empty + sb, (uint32_t)((i / kBufs - 1) & 1))) return false;
+      tc_fence_after();
+      const uint32_t lo = k_lo + (uint32_t)(st * 2 * C::kKvBytes / 16), d = tm + (uint32_t)(sb * 64);
+      if (elected()) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma(tmem + (uint32_t)(sb * 64), tmem + kColQ<D> + kk * 8, dk + ((kk >> 2) * kSub + (kk & 3) * 32) / 16, idesc(64), kk != 0);
+          umma(d, tm + kColQ<D> + kk * 8, lo + ((kk >> 2) * kSub + (kk & 3) * 32) / 16, k_hi, idesc(64), kk != 0);
         mma_commit(s_full + sb);
-        return true;
-      };
-      int i = 0;
-      for (int seg = 0; ok && cur.w < w1; ++seg) {
-        const int n = min(cur.tiles - cur.tile, w1 - cur.w);  // tiles of the item's run
-        if (!(ok = wait(q_full, (uint32_t)(seg & 1)))) break;
-        for (int t = 0; ok && t < min(n, kBufs); ++t) ok = issue_s(i + t);
-        for (int t = 0; ok && t < n; ++t, ++i) {
-          const int st = i % NS, pb = i % kBufs, og = i & 1;
-          if (!(ok = wait(p_full + pb, (uint32_t)((i / kBufs) & 1)))) break;
-          tc_fence_after();
-          const uint64_t dv = dv0 + (uint64_t)((st * 2 + 1) * C::kKvBytes / 16);
+      }
+      __syncwarp();
+      return true;
+    };
+    int i = 0;
+    const int end = all(w1);
+    int w = all(cur.w);
+    for (int seg = 0; ok && w < end; ++seg) {
+      const int n = all(min(cur.tiles - cur.tile, w1 - cur.w));  // tiles of the item's run
+      if (!(ok = wait_all(q_full, (uint32_t)(seg & 1)))) break;
+      for (int t = 0; ok && t < min(n, kBufs); ++t) ok = issue_s(i + t);
+      for (int t = 0; ok && t < n; ++t, ++i) {
+        const int st = i % NS, pb = i % kBufs, og = i & 1;
+        if (!(ok = wait_all(p_full + pb, (uint32_t)((i / kBufs) & 1)))) break;
+        tc_fence_after();
+        const uint32_t lo = v_lo + (uint32_t)((st * 2 + 1) * C::kKvBytes / 16), d = tm + kColO + (uint32_t)(og * D);
+        const uint32_t a = tm + (uint32_t)(pb * 64);
+        if (elected()) {
 #pragma unroll
           for (int part = 0; part < 2; ++part)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma(tmem + kColO + (uint32_t)(og * D), tmem + (uint32_t)(pb * 64 + part * 32 + kk * 8), dv + kk * 2048 / 16,
-                   idesc(D) | kMnMajorB, (part || t >= 2 || kk) ? 1u : 0u);
+              umma(d, a + part * 32 + kk * 8, lo + kk * 2048 / 16, v_hi, idesc(D) | kMnMajorB, (part || kk) ? 1u : (uint32_t)(t >= 2));
           mma_commit(p_empty + pb);
           mma_commit(kv_empty + st);
-          if (t + kBufs < n) ok = issue_s(i + kBufs);  // once these products have retired
         }
-        if (ok) mma_commit(o_done);
-        // To the next item.
-        cur.w += n - 1;
-        cur.tile += n - 1;
-        cur.next(lens, batch, p.c.kv_heads, blocks, nodes);
+        __syncwarp();
+        if (t + kBufs < n) ok = issue_s(i + kBufs);  // once these products have retired
       }
-      // Every product issued so far has retired before TMEM is released.
-      mma_commit(drain);
-      mbar_wait_bounded(drain, 0, nullptr);
+      if (ok && elected()) mma_commit(o_done);
+      __syncwarp();
+      // To the next item.
+      cur.w += n - 1;
+      cur.tile += n - 1;
+      cur.next(lens, batch, p.c.kv_heads, blocks, nodes);
+      w += n;
     }
+    // Every product issued so far has retired before TMEM is released.
+    if (elected()) mma_commit(drain);
+    __syncwarp();
+    mbar_wait_bounded(drain, 0, nullptr);
   } else {
     // ---- softmax ----
-    const int row = tid & (kRows - 1), half = tid >> 7;
+    const int row = tid & (kRows - 1), group = (tid >> 7) & 1, half = tid >> 8, part4 = group * 2 + half;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ocol = kColO + (uint32_t)(half * D);  // half: the group, too
+    const uint32_t ocol = kColO + (uint32_t)(group * D + half * (D / 2));  // this thread's columns of O when it is scaled
     constexpr bool POW2 = !BIAS;
     // Not zero: it multiplies -inf.
     const float unit = fmaxf(fabsf(POW2 ? p.scale * kLog2e : p.scale), 1e-30f);
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale is the queries'
+    const int c0 = half * 32;  // first column of this thread's half
     auto weight = [](float x) { return ex2(POW2 ? x : x * kLog2e); };
+    // The two threads of each row of this warp's quarter.
+    auto row_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + group * 4 + (warp & 3)) : "memory"); };
     auto soft_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory"); };
     bool ok = true;
     int i = 0, masks_of = -1;
@@ -239,28 +276,30 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       const bool last = first_tile + n == cur.tiles, live = (warp & 3) * 32 < here;
       // The item's rows: into shared memory, and this thread's own.
       const int hd = (row0 + row) / nodes, nd = row0 + row - hd * nodes, head = kvh * heads_per + hd;
-      // Columns [half * D / 2, + D / 2) of this row's query.
-      const bf16* q = reinterpret_cast<const bf16*>(p.q.ptr) + b * p.q.sb + head * p.q.sh + nd * p.q.sn + half * (D / 2);
-      uint4 qv[D / 16];
+      // 32 columns of this row's query (head_dim 64: two threads have them all).
+      const bool takes = D == 128 || half == 0;
+      const int q_part = D == 128 ? part4 : group;
+      const bf16* q = reinterpret_cast<const bf16*>(p.q.ptr) + b * p.q.sb + head * p.q.sh + nd * p.q.sn + q_part * 32;
+      uint4 qv[4];
 #pragma unroll
-      for (int e = 0; e < D / 16; ++e) qv[e] = row < here ? *reinterpret_cast<const uint4*>(q + 8 * e) : make_uint4(0, 0, 0, 0);
+      for (int e = 0; e < 4; ++e)
+        qv[e] = takes && row < here ? *reinterpret_cast<const uint4*>(q + 8 * e) : make_uint4(0, 0, 0, 0);
       const int next = p.c.next_pos ? p.c.next_pos[b] : len;
       if (masks_of != b) {
         masks_of = b;
         if (warp == 0) node_masks(seen, p.parents ? p.parents + b * nodes : nullptr, nodes, cur.len >= 0, lane);
       }
       if (tid == 0) poison = 0;
-#pragma unroll
-      for (int cc = 0; cc < D / 16; cc += 4) {
+      if (takes) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[4 * e] = qv[cc + e].x ^ flip;
-          w[4 * e + 1] = qv[cc + e].y ^ flip;
-          w[4 * e + 2] = qv[cc + e].z ^ flip;
-          w[4 * e + 3] = qv[cc + e].w ^ flip;
+          w[4 * e] = qv[e].x ^ flip;
+          w[4 * e + 1] = qv[e].y ^ flip;
+          w[4 * e + 2] = qv[e].z ^ flip;
+          w[4 * e + 3] = qv[e].w ^ flip;
         }
-        tmem_st16(tmem + lane_base + kColQ<D> + (uint32_t)(half * (D / 4) + 4 * cc), w);
+        tmem_st16(tmem + lane_base + kColQ<D> + (uint32_t)(q_part * 16), w);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -273,26 +312,22 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       const int32_t* ps = BIAS && p.c.pos ? p.c.pos + (int64_t)(b * p.c.kv_heads + kvh) * p.c.capacity : nullptr;
 
       float m = -INFINITY, l = 0.f;
-      for (int t = (half ^ i) & 1; t < n; t += 2) {
+      for (int t = (group ^ i) & 1; t < n; t += 2) {
         const int it = i + t, tile = first_tile + t, st = it % NS;
         const bool fresh = tile + 1 == cur.tiles;
         const int key0 = tile * kTile, valid = fresh ? nodes : len - key0;  // columns that exist
-        // Positions of the keys, two per lane.
-        int mine[2] = {0, 0};
+        // Positions of this half's keys, one per lane.
+        int mine = 0;
         bool near = false;
         if (BIAS) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = 32 * h + lane;
-            if (fresh) {
-              const unsigned long long s = k < nodes ? seen[k] : 0ull;
-              mine[h] = (int)((unsigned)next + (unsigned)(s ? __popcll(s) - 1 : 0));
-            } else {
-              mine[h] = ps ? ps[min(key0 + k, max(len - 1, 0))] : key0 + k;
-            }
-            near |= k < valid && (int)((unsigned)next - (unsigned)mine[h]) < p.rel_len - 1;
+          const int k = c0 + lane;
+          if (fresh) {
+            const unsigned long long s = k < nodes ? seen[k] : 0ull;
+            mine = (int)((unsigned)next + (unsigned)(s ? __popcll(s) - 1 : 0));
+          } else {
+            mine = ps ? ps[min(key0 + k, max(len - 1, 0))] : key0 + k;
           }
-          near = __any_sync(0xffffffffu, near);
+          near = __any_sync(0xffffffffu, k < valid && (int)((unsigned)next - (unsigned)mine) < p.rel_len - 1);
         }
         const int buf = it % kBufs;
         if (ok) ok = wait(s_full + buf, (uint32_t)((it / kBufs) & 1));
@@ -300,10 +335,10 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         if (!(ok = __all_sync(0xffffffffu, ok) != 0)) break;
         tc_fence_after();
         const uint32_t scores = tmem + lane_base + (uint32_t)(buf * 64);
-        float x[64];
+        float x[32];
         if (live) {
-#pragma unroll
-          for (int e = 0; e < 64; e += 16) tmem_ld16(scores + (uint32_t)e, reinterpret_cast<uint32_t*>(x) + e);
+          tmem_ld16(scores + (uint32_t)c0, reinterpret_cast<uint32_t*>(x));
+          tmem_ld16(scores + (uint32_t)(c0 + 16), reinterpret_cast<uint32_t*>(x) + 16);
           tmem_wait_ld();
         }
         // Values that must not meet the products.
@@ -311,7 +346,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         if (cleaned) {
           if (!(ok = __all_sync(0xffffffffu, wait(kv_full + st, (uint32_t)((it / NS) & 1))) != 0)) break;
           uint8_t* vs = smem + st * 2 * C::kKvBytes + C::kKvBytes;
-          for (int x4 = row; x4 < kTile * (D / 8); x4 += kRows) {
+          for (int x4 = half * kRows + row; x4 < kTile * (D / 8); x4 += 2 * kRows) {
             const int r = x4 / (D / 8), ch = x4 % (D / 8);
             uint4* v4 = reinterpret_cast<uint4*>(vs + (ch >> 3) * kSub + sw128(r, ch & 7));
             if (!fresh) {
@@ -336,32 +371,38 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         if (live) {
           if (BIAS) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e) x[e] *= unit;
+            for (int e = 0; e < 32; ++e) x[e] *= unit;
             if (near) {
 #pragma unroll
-              for (int e = 0; e < 64; ++e) {
-                const int pos = __shfl_sync(0xffffffffu, mine[e >> 5], e & 31);
+              for (int e = 0; e < 32; ++e) {
+                const int pos = __shfl_sync(0xffffffffu, mine, e);
                 x[e] += __ldg(tab + min(max((int)((unsigned)at - (unsigned)pos), 0), p.rel_len - 1));
               }
             } else {
 #pragma unroll
-              for (int e = 0; e < 64; ++e) x[e] += far;
+              for (int e = 0; e < 32; ++e) x[e] += far;
             }
           }
           if (fresh) {
-            const uint32_t bits[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
+            const uint32_t bits = (uint32_t)(see >> c0);
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (!(bits[e >> 5] >> (e & 31) & 1)) x[e] = -INFINITY;
+            for (int e = 0; e < 32; ++e)
+              if (!(bits >> e & 1)) x[e] = -INFINITY;
           } else if (valid < kTile || !see) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (e >= valid || !see) x[e] = -INFINITY;
+            for (int e = 0; e < 32; ++e)
+              if (c0 + e >= valid || !see) x[e] = -INFINITY;
           }
           float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-          for (int e = 4; e < 64; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          for (int e = 4; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
           float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          // The row's: the other thread has its scores in registers, too, when
+          // it tells its maximum, so the weights may take their place.
+          const int slot = (it >> 1) & 1;
+          tops[slot][group][half][row] = mt;
+          row_sync();
+          mt = fmaxf(mt, tops[slot][group][half ^ 1][row]);
           if (!BIAS) mt *= unit;  // x itself is scaled where its weight is taken
           float alpha = 1.f;
           bool scale = false;
@@ -379,7 +420,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
             if (!(ok = __all_sync(0xffffffffu, wait(p_empty + (it - 2) % kBufs, (uint32_t)(((it - 2) / kBufs) & 1))) != 0)) break;
             tc_fence_after();
 #pragma unroll
-            for (int cc = 0; cc < D; cc += 16) {
+            for (int cc = 0; cc < D / 2; cc += 16) {
               uint32_t o[16];
               tmem_ld16(tmem + lane_base + ocol + (uint32_t)cc, o);
               tmem_wait_ld();
@@ -387,24 +428,23 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
               tmem_st16(tmem + lane_base + ocol + (uint32_t)cc, o);
             }
-            tmem_wait_st();
           }
           const float u = m == -INFINITY ? 0.f : m;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
           // Into the place of the scores.
 #pragma unroll
-          for (int cc = 0; cc < 64; cc += 32) {
-            uint32_t hi[16], lo[16];
+          for (int cc = 0; cc < 32; cc += 16) {
+            uint32_t hi[8], lo[8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < 8; ++e) {
               const float a = weight(BIAS ? x[cc + 2 * e] - u : fmaf(x[cc + 2 * e], unit, -u));
               const float d = weight(BIAS ? x[cc + 2 * e + 1] - u : fmaf(x[cc + 2 * e + 1], unit, -u));
               sum[e & 3] += a + d;
               hi[e] = pack_bf16(a, d);
               lo[e] = pack_bf16(a - __uint_as_float(hi[e] << 16), d - __uint_as_float(hi[e] & 0xffff0000u));
             }
-            tmem_st16(scores + (uint32_t)(cc / 2), hi);
-            tmem_st16(scores + (uint32_t)(32 + cc / 2), lo);
+            tmem_st8(scores + (uint32_t)((c0 + cc) / 2), hi);
+            tmem_st8(scores + (uint32_t)(32 + (c0 + cc) / 2), lo);
           }
           tmem_wait_st();
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -416,11 +456,11 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       if (ok) ok = wait(o_done, (uint32_t)(seg & 1));
       ok = __all_sync(0xffffffffu, ok) != 0;
       // Join the groups; every softmax thread passes here once per item.
-      xm[half][row] = m;
-      xl[half][row] = l;
+      if (half == 0) xm[group][row] = m;
+      xl[part4][row] = l;
       soft_sync();
       const float m0 = xm[0][row], m1 = xm[1][row], mx = fmaxf(m0, m1), u = mx == -INFINITY ? 0.f : mx;
-      const float a0 = weight(m0 - u), a1 = weight(m1 - u), sum = xl[0][row] * a0 + xl[1][row] * a1;
+      const float a0 = weight(m0 - u), a1 = weight(m1 - u), sum = (xl[0][row] + xl[1][row]) * a0 + (xl[2][row] + xl[3][row]) * a1;
       const float mn = POW2 ? mx * kLn2 : mx;
       const bool whole = first_tile == 0 && last, empty = !see || sum == 0.f;
       const unsigned long long bad = last ? poison & see : 0ull;
@@ -430,10 +470,10 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         float* part = p.ws + (int64_t)(blockIdx.x * 2 + (first_tile == 0)) * kRows * (D + 2) + row * 4;
         bf16* out = row < here ? reinterpret_cast<bf16*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + nd * p.out.sn
                                : nullptr;
-        // Columns [half * D / 2, + D / 2) of this row.
+        // A quarter of this row's columns.
 #pragma unroll
-        for (int cc = 0; cc < D / 2; cc += 16) {
-          const int col = half * (D / 2) + cc;
+        for (int cc = 0; cc < D / 4; cc += 16) {
+          const int col = part4 * (D / 4) + cc;
           float o0[16], o1[16];
           tmem_ld16(tmem + lane_base + kColO + (uint32_t)col, reinterpret_cast<uint32_t*>(o0));
           tmem_ld16(tmem + lane_base + kColO + (uint32_t)(D + col), reinterpret_cast<uint32_t*>(o1));
@@ -467,7 +507,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
             }
           }
         }
-        if (row < here && half == 0) {
+        if (row < here && part4 == 0) {
           if (whole) {
             if (p.lse) p.lse[((int64_t)b * p.heads + head) * nodes + nd] = !ok ? NAN : empty ? -INFINITY : mn + logf(sum);
           } else {
@@ -518,7 +558,7 @@ cudaError_t tc_run(const TreeParams& p, cudaStream_t s) {
       !make_map(&maps.vn, p.v_new.ptr, D, p.nodes, c.kv_heads, c.batch, p.v_new.sn, p.v_new.sh, p.v_new.sb))
     return cudaErrorInvalidValue;
   constexpr auto K = tree_attn_tc_kernel<D, BIAS>;
-  constexpr int kMost = 220 * 1024;
+  constexpr int kMost = 216 * 1024;  // next to 8 KB of static shared memory
   static_assert(TcCfg<D>::kOffSched + (2 * kOpMaxBatch + 1) * 4 + 1024 <= kMost, "fits");
   cudaError_t e = allow_smem<K, kMost>();
   if (e != cudaSuccess) return e;
