@@ -490,7 +490,7 @@ struct MassSmem {
   static constexpr int kStageBytes = kTile * Rows<T, D>::kBytes;
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kQ = kMassRows * Rows<T, D>::kBytes;
-  static constexpr int kFixed = kRing + kQ + kStages * kTile * 4 + kMassRows * 4 + kOpMaxNodes * 4;
+  static constexpr int kFixed = kRing + kQ + kStages * kTile * 4 + 3 * kMassRows * 4 + kOpMaxNodes * 4;
   static int bytes(int batch) { return kFixed + (2 * batch + 1) * 4; }
 };
 
@@ -529,11 +529,16 @@ template <typename T, int D, bool BIAS>
 __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_constant__ MassParams p) {
   using R = Rows<T, D>;
   using S = MassSmem<T, D>;
+  // As in the attention: powers of two where the last bits do not matter.
+  constexpr bool POW2 = !BIAS && sizeof(T) == 2;
+  const float unit = POW2 ? p.scale * kLog2e : p.scale;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* q_s = smem + S::kRing;
   int* pos_s = reinterpret_cast<int*>(q_s + S::kQ);
   float* lse_s = reinterpret_cast<float*>(pos_s + kStages * kTile);
-  int* path_s = reinterpret_cast<int*>(lse_s + kMassRows);
+  int* node_s = reinterpret_cast<int*>(lse_s + kMassRows);  // of each row: its place on the path,
+  int* head_s = node_s + kMassRows;                         // its query head of the kv head
+  int* path_s = head_s + kMassRows;
   int* lens = path_s + kOpMaxNodes;
   int* first = lens + p.c.batch;
 
@@ -599,11 +604,21 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
       for (int i = tid; i < kMassRows * R::kChunks; i += kThreads) {
         const int row = i / R::kChunks, ch = i % R::kChunks, r = rb + row;
         uint4 v = make_uint4(0, 0, 0, 0);
+        if (ch == 0) {  // a row that does not exist: weights of exp(-inf)
+          lse_s[row] = INFINITY;
+          node_s[row] = head_s[row] = 0;
+        }
         if (row < here) {
-          const int hd = r / count, n = path_s[r - hd * count], head = kvh * heads_per + hd;
+          const int hd = r / count, at = r - hd * count, n = path_s[at], head = kvh * heads_per + hd;
           v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q.ptr) + layer * p.q.sl + b * p.q.sb +
                                               head * p.q.sh + n * p.q.sn + ch * (16 / sizeof(T)));
-          if (ch == 0) lse_s[row] = p.lse[((int64_t)(layer * batch + b) * p.heads + head) * p.nodes + n];
+          if (ch == 0) {
+            // A row whose softmax is empty (lse = -inf) gives nothing either.
+            const float lse = p.lse[((int64_t)(layer * batch + b) * p.heads + head) * p.nodes + n];
+            lse_s[row] = lse == -INFINITY ? INFINITY : POW2 ? lse * kLog2e : lse;
+            node_s[row] = at;
+            head_s[row] = hd;
+          }
         }
         *reinterpret_cast<uint4*>(q_s + R::at(row, ch)) = v;
       }
@@ -634,33 +649,30 @@ __global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_const
                             : 0.f;
           }
         float col[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        const bool tail = key0 + 16 > len;
         for (int mt = 0; mt * 16 < here; ++mt) {
           if (here > 16) q_from_smem<D>(q, smem_u32(q_s) + mt * 16 * R::kBytes, lane);
           float s[2][4] = {};
           qk_tile<D, 2>(s, q, keys, lane);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int row = mt * 16 + g + 8 * h, r = rb + row;
-            if (row >= here) continue;
-            const int hd = r / count, i = r - hd * count;
+            const int row = mt * 16 + g + 8 * h, i = BIAS || tail ? node_s[row] : 0;
             const float lse = lse_s[row];
-            const float* tab = BIAS ? p.rel_bias + (int64_t)(kvh * heads_per + hd) * p.rel_len : nullptr;
+            const float* tab = BIAS ? p.rel_bias + (int64_t)(kvh * heads_per + head_s[row]) * p.rel_len : nullptr;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const int key = key0 + 8 * j + 2 * c + e;
-                float x = s[j][2 * h + e] * p.scale;
+                const int k = 8 * j + 2 * c + e;
+                float x = s[j][2 * h + e] * unit;
                 if (BIAS) {
-                  const int at = key >= len ? next + (key - len)
-                                 : p.c.pos  ? pos_s[st * kTile + warp * 16 + 8 * j + 2 * c + e]
-                                            : key;
-                  const int d = min(max((int)((unsigned)(next + i) - (unsigned)at), 0), p.rel_len - 1);
-                  x += __ldg(tab + d);
+                  const int at = key0 + k >= len ? next + (key0 + k - len)
+                                 : p.c.pos       ? pos_s[st * kTile + warp * 16 + k]
+                                                 : key0 + k;
+                  x += __ldg(tab + min(max((int)((unsigned)(next + i) - (unsigned)at), 0), p.rel_len - 1));
                 }
-                // A row whose softmax is empty (lse = -inf) gives nothing.
-                const bool on = key - len <= i && lse != -INFINITY;
-                col[j][e] += on ? ex2((x - lse) * kLog2e) : 0.f;
+                const float w = ex2(POW2 ? x - lse : (x - lse) * kLog2e);
+                col[j][e] += !tail || key0 + k - len <= i ? w : 0.f;
               }
           }
         }

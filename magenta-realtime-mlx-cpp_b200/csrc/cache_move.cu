@@ -161,7 +161,19 @@ __global__ __launch_bounds__(kEvictThreads, 4) void cache_evict_kernel(const __g
   int need = p.budget;    // `need` of its equals too (the lowest ones),
   bool some = false;      // which are not all of them
   if (counted) {
-    for (int t = tid; t < slice; t += kEvictThreads) keys[t] = t < len ? key_of(pos[t], mass[t]) : 0u;
+    for (int t = tid; t < slice; t += kEvictThreads) {
+      uint32_t k = 0;
+      if (t < len) {
+        const int at = pos[t];
+        const float w = mass[t];
+        k = key_of(at, w);
+        if (apart && t < p.budget) {
+          mass_out[t] = w;
+          pos_out[t] = at;
+        }
+      }
+      keys[t] = k;
+    }
     __syncthreads();
   } else {
     for (int i = tid; i < kBins; i += kEvictThreads) s.hist[i] = s.all[0][i] = s.all[1][i] = 0;
@@ -187,7 +199,14 @@ __global__ __launch_bounds__(kEvictThreads, 4) void cache_evict_kernel(const __g
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             k[u] = key_of(at[u], w[u]);
-            if (held && t0 + u * kEvictThreads < hi) keys[t0 + u * kEvictThreads - lo] = k[u];
+            const int t = t0 + u * kEvictThreads;
+            if (held && t < hi) keys[t - lo] = k[u];
+            // What stays in its slot; a hole's entry is written again when it is
+            // filled, barriers later.
+            if (pass == 0 && apart && t < hi && t < p.budget) {
+              mass_out[t] = w[u];
+              pos_out[t] = at[u];
+            }
           }
         }
 #pragma unroll
@@ -317,7 +336,8 @@ __global__ __launch_bounds__(kEvictThreads, 4) void cache_evict_kernel(const __g
   const int fill0 = sum_of(s.cluster_fill, rank) + sum_of(s.warp_c, warp);
   const int moves = sum_of(s.cluster_hole, ranks);
 
-  // Rounds of up to `list` moves per CTA: move m is CTA m % ranks's.
+  // Rounds of up to `list` moves per CTA: move m is CTA m % ranks's (a power of two).
+  const int log_ranks = __ffs(ranks) - 1;
   uint8_t* kc = (uint8_t*)p.c.k + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
   uint8_t* vc = (uint8_t*)p.c.v + (layer * p.c.sl + b * p.c.sb + kvh * p.c.sh) * esize;
   const int64_t row_bytes = p.c.st * esize;
@@ -332,7 +352,7 @@ __global__ __launch_bounds__(kEvictThreads, 4) void cache_evict_kernel(const __g
       const bool hole = hm >> lane & 1;
       const int m = hole ? h + __popc(hm & lt) : f + __popc(fm & lt);
       if (((hm | fm) >> lane & 1) && m >= from && m < upto) {
-        const unsigned at = (unsigned)(m - from) / (unsigned)ranks, to = (unsigned)(m - from) % (unsigned)ranks;
+        const unsigned at = (unsigned)(m - from) >> log_ranks, to = (unsigned)(m - from) & (ranks - 1);
         int* slot = (hole ? list_to : list_from) + at;
         if (ranks > 1) st_cluster_u32(slot, to, (uint32_t)(t + lane));
         else *slot = t + lane;
@@ -369,13 +389,6 @@ __global__ __launch_bounds__(kEvictThreads, 4) void cache_evict_kernel(const __g
     }
     if (from + list * ranks < moves) meet();  // the lists are used again
   }
-  // Weights and positions that stay in their slots.
-  if (apart)
-    for (int t = w_lo + lane; t < min(w_hi, p.budget); t += 32)
-      if (words[(t - w_lo) / 32] >> ((t - w_lo) & 31) & 1) {
-        mass_out[t] = mass[t];
-        pos_out[t] = pos[t];
-      }
   if (ranks > 1) cluster_sync();  // no CTA leaves while another may still write its lists
 }
 
