@@ -93,6 +93,8 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   unsigned long long* seen = seen_all + warp * kOpMaxNodes;
   const int batch = p.c.batch, blocks = p.row_blocks, items = p.c.kv_heads * blocks, nodes = p.nodes;
   const int heads_per = p.heads / p.c.kv_heads, rows = heads_per * nodes;
+  // The grid is resident at once: the join may take its places beside it.
+  pdl_launch_dependents();
   build_schedule<false>(p.c, batch, items, nodes, lens, first);
 
   // This CTA's run of tiles.
@@ -100,10 +102,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   int w0, w1, parts;
   if (p.stream) {
     parts = active(p.grid, total);
-    if ((int)blockIdx.x >= parts) {
-      pdl_launch_dependents();
-      return;
-    }
+    if ((int)blockIdx.x >= parts) return;
     w0 = share(blockIdx.x, parts, total);
     w1 = share(blockIdx.x + 1, parts, total);
   } else {
@@ -473,7 +472,6 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
       }
     }
   }
-  pdl_launch_dependents();
 }
 
 // ---- collected weight ------------------------------------------------------------
@@ -525,8 +523,13 @@ __device__ int path_nodes(const int32_t* path, int path_len, int nodes, int room
   return min(n, room);
 }
 
+// CTAs per SM, by shared memory (67 KB for bf16 rows of 128: three).
+template <typename T, int D>
+constexpr int mass_ctas() {
+  return sizeof(T) * D == 128 ? 4 : sizeof(T) * D == 256 ? 3 : 1;
+}
 template <typename T, int D, bool BIAS>
-__global__ __launch_bounds__(kThreads) void cache_mass_kernel(const __grid_constant__ MassParams p) {
+__global__ __launch_bounds__(kThreads, mass_ctas<T, D>()) void cache_mass_kernel(const __grid_constant__ MassParams p) {
   using R = Rows<T, D>;
   using S = MassSmem<T, D>;
   // As in the attention: powers of two where the last bits do not matter.
@@ -721,7 +724,7 @@ cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D, false>, p, 16 * WM);
+  return cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D, false>, p, 16 * WM, join_by_item(p));
 }
 
 template <typename T, int D, bool BIAS>
@@ -793,7 +796,7 @@ cudaError_t mass_run(MassParams& p, cudaStream_t s) {
   int dev = 0;
   e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  const int per_sm = max(1, min(4, kSmSmem / (bytes + 1024)));
+  const int per_sm = max(1, min(mass_ctas<T, D>(), kSmSmem / (bytes + 1024)));
   const long long most = (long long)p.c.batch * p.c.layers * p.c.kv_heads * ((p.c.capacity + p.path_len + kTile - 1) / kTile);
   p.grid = (int)min((long long)op_sm_count(dev) * per_sm, max(1ll, most / 2));
   K<<<p.grid, kThreads, bytes, s>>>(p);

@@ -127,6 +127,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   const int batch = p.c.batch, blocks = p.row_blocks, items = p.c.kv_heads * blocks, nodes = p.nodes;
   const int heads_per = p.heads / p.c.kv_heads, rows = heads_per * nodes;
 
+  pdl_launch_dependents();  // the grid is resident at once: the join may take its places beside it
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmem)
                  : "memory");
@@ -524,7 +525,6 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       cur.next(lens, batch, p.c.kv_heads, blocks, nodes);
     }
   }
-  pdl_launch_dependents();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -575,7 +575,7 @@ cudaError_t tc_run(const TreeParams& p, cudaStream_t s) {
   cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tree_join_kernel<bf16, D, true>, p, kRows);
+  return cudaLaunchKernelEx(&cfg, tree_join_kernel<bf16, D, true>, p, kRows, join_by_item(p));
 }
 
 }  // namespace

@@ -160,50 +160,61 @@ __device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpre
 // Joins the partial rows of items that several CTAs worked on. A CTA's two
 // partial blocks of mb rows hold [head_dim / 4][row][4] sums, then the rows'
 // maxima (natural units) and sums of weights. A thread per row and four columns.
+// blockIdx.x is an item, or where there are more items than CTAs, a CTA whose run
+// may begin inside one (the first such run of an item joins it).
+inline bool join_by_item(const TreeParams& p) { return p.c.batch * p.c.kv_heads * p.row_blocks <= p.grid; }
 inline dim3 join_grid(const TreeParams& p, int mb, int d) {
-  return dim3(p.c.batch * p.c.kv_heads * p.row_blocks, (mb * d / 4 + kThreads - 1) / kThreads);
+  return dim3(join_by_item(p) ? p.c.batch * p.c.kv_heads * p.row_blocks : p.grid, (mb * d / 4 + kThreads - 1) / kThreads);
 }
 template <typename T, int D, bool APART>
-__global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_constant__ TreeParams p, int mb) {
+__global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_constant__ TreeParams p, int mb, bool by_item) {
   extern __shared__ __align__(16) int sched[];
   int *lens = sched, *first = sched + p.c.batch;
   const int items = p.c.kv_heads * p.row_blocks, nodes = p.nodes;
   build_schedule<APART>(p.c, p.c.batch, items, nodes, lens, first);
-  const int b = blockIdx.x / items, item = blockIdx.x % items, total = first[p.c.batch];
-  const int parts = active(p.grid, total), tiles = tiles_of<APART>(lens[b], nodes), w = first[b] + item * tiles;
-  const int c0 = owner(w, parts, total), c1 = owner(w + tiles - 1, parts, total);
+  const int total = first[p.c.batch], parts = active(p.grid, total), mine = blockIdx.x;
+  Cursor<APART> cur;
+  if (by_item) {
+    const int b = mine / items;
+    cur.seek(first[b] + (mine - b * items) * tiles_of<APART>(lens[b], nodes), lens, first, p.c.batch, p.row_blocks, nodes);
+  } else {
+    cur.seek(share(min(mine, parts - 1), parts, total), lens, first, p.c.batch, p.row_blocks, nodes);
+  }
+  const int b = cur.b, w = cur.w - cur.tile;
+  const int c0 = owner(w, parts, total), c1 = owner(w + cur.tiles - 1, parts, total);
   pdl_wait();
-  if (c0 == c1) return;
-  const int at = blockIdx.y * kThreads + threadIdx.x, r = at % mb, quad = at / mb;
-  const int heads_per = p.heads / p.c.kv_heads, row = (item % p.row_blocks) * mb + r;
-  if (quad >= D / 4 || row >= heads_per * nodes) return;
+  if (by_item ? c0 == c1 : mine >= parts || cur.tile == 0 || c0 + 1 != mine) return;
+  const int heads_per = p.heads / p.c.kv_heads;
   // The first CTA began with the item (its block 1), the others went on with it.
   auto part = [&](int c) { return p.ws + (int64_t)(c * 2 + (c == c0)) * mb * (D + 2); };
-  float m = -INFINITY;
+  const int at = blockIdx.y * kThreads + threadIdx.x, r = at % mb, quad = at / mb, row = cur.inner * mb + r;
+  if (quad < D / 4 && row < heads_per * nodes) {
+    float m = -INFINITY;
 #pragma unroll 4
-  for (int c = c0; c <= c1; ++c) m = fmaxf(m, part(c)[mb * D + r]);
-  const float u = m == -INFINITY ? 0.f : m;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+    for (int c = c0; c <= c1; ++c) m = fmaxf(m, part(c)[mb * D + r]);
+    const float u = m == -INFINITY ? 0.f : m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
 #pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const float* src = part(c);
-    const float f = ex2((src[mb * D + r] - u) * kLog2e), l = src[mb * D + mb + r];
-    const float4 v = *reinterpret_cast<const float4*>(src + (quad * mb + r) * 4);
-    if (f == 0.f) continue;  // an empty part's sums may be anything
-    sum += l * f;
-    acc.x += v.x * f;
-    acc.y += v.y * f;
-    acc.z += v.z * f;
-    acc.w += v.w * f;
+    for (int c = c0; c <= c1; ++c) {
+      const float* src = part(c);
+      const float f = ex2((src[mb * D + r] - u) * kLog2e), l = src[mb * D + mb + r];
+      const float4 v = *reinterpret_cast<const float4*>(src + (quad * mb + r) * 4);
+      if (f == 0.f) continue;  // an empty part's sums may be anything
+      sum += l * f;
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+    }
+    const int hd = row / nodes, n = row - hd * nodes, head = cur.outer * heads_per + hd;
+    T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + n * p.out.sn + quad * 4;
+    const bool empty = sum == 0.f;
+    const float inv = empty ? 0.f : 1.f / sum;
+    store2(dst, empty ? 0.f : acc.x * inv, empty ? 0.f : acc.y * inv);
+    store2(dst + 2, empty ? 0.f : acc.z * inv, empty ? 0.f : acc.w * inv);
+    if (p.lse && quad == 0) p.lse[((int64_t)b * p.heads + head) * nodes + n] = empty ? -INFINITY : m + logf(sum);
   }
-  const int hd = row / nodes, n = row - hd * nodes, head = (item / p.row_blocks) * heads_per + hd;
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(p.out.ptr)) + b * p.out.sb + head * p.out.sh + n * p.out.sn + quad * 4;
-  const bool empty = sum == 0.f;
-  const float inv = empty ? 0.f : 1.f / sum;
-  store2(dst, empty ? 0.f : acc.x * inv, empty ? 0.f : acc.y * inv);
-  store2(dst + 2, empty ? 0.f : acc.z * inv, empty ? 0.f : acc.w * inv);
-  if (p.lse && quad == 0) p.lse[((int64_t)b * p.heads + head) * nodes + n] = empty ? -INFINITY : m + logf(sum);
 }
 
 }  // namespace mrtdf
