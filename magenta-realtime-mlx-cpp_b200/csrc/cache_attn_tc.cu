@@ -286,11 +286,6 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       for (int e = 0; e < 4; ++e)
         qv[e] = takes && row < here ? *reinterpret_cast<const uint4*>(q + 8 * e) : make_uint4(0, 0, 0, 0);
       const int next = p.c.next_pos ? p.c.next_pos[b] : len;
-      if (masks_of != b) {
-        masks_of = b;
-        if (warp == 0) node_masks(seen, p.parents ? p.parents + b * nodes : nullptr, nodes, cur.len >= 0, lane);
-      }
-      if (tid == 0) poison = 0;
       if (takes) {
         uint32_t w[16];
 #pragma unroll
@@ -305,7 +300,13 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       tmem_wait_st();
       tc_fence_before();
       arrive(q_full);
-      soft_sync();  // the masks
+      // The masks, while the first scores are made.
+      if (masks_of != b) {
+        masks_of = b;
+        if (warp == 0) node_masks(seen, p.parents ? p.parents + b * nodes : nullptr, nodes, cur.len >= 0, lane);
+      }
+      if (tid == 0) poison = 0;
+      soft_sync();
       const unsigned long long see = row < here ? seen[nd] : 0ull;
       const int at = (int)((unsigned)next + (unsigned)(see ? __popcll(see) - 1 : 0));
       const float* tab = BIAS ? p.rel_bias + (row < here ? (int64_t)head * p.rel_len : 0) : nullptr;

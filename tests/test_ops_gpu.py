@@ -825,3 +825,91 @@ def test_stream_cache_is_the_streams_own(ops, mrtdf, tiny_weights, dtype):
         ops.stream_cache(st, 3)
     st.close()
     eng.close()
+
+
+# ---- the tcgen05 form of tree attention (bf16, more than 16 rows, long caches) ----------
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,KV,N,cap", [(2, 2, 17, 300), (4, 1, 32, 520), (4, 2, 64, 1000), (8, 1, 64, 700), (3, 1, 43, 2100), (16, 1, 64, 400)])
+def test_tree_many_rows(ops, D, H, KV, N, cap):
+    """17 to 1024 rows per kv head: one block of 128 rows and several, ragged."""
+    rng = np.random.default_rng(N + cap)
+    lens = [cap, 0, 1, 64 * (cap // 64), cap - 1, -3]
+    parents = ints([tree_of(rng, N, N // 4 if b == 4 else 0) for b in range(6)])
+    check_tree(ops, tree_inputs(N, BF, 6, H, KV, N, D, cap), ints(lens), parents)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rel_len,stored", [(64, False), (64, True), (2000, True), (1, False)])
+def test_tree_many_rows_with_bias(ops, D, rel_len, stored):
+    B, H, KV, N, cap = 3, 8, 2, 12, 900
+    rng = np.random.default_rng(rel_len)
+    kw = dict(rel_bias=normal(9, H, rel_len))
+    if stored:
+        pos = torch.stack([torch.from_numpy(rng.permutation(3 * cap)[:cap]) for _ in range(B * KV)])
+        kw |= dict(pos=pos.view(B, KV, cap).to(torch.int32).to(DEV), next_pos=ints([3 * cap, 3 * cap + 5, 4 * cap]))
+    parents = ints([tree_of(rng, N, 2) for _ in range(B)])
+    check_tree(ops, tree_inputs(cap, BF, B, H, KV, N, D, cap), ints([cap, 7, 450]), parents, **kw)
+
+
+def test_tree_many_rows_values_that_are_not_seen(ops):
+    """NaN and infinities behind the length, in absent nodes and in a branch that
+    other branches do not see; an infinity that a row does see stays one."""
+    B, H, KV, N, cap = 2, 8, 2, 6, 700
+    q, kn, vn, k, v = tree_inputs(5, BF, B, H, KV, N, 64, cap)
+    lens = ints([cap - 30, 0])
+    for b in range(B):
+        k[b, :, int(lens[b]):], v[b, :, int(lens[b]):] = math.nan, math.inf
+    parents = ints([[-1, 0, -1, 2, -2, 4]] * B)
+    kn[:, :, 4:], vn[:, :, 4:], q[:, :, 4:] = math.nan, -math.inf, math.nan
+    vn[:, :, 3, 5], vn[:, :, 3, 6] = math.inf, math.nan
+    out, lse = ops.tree_attention(q, kn, vn, k, v, lens, parents)
+    zero = [t.clone() for t in (q, kn, vn, k, v)]
+    for t in zero:
+        t[~torch.isfinite(t)] = 0
+    wo, wl, to, tl = attend(*zero, lens, parents)
+    near(lse, wl, tl)
+    assert bool((out[:, :, 3, 5] == math.inf).all()) and bool(torch.isnan(out[:, :, 3, 6]).all())
+    out[:, :, 3, 5:7] = wo[:, :, 3, 5:7].to(out)
+    near(out, wo, to)
+
+
+@pytest.mark.parametrize("scale", [0.125, -0.25, 0.0])
+def test_tree_many_rows_scales_and_large_scores(ops, scale):
+    """Scores that rise along the cache (the maximum is raised often), a negative
+    and a zero scale."""
+    x = list(tree_inputs(8, BF, 1, 8, 2, 9, 128, 1500, std=0.5))
+    x[3] *= torch.linspace(0.1, 12, 1500, device=DEV)[None, None, :, None].to(BF)
+    check_tree(ops, x, ints([1500]), None, scale=scale)
+
+
+def test_tree_many_rows_strided_and_expanded(ops):
+    """A cache with the heads inside the rows, and one shared by two sequences
+    through an expanded view (no tensor map takes that: the other kernel)."""
+    B, H, KV, N, D, cap = 2, 8, 2, 9, 64, 800
+    rows = normal(1, B, N, (H + 2 * KV) * D, dtype=BF, std=0.3).view(B, N, H + 2 * KV, D).transpose(1, 2)
+    both = normal(2, B, cap, 2, KV, D, dtype=BF)
+    k, v = both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)
+    a = check_tree(ops, (rows[:, :H], rows[:, H:H + KV], rows[:, H + KV:], k, v), ints([cap, 77]), None)
+    one = (rows[:, :H], rows[:, H:H + KV], rows[:, H + KV:], k[:1].expand(B, -1, -1, -1), v[:1].expand(B, -1, -1, -1))
+    b = check_tree(ops, one, ints([cap, 77]), None)
+    assert torch.equal(a[1].isfinite(), b[1].isfinite())
+
+
+def test_tree_many_rows_same_every_time_and_captured(ops):
+    x = tree_inputs(9, BF, 3, 16, 2, 12, 128, 1500)
+    lens = ints([1500, 3, 800])
+    first = ops.tree_attention(*x, lens)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            r = ops.tree_attention(*x, lens)
+        graphs.append((g, r, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, _, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, r, _ in graphs:
+        assert torch.equal(first[0], r[0]) and torch.equal(first[1], r[1])
