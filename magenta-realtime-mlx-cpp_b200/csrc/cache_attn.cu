@@ -132,6 +132,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   const uint32_t x0 = (uint32_t)((ch ^ (r0 & 7)) << 4);
   const int64_t row_step = (int64_t)RS * p.c.st;
   Cursor<false> ahead;
+  ahead.seek(w0, lens, first, batch, blocks, nodes);
   const T *kb = nullptr, *vb = nullptr;  // this lane's chunk of row 0 of ahead's item
   auto enter = [&] {
     const int64_t at = ahead.b * p.c.sb + ahead.outer * p.c.sh + ch * (16 / (int)sizeof(T));
@@ -171,7 +172,6 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
     if (ahead.next(lens, batch, p.c.kv_heads, blocks, nodes)) enter();
   };
 
-  ahead.seek(w0, lens, first, batch, blocks, nodes);
   Cursor<false> cur = ahead;
   enter();
 #pragma unroll
@@ -756,14 +756,31 @@ int tree_smem(const TreeParams& p, int wm) {
 }
 
 constexpr int kSmSmem = 227 * 1024;
-// Rows and capacity above which the tcgen05 kernel takes bf16 calls.
-constexpr int kTcRows = 16, kTcCapacity = 256;
+// Which bf16 calls the tcgen05 kernel takes. us, mma.sync / tcgen05, 16
+// sequences of 4 kv heads without a bias (which costs the first 1.2 to 1.8
+// times as much, the second 1.1 times):
+//                    32 rows      64 rows      128 rows     256 rows
+//   64 x   300     13.2/ 16.4   16.7/ 17.5    19.7/ 20.8   31.1/ 24.3
+//   64 x  1024     17.5/ 19.7   23.1/ 21.2    28.6/ 24.6   42.8/ 32.4
+//   64 x  4096     27.2/ 33.8   39.9/ 37.9    60.5/ 41.3    106/ 65
+//   64 x 16384     63.9/ 88.1    104/ 103      188/ 106     356/ 194
+//  128 x   300     16.7/ 22.6   21.3/ 23.7    26.3/ 27.1   46.6/ 34.5
+//  128 x  1024     22.0/ 26.8   30.2/ 28.2    44.0/ 31.7   75.0/ 43.9
+//  128 x  4096     47.3/ 47.9   67.8/ 51.8     116/ 56      217/ 85
+//  128 x 16384      139/ 112     207/ 125      396/ 131     773/ 239
+// (256 kv heads alike; head_dim 64 and 64 rows even out there.)
+bool tree_uses_tc(const TreeParams& p, int rows) {
+  const int cap = p.c.capacity;
+  if (rows > 64) return cap > 512;
+  if (rows > 32) return cap > (p.c.head_dim == 128 ? 768 : 2048);
+  return rows > 16 && p.c.head_dim == 128 && cap > 4096;
+}
 
 }  // namespace
 
 cudaError_t plan_tree_attention(TreeParams& p, int sms, size_t* ws_floats) {
   const int wm = tree_wm(p), mb = 16 * wm, rows = p.heads / p.c.kv_heads * p.nodes;
-  p.tc = rows > kTcRows && p.c.capacity > kTcCapacity && tree_attention_tc_takes(p);
+  p.tc = tree_uses_tc(p, rows) && tree_attention_tc_takes(p);
   if (p.tc) {
     plan_tree_attention_tc(p, sms, ws_floats);
     return cudaSuccess;

@@ -20,7 +20,7 @@
 //              queries are zero, their scores stay zero bits);
 //   warp 16    TMA producer: K and V tiles through a ring, 128-byte swizzle,
 //              over the items of the run without a stop;
-//   warp 17    MMA issuer: S = Q K^T into one of three TMEM buffers, three
+//   warp 17    MMA issuer: S = Q K^T into one of three TMEM buffers, two
 //              tiles ahead, then O_g += P V for the tile's group g, weights as two bf16 parts (16 bits of a
 //              weight; the second product is hidden too).
 //              V is an MN-major operand of 64-column parts kSub bytes apart.
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 32) {
-    mbar_init(q_full, kSoft);
+    mbar_init(q_full, kSoft / 32);
     mbar_init(o_done, 1);
     mbar_init(drain, 1);
     for (int i = 0; i < NS; ++i) {
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, kSoft / 2);  // one group
+      mbar_init(p_full + i, kSoft / 64);  // the warps of one group
       mbar_init(p_empty + i, 1);
     }
     fence_mbar_init();
@@ -224,10 +224,14 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     for (int seg = 0; ok && w < end; ++seg) {
       const int n = all(min(cur.tiles - cur.tile, w1 - cur.w));  // tiles of the item's run
       if (!(ok = wait_all(q_full, (uint32_t)(seg & 1)))) break;
-      for (int t = 0; ok && t < min(n, kBufs); ++t) ok = issue_s(i + t);
+      for (int t = 0; ok && t < min(n, 2); ++t) ok = issue_s(i + t);
       for (int t = 0; ok && t < n; ++t, ++i) {
         const int st = i % NS, pb = i % kBufs, og = i & 1;
         if (!(ok = wait_all(p_full + pb, (uint32_t)((i / kBufs) & 1)))) break;
+        // The next scores of the group that made these weights come first: it
+        // has nothing else to do. Their buffer was the tile's before, whose
+        // products are long done.
+        if (t + 2 < n && !(ok = issue_s(i + 2))) break;
         tc_fence_after();
         const uint32_t lo = v_lo + (uint32_t)((st * 2 + 1) * C::kKvBytes / 16), d = tm + kColO + (uint32_t)(og * D);
         const uint32_t a = tm + (uint32_t)(pb * 64);
@@ -241,7 +245,6 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
           mma_commit(kv_empty + st);
         }
         __syncwarp();
-        if (t + kBufs < n) ok = issue_s(i + kBufs);  // once these products have retired
       }
       if (ok && elected()) mma_commit(o_done);
       __syncwarp();
@@ -268,6 +271,12 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
     auto weight = [](float x) { return ex2(POW2 ? x : x * kLog2e); };
     // The two threads of each row of this warp's quarter.
     auto row_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(2 + group * 4 + (warp & 3)) : "memory"); };
+    // One arrival per warp: 256 of them one after the other took longer than the
+    // weights.
+    auto warp_arrive = [&](uint64_t* b) {
+      __syncwarp();
+      if (lane == 0) arrive(b);
+    };
     auto soft_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory"); };
     bool ok = true;
     int i = 0, masks_of = -1;
@@ -299,7 +308,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       }
       tmem_wait_st();
       tc_fence_before();
-      arrive(q_full);
+      warp_arrive(q_full);
       // The masks, while the first scores are made.
       if (masks_of != b) {
         masks_of = b;
@@ -452,7 +461,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         tc_fence_before();
-        arrive(p_full + buf);
+        warp_arrive(p_full + buf);
       }
       i += n;
       if (ok) ok = wait(o_done, (uint32_t)(seg & 1));
