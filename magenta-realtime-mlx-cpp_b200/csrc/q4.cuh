@@ -34,6 +34,8 @@ struct Q4PackParams {
 // With ws_bytes: only the size of the workspace that the call needs, on a GPU of
 // `sms` multiprocessors.
 cudaError_t launch_q4_linear(const Q4Params& p, int dtype, int out_dtype, int sms, size_t* ws_bytes, cudaStream_t s);
+// The part for wide x (q4_wide.cu).
+cudaError_t launch_q4_wide(const Q4Params& p, int dtype, int out_dtype, int sms, size_t* ws_bytes, cudaStream_t s);
 cudaError_t launch_q4_quantize(const Q4PackParams& p, int dtype, cudaStream_t s);
 
 }  // namespace mrtdf

@@ -1,0 +1,179 @@
+// Products with 4-bit weights: what the two kernels share (q4.cu, q4_wide.cu).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "cache_ops.cuh"
+#include "cache_tile.cuh"
+#include "q4.cuh"
+
+namespace mrtdf {
+namespace {
+
+constexpr int kStep = 128;  // columns multiplied at a time: 64 bytes of 16 rows
+
+// Byte offset of 16-byte chunk `ch` (0 .. 3) of row `row` of a step. Rows are
+// 64 bytes apart; the swizzle puts the eight rows of one access in different
+// banks.
+__device__ __forceinline__ uint32_t w_at(int row, int ch) {
+  return (uint32_t)(row * (kStep / 2) + ((ch ^ (row >> 1 & 3)) << 4));
+}
+
+// Words of a step that lane c multiplies for its group `gi`, from row address
+// `row` (of a step, without the chunk) whose swizzle is x: WL = G / 32 words,
+// columns gi * G + (c * WL + i) * 8.
+template <int WL>
+__device__ __forceinline__ void load_words(uint32_t* w, uint32_t row, uint32_t x, int c, int gi) {
+  if constexpr (WL == 1) {
+    w[0] = lds32(row + ((gi << 4) ^ x) + 4 * c);
+  } else if constexpr (WL == 2) {
+    const uint32_t a = row + (((2 * gi + (c >> 1)) << 4) ^ x) + 8 * (c & 1);
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+  } else {
+    const uint32_t a = row + ((c << 4) ^ x);
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(a));
+  }
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+
+// The column pairs (0, 4), (1, 5) of w, or with w >> 8 (2, 6), (3, 7): q - 8
+// (EIGHT), or 1024 + q and 1024 + 16 q.
+template <bool EIGHT>
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t& even, uint32_t& odd) {
+  // (w & mask) | magic in one instruction each
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(even) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(odd) : "r"(w), "n"(0x00f000f0), "r"(0x64006400u));
+  if (EIGHT) {
+    const __half2 e = __hadd2(*reinterpret_cast<const __half2*>(&even), __float2half2_rn(-1032.f));
+    const __half2 o = __hfma2(*reinterpret_cast<const __half2*>(&odd), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+    even = *reinterpret_cast<const uint32_t*>(&e);
+    odd = *reinterpret_cast<const uint32_t*>(&o);
+  }
+}
+
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c = a b: the first product of a sum, on zeros that take no registers.
+__device__ __forceinline__ void mma_f16_first(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A scale and its bias, side by side in shared memory.
+template <typename T>
+struct alignas(2 * sizeof(T)) ScalePair {
+  T s, b;
+};
+__device__ __forceinline__ void load_pair(uint32_t at, float& s, float& b, __nv_bfloat16) {
+  const uint32_t w = lds32(at);
+  s = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void load_pair(uint32_t at, float& s, float& b, float) {
+  uint32_t x, y;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(at));
+  s = __uint_as_float(x);
+  b = __uint_as_float(y);
+}
+
+template <typename T>
+struct Parts;  // fp16 columns per row of x
+template <>
+struct Parts<__nv_bfloat16> {
+  static constexpr int N = 1;
+};
+template <>
+struct Parts<float> {
+  static constexpr int N = 2;
+};
+// x to fp16: 8 columns from kk on (one word of weights) per lane, a group by
+// 4 WL neighbouring lanes, all lanes of a warp together. put(h, words) gets the
+// lane's eight values of part h, sums(h, {factor, addend, X, 0}) the group's.
+// Rows that do not exist (m < 0) and columns past k are zero.
+template <typename T, int G, bool EIGHT, typename Put, typename Sums>
+__device__ __forceinline__ void bring_x(const Q4Params& p, int m, int kk, Put&& put, Sums&& sums) {
+  constexpr int WL = G / 32, P = Parts<T>::N, V = 8 * (int)sizeof(T) / 16;
+  float v[8], big = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  if (m >= 0 && kk < p.k) {
+    const T* src = reinterpret_cast<const T*>(p.x) + m * p.x_stride + kk;
+#pragma unroll
+    for (int e = 0; e < V; ++e) Vec16<T>::unpack(*reinterpret_cast<const uint4*>(src + e * (8 / V)), v + e * (8 / V));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(v[e]));
+#pragma unroll
+  for (int o = 1; o < 4 * WL; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  const uint32_t ex = max(__float_as_uint(big) >> 23, 15u);
+  const float up = __uint_as_float((268u - ex) << 23), down = __uint_as_float((ex - 14u) << 23);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= up;
+#pragma unroll
+  for (int h = 0; h < P; ++h) {
+    uint32_t w[4];
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = pack_f16(v[e], v[e + 4]);
+      const float2 t2 = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      f[e] = t2.x;
+      f[e + 4] = t2.y;
+    }
+    float even = (f[0] + f[4]) + (f[2] + f[6]), odd = (f[1] + f[5]) + (f[3] + f[7]);
+#pragma unroll
+    for (int o = 1; o < 4 * WL; o <<= 1) {
+      even += __shfl_xor_sync(0xffffffffu, even, o);
+      odd += __shfl_xor_sync(0xffffffffu, odd, o);
+    }
+    if (!EIGHT) {
+      w[1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
+      w[3] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
+    }
+    put(h, make_uint4(w[0], w[1], w[2], w[3]));
+    const float sum = down * (even + odd);
+    sums(h, make_float4(down, EIGHT ? 8.f * sum : -down * (1024.f * even + 64.f * odd), sum, 0.f));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] -= f[e];
+  }
+}
+
+// A group's products, scaled, onto y: rows g and g + 8 of the weights and
+// columns 2 c, 2 c + 1 with the factors u and v. The two are two rows of x
+// (y[0], y[1] of row g, y[2], y[3] of row g + 8), or the parts of one (y[0] and
+// y[1]), which are added before a scale meets them.
+template <int P>
+__device__ __forceinline__ void add_group(float* y, const float* acc, uint4 u, uint4 v, float s0, float b0, float s1, float b1) {
+  const float fu = __uint_as_float(u.x), ou = __uint_as_float(u.y), xu = __uint_as_float(u.z);
+  const float fv = __uint_as_float(v.x), ov = __uint_as_float(v.y), xv = __uint_as_float(v.z);
+  if constexpr (P == 2) {
+    const float o = ou + ov, x = xu + xv;
+    y[0] = fmaf(s0, fmaf(fu, acc[0], fmaf(fv, acc[1], o)), fmaf(b0, x, y[0]));
+    y[1] = fmaf(s1, fmaf(fu, acc[2], fmaf(fv, acc[3], o)), fmaf(b1, x, y[1]));
+  } else {
+    y[0] = fmaf(s0, fmaf(fu, acc[0], ou), fmaf(b0, xu, y[0]));
+    y[1] = fmaf(s0, fmaf(fv, acc[1], ov), fmaf(b0, xv, y[1]));
+    y[2] = fmaf(s1, fmaf(fu, acc[2], ou), fmaf(b1, xu, y[2]));
+    y[3] = fmaf(s1, fmaf(fv, acc[3], ov), fmaf(b1, xv, y[3]));
+  }
+}
+
+}  // namespace
+}  // namespace mrtdf

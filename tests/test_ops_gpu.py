@@ -693,6 +693,42 @@ def test_q4_sizes(ops, dtype, n, k, group, m):
     check_q4(ops, *q4_case(n, dtype, m, n, k, group))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,n,k,group", [(30, 3324, 5504, 64), (64, 300, 2080, 32), (17, 20000, 256, 128), (9, 130, 131072, 128),
+                                         (40, 18944, 512, 64), (3, 16500, 8192, 32), (1, 7, 65536, 64)])
+def test_q4_streams_weights(ops, dtype, m, n, k, group):
+    """Row blocks that two or more CTAs share, several passes over x, groups
+    that no wide load fits."""
+    check_q4(ops, *q4_case(m, dtype, m, n, k, group))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k", [(1, 1024), (2, 4096), (20, 1024)])
+def test_q4_scales_at_odd_addresses(ops, dtype, m, k):
+    x, packed, scales, biases = q4_case(m, dtype, m, 70, k, 64)
+    want = check_q4(ops, x, packed, scales, biases)
+
+    def moved(t):
+        return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+    for s, b in ((moved(scales), biases), (scales, moved(biases)), (moved(scales), moved(biases))):
+        assert (s.data_ptr() | b.data_ptr()) % 16
+        assert torch.equal(check_q4(ops, x, packed, s, b), want)
+
+
+@pytest.mark.parametrize("m", [2, 33])
+def test_q4_infinite_scales_stay_in_their_rows(ops, m):
+    """k is not a multiple of the kernels' steps: what stands for the columns
+    past it must not meet the last group's scale."""
+    x, packed, scales, biases = q4_case(m, F32, m, 40, 160, 32)
+    x, packed = x.abs() + 0.1, packed | 0x11  # no zero times infinity in the formula
+    scales[3, -1] = float("inf")
+    y, fine = ops.q4_linear(x, packed, scales, biases), ops.q4_linear(x, packed, scales.clamp(max=1.0), biases)
+    assert bool((y[:, 3] == float("inf")).all())
+    keep = torch.arange(40, device=DEV) != 3
+    assert torch.equal(y[:, keep], fine[:, keep])
+
+
 def test_q4_out_types_views_and_streams(ops):
     x, packed, scales, biases = q4_case(5, BF, 6, 100, 256, 64)
     a = check_q4(ops, x, packed, scales, biases, out_dtype=F32)
