@@ -46,11 +46,22 @@ __device__ __forceinline__ float2 val2(uint32_t vals, int row, int n, int c, flo
   return make_float2(__uint_as_float(lds32(at)), __uint_as_float(lds32(at + 4)));
 }
 
+// Rows of 512 bytes (float32, 128): a tile's keys and values take 64 KB, three
+// stages leave room for one CTA, whose four warps issue 1.1 instructions a
+// clock. So the ring holds three halves there, the keys of a tile or its values,
+// and the groups' sums are joined one after another: two CTAs fit (21 sequences
+// x 4 heads x 1334 keys: 67 us with one, 51 with two).
+template <typename T, int D>
+constexpr bool halves() {
+  return sizeof(T) * D == 512;
+}
+
 // Shared memory of the attention kernel.
 template <typename T, int D, int WM>
 struct TreeSmem {
-  static constexpr int kStageBytes = 2 * kTile * Rows<T, D>::kBytes;
-  static constexpr int kMergeBytes = WM == 1 ? 2 * 16 * D * 4 : WM == 2 ? 32 * D * 4 : 0;
+  static constexpr bool HALVES = halves<T, D>();
+  static constexpr int kStageBytes = (HALVES ? 1 : 2) * kTile * Rows<T, D>::kBytes;
+  static constexpr int kMergeBytes = WM == 4 ? 0 : (HALVES ? 1 : 2) * 16 * D * 4;
   static constexpr int kScoreBytes = 16 * kTile * WM * 4;  // four warps x 16 rows x 16 WM keys
   static constexpr int kScratch = kMergeBytes > kScoreBytes ? kMergeBytes : kScoreBytes;
   static constexpr int kRing = kStages * kStageBytes;
@@ -66,7 +77,7 @@ struct TreeSmem {
 // positions take the registers of the fourth).
 template <typename T, int D, bool BIAS>
 constexpr int tree_ctas() {
-  return sizeof(T) * D == 128 ? (BIAS ? 3 : 4) : sizeof(T) * D == 256 ? 2 : 1;
+  return sizeof(T) * D == 128 ? (BIAS ? 3 : 4) : 2;
 }
 template <typename T, int D, int WM, bool BIAS, bool HALF>
 __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_kernel(const __grid_constant__ TreeParams p) {
@@ -118,7 +129,8 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
     w1 = start(i1);
   }
 
-  const uint32_t ring = smem_u32(smem) + group * (2 * KT * R::kBytes);
+  constexpr bool HALVES = S::HALVES;
+  const uint32_t ring = smem_u32(smem) + group * ((HALVES ? 1 : 2) * KT * R::kBytes);
   const T* kc = reinterpret_cast<const T*>(p.c.k);
   const T* vc = reinterpret_cast<const T*>(p.c.v);
   const T* kn = reinterpret_cast<const T*>(p.k_new.ptr);
@@ -139,17 +151,19 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
     kb = kc + at;
     vb = vc + at;
   };
-  auto fetch = [&](int st) {
+  // The tile's keys (with their positions, in place `ps_at`) to kd, its values to vd.
+  auto copy = [&](uint32_t kd, uint32_t vd, int ps_at, bool keys, bool vals) {
     const int len = max(ahead.len, 0), key0 = ahead.tile * kTile + group * KT;
-    const uint32_t kd = ring + st * S::kStageBytes + r0 * R::kBytes, vd = kd + KT * R::kBytes;
+    kd += r0 * R::kBytes;
+    vd += r0 * R::kBytes;
     if (key0 + KT <= len) {
       const int64_t at = (int64_t)(key0 + r0) * p.c.st;
       const T *ks = kb + at, *vs = vb + at;
 #pragma unroll
       for (int i = 0; i < COPIES; ++i) {
         const uint32_t to = i * RS * R::kBytes + (x0 ^ ((i * RS & 7) << 4));
-        cp_async16(kd + to, ks);
-        cp_async16(vd + to, vs);
+        if (keys) cp_async16(kd + to, ks);
+        if (vals) cp_async16(vd + to, vs);
         ks += row_step;
         vs += row_step;
       }
@@ -160,24 +174,39 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
         const T* ks = j < len ? kb + j * p.c.st : kn + ahead.b * p.k_new.sb + ahead.outer * p.k_new.sh + n * p.k_new.sn + el;
         const T* vs = j < len ? vb + j * p.c.st : vn + ahead.b * p.v_new.sb + ahead.outer * p.v_new.sh + n * p.v_new.sn + el;
         const uint32_t to = i * RS * R::kBytes + (x0 ^ ((i * RS & 7) << 4));
-        cp_async16_zfill(kd + to, ks, j < len + nodes);
-        cp_async16_zfill(vd + to, vs, j < len + nodes);
+        if (keys) cp_async16_zfill(kd + to, ks, j < len + nodes);
+        if (vals) cp_async16_zfill(vd + to, vs, j < len + nodes);
       }
     }
-    if (BIAS && p.c.pos && gt < KT) {
+    if (BIAS && p.c.pos && keys && gt < KT) {
       const int j = key0 + gt;
       const int32_t* ps = p.c.pos + (int64_t)(ahead.b * p.c.kv_heads + ahead.outer) * p.c.capacity;
-      cp_async4_zfill(smem_u32(pos_s + st * kTile + group * KT + gt), ps + min(j, max(len - 1, 0)), j < len);
+      cp_async4_zfill(smem_u32(pos_s + ps_at * kTile + group * KT + gt), ps + min(j, max(len - 1, 0)), j < len);
     }
-    if (ahead.next(lens, batch, p.c.kv_heads, blocks, nodes)) enter();
+    if (vals && ahead.next(lens, batch, p.c.kv_heads, blocks, nodes)) enter();
+  };
+  auto fetch = [&](int st) {
+    const uint32_t to = ring + st * S::kStageBytes;
+    copy(to, to + KT * R::kBytes, st, true, true);
   };
 
   Cursor<false> cur = ahead;
   enter();
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (ahead.w < w1) fetch(i);
+  // HALVES: slots of this tile's keys and values; the next tile's keys go where
+  // the values before these were, its values where these keys are.
+  int k_slot = 0, v_slot = 1, free_slot = 2, turn = 0;
+  auto slot = [&](int i) { return ring + i * S::kStageBytes; };
+  if (HALVES) {
+    copy(slot(k_slot), 0, 0, true, false);
     cp_async_commit();
+    copy(0, slot(v_slot), 0, false, true);
+    cp_async_commit();
+  } else {
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (ahead.w < w1) fetch(i);
+      cp_async_commit();
+    }
   }
 
   QFrag<T, D> q;
@@ -188,9 +217,15 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
   bool fresh = true;
 
   for (int st = 0, fill = kStages - 1; cur.w < w1; cur.next(lens, batch, p.c.kv_heads, blocks, nodes)) {
-    cp_async_wait<kStages - 2>();
-    group_sync<WM>(group);
-    if (ahead.w < w1) fetch(fill);
+    if (HALVES) {
+      cp_async_wait<1>();  // the keys; the values are still on their way
+      group_sync<WM>(group);
+      if (ahead.w < w1) copy(slot(free_slot), 0, turn ^ 1, true, false);
+    } else {
+      cp_async_wait<kStages - 2>();
+      group_sync<WM>(group);
+      if (ahead.w < w1) fetch(fill);
+    }
     cp_async_commit();
     const int len = max(cur.len, 0), kvh = cur.outer, row0 = cur.inner * MB + wm * 16;
 
@@ -231,13 +266,26 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
       for (int n = 0; n < ND; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     }
 
-    const uint32_t keys = ring + st * S::kStageBytes, vals = keys + KT * R::kBytes;
+    const uint32_t keys = HALVES ? slot(k_slot) : ring + st * S::kStageBytes, vals = HALVES ? slot(v_slot) : keys + KT * R::kBytes;
+    const int pos_at = (HALVES ? turn : st) * kTile + group * KT;
     const int key0 = cur.tile * kTile + group * KT;
-    if (key0 < len + nodes) {
-      float s[NT][4];
+    const bool any = key0 < len + nodes;  // for the whole group of warps
+    float s[NT][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-      qk_tile<D, NT>(s, q, keys, lane);
+    for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    if (any) qk_tile<D, NT>(s, q, keys, lane);
+    if (HALVES) {
+      group_sync<WM>(group);  // the keys are read: the next tile's values
+      if (ahead.w < w1) copy(0, slot(k_slot), 0, false, true);
+      cp_async_commit();
+      const int was = k_slot;
+      k_slot = free_slot;
+      free_slot = v_slot;
+      v_slot = was;
+      cp_async_wait<2>();
+      group_sync<WM>(group);
+    }
+    if (any) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -252,7 +300,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
           const unsigned long long s = key - len < nodes ? seen[key - len] : 0ull;
           return (int)((unsigned)next + (unsigned)(__popcll(s) - (s ? 1 : 0)));
         }
-        return p.c.pos ? pos_s[st * kTile + group * KT + k] : key;
+        return p.c.pos ? pos_s[pos_at + k] : key;
       };
       if (BIAS) {
         int ps[NT][2];
@@ -381,6 +429,7 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
     }
     st = st + 1 == kStages ? 0 : st + 1;
     fill = fill + 1 == kStages ? 0 : fill + 1;
+    turn ^= 1;
 
     if (cur.tile + 1 < cur.tiles && cur.w + 1 < w1) continue;
     // ---- the item's run ends here: join the key groups, write ----------------
@@ -393,36 +442,53 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
     if constexpr (WK > 1) {
       float4* buf = reinterpret_cast<float4*>(scratch);
       __syncthreads();  // nobody still reads scores or an earlier join there
+      // Half of the groups to the other half, or (HALVES) one after another,
+      // the columns in two parts where two warps share a group.
+      constexpr bool BY_ONE = HALVES && WM == 1;
+      constexpr int PARTS = HALVES && WM == 2 ? 2 : 1, NP = ND / PARTS;
 #pragma unroll
-      for (int half = WK / 2; half >= 1; half >>= 1) {
-        const int slot = ((group % half) * WM + wm) * 32 + lane;
-        if (group >= half && group < 2 * half) {
+      for (int step = BY_ONE ? WK - 1 : WK / 2; step >= 1; BY_ONE ? --step : step >>= 1) {
+        const bool gives = BY_ONE ? group == step : group >= step && group < 2 * step;
+        const bool takes = BY_ONE ? group == 0 : group < step;
+        const int at = BY_ONE ? 0 : (group % step) * WM + wm;
+        float a0 = 0, a1 = 0, b0 = 0, b1 = 0;
 #pragma unroll
-          for (int n = 0; n < ND; ++n)
-            buf[(((group % half) * WM + wm) * ND + n) * 32 + lane] = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
-          stat[slot] = make_float4(m0, m1, l0, l1);
-        }
-        __syncthreads();
-        if (group < half) {
-          const float4 t = stat[slot];
-          const float x0 = fmaxf(m0, t.x), x1 = fmaxf(m1, t.y);
-          const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
-          const float a0 = weight(m0 - u0), a1 = weight(m1 - u1);
-          const float b0 = weight(t.x - u0), b1 = weight(t.y - u1);
-          l0 = l0 * a0 + t.z * b0;
-          l1 = l1 * a1 + t.w * b1;
-          m0 = x0;
-          m1 = x1;
+        for (int part = 0; part < PARTS; ++part) {
+          if (gives) {
 #pragma unroll
-          for (int n = 0; n < ND; ++n) {
-            const float4 v = buf[(((group % half) * WM + wm) * ND + n) * 32 + lane];
-            o[n][0] = o[n][0] * a0 + v.x * b0;
-            o[n][1] = o[n][1] * a0 + v.y * b0;
-            o[n][2] = o[n][2] * a1 + v.z * b1;
-            o[n][3] = o[n][3] * a1 + v.w * b1;
+            for (int n = 0; n < NP; ++n) {
+              const float* v = o[part * NP + n];
+              buf[(at * NP + n) * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
+            }
+            stat[at * 32 + lane] = make_float4(m0, m1, l0, l1);
           }
+          __syncthreads();
+          if (takes) {
+            if (part == 0) {
+              const float4 t = stat[at * 32 + lane];
+              const float x0 = fmaxf(m0, t.x), x1 = fmaxf(m1, t.y);
+              const float u0 = x0 == -INFINITY ? 0.f : x0, u1 = x1 == -INFINITY ? 0.f : x1;
+              a0 = weight(m0 - u0);
+              a1 = weight(m1 - u1);
+              b0 = weight(t.x - u0);
+              b1 = weight(t.y - u1);
+              l0 = l0 * a0 + t.z * b0;
+              l1 = l1 * a1 + t.w * b1;
+              m0 = x0;
+              m1 = x1;
+            }
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+              const float4 v = buf[(at * NP + n) * 32 + lane];
+              float* to = o[part * NP + n];
+              to[0] = to[0] * a0 + v.x * b0;
+              to[1] = to[1] * a0 + v.y * b0;
+              to[2] = to[2] * a1 + v.z * b1;
+              to[3] = to[3] * a1 + v.w * b1;
+            }
+          }
+          __syncthreads();
         }
-        __syncthreads();
       }
     }
     if (group == 0) {
@@ -483,8 +549,10 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
 // and sums its columns over all rows, so every sum has one owner and one order.
 constexpr int kMassRows = 64;  // query rows held in shared memory at a time
 
+// Rows of 512 bytes: two stages, so that two CTAs fit an SM.
 template <typename T, int D>
 struct MassSmem {
+  static constexpr int kStages = sizeof(T) * D == 512 ? 2 : 3;
   static constexpr int kStageBytes = kTile * Rows<T, D>::kBytes;
   static constexpr int kRing = kStages * kStageBytes;
   static constexpr int kQ = kMassRows * Rows<T, D>::kBytes;
@@ -526,12 +594,13 @@ __device__ int path_nodes(const int32_t* path, int path_len, int nodes, int room
 // CTAs per SM, by shared memory (67 KB for bf16 rows of 128: three).
 template <typename T, int D>
 constexpr int mass_ctas() {
-  return sizeof(T) * D == 128 ? 4 : sizeof(T) * D == 256 ? 3 : 1;
+  return sizeof(T) * D == 128 ? 4 : sizeof(T) * D == 256 ? 3 : 2;
 }
 template <typename T, int D, bool BIAS>
 __global__ __launch_bounds__(kThreads, mass_ctas<T, D>()) void cache_mass_kernel(const __grid_constant__ MassParams p) {
   using R = Rows<T, D>;
   using S = MassSmem<T, D>;
+  constexpr int kStages = S::kStages;
   // As in the attention: powers of two where the last bits do not matter.
   constexpr bool POW2 = !BIAS && sizeof(T) == 2;
   const float unit = POW2 ? p.scale * kLog2e : p.scale;
@@ -730,28 +799,30 @@ cudaError_t tree_run(const TreeParams& p, cudaStream_t s) {
 template <typename T, int D, bool BIAS>
 cudaError_t tree_variant(const TreeParams& p, int wm, cudaStream_t s) {
   if (p.heads / p.c.kv_heads * p.nodes <= 8) return tree_run<T, D, 1, BIAS, true>(p, s);
-  return wm == 1   ? tree_run<T, D, 1, BIAS, false>(p, s)
-         : wm == 2 ? tree_run<T, D, 2, BIAS, false>(p, s)
-                   : tree_run<T, D, 4, BIAS, false>(p, s);
+  if constexpr (sizeof(T) == 2)
+    if (wm == 4) return tree_run<T, D, 4, BIAS, false>(p, s);
+  return wm == 1 ? tree_run<T, D, 1, BIAS, false>(p, s) : tree_run<T, D, 2, BIAS, false>(p, s);
 }
 template <typename T, int D>
 cudaError_t tree_variant(const TreeParams& p, int wm, cudaStream_t s) {
   return p.rel_bias ? tree_variant<T, D, true>(p, wm, s) : tree_variant<T, D, false>(p, wm, s);
 }
 
-// Warps that share a key range: one per 16 query rows, up to four.
+// Warps that share a key range: one per 16 query rows, up to four. float32: up
+// to two, since each takes all the keys apart for its products (96 rows of 128
+// x 1334 keys, 21 sequences of 4 heads: 381 us with four, 225 with two).
 int tree_wm(const TreeParams& p) {
   const int rows = p.heads / p.c.kv_heads * p.nodes;
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  return rows <= 16 ? 1 : rows <= 32 || p.c.dtype == 0 ? 2 : 4;
 }
 int tree_smem(const TreeParams& p, int wm) {
   const int b = p.c.batch;
   const bool f = p.c.dtype == 0;
   if (p.c.head_dim == 64) {
-    if (f) return wm == 1 ? TreeSmem<float, 64, 1>::bytes(b) : wm == 2 ? TreeSmem<float, 64, 2>::bytes(b) : TreeSmem<float, 64, 4>::bytes(b);
+    if (f) return wm == 1 ? TreeSmem<float, 64, 1>::bytes(b) : TreeSmem<float, 64, 2>::bytes(b);
     return wm == 1 ? TreeSmem<__nv_bfloat16, 64, 1>::bytes(b) : wm == 2 ? TreeSmem<__nv_bfloat16, 64, 2>::bytes(b) : TreeSmem<__nv_bfloat16, 64, 4>::bytes(b);
   }
-  if (f) return wm == 1 ? TreeSmem<float, 128, 1>::bytes(b) : wm == 2 ? TreeSmem<float, 128, 2>::bytes(b) : TreeSmem<float, 128, 4>::bytes(b);
+  if (f) return wm == 1 ? TreeSmem<float, 128, 1>::bytes(b) : TreeSmem<float, 128, 2>::bytes(b);
   return wm == 1 ? TreeSmem<__nv_bfloat16, 128, 1>::bytes(b) : wm == 2 ? TreeSmem<__nv_bfloat16, 128, 2>::bytes(b) : TreeSmem<__nv_bfloat16, 128, 4>::bytes(b);
 }
 

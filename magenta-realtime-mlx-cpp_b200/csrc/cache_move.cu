@@ -305,12 +305,24 @@ __global__ __launch_bounds__(kEvictThreads, 4) void cache_evict_kernel(const __g
     const uint32_t k = in ? key_at(t + lane) : 0u;
     bool keep;
     if (counted) {
-      int ahead = 0;  // slots that come before this one
-#pragma unroll 4
-      for (int j = 0; j < slice; j += 4) {
+      // Slots that come before this one: of those before this warp's 32 the
+      // equal ones too, of those behind only the larger ones.
+      int ahead = 0;
+      const int end = (len + 3) / 4 * 4;
+#pragma unroll 8
+      for (int j = 0; j < t; j += 4) {
         const uint4 v = *reinterpret_cast<const uint4*>(keys + j);
-        ahead += (v.x > k || (v.x == k && j < t + lane)) + (v.y > k || (v.y == k && j + 1 < t + lane)) +
-                 (v.z > k || (v.z == k && j + 2 < t + lane)) + (v.w > k || (v.w == k && j + 3 < t + lane));
+        ahead += (v.x >= k) + (v.y >= k) + (v.z >= k) + (v.w >= k);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t v = __shfl_sync(0xffffffffu, k, i);
+        ahead += v > k || (v == k && i < lane);
+      }
+#pragma unroll 8
+      for (int j = t + 32; j < end; j += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(keys + j);
+        ahead += (v.x > k) + (v.y > k) + (v.z > k) + (v.w > k);
       }
       keep = in && ahead < p.budget;
     } else {
