@@ -423,8 +423,9 @@ int mrtdf_resolve_inference_bundle(const char* cache_root, const char* tag, mrtd
 /* Rows of head_dim contiguous elements of the cache's dtype: row (l, b, h, n)
  * of layer, sequence, head and node starts at ptr + l * stride_l + b * stride_b
  * + h * stride_h + n * stride_n elements. Every row starts on a 16-byte
- * boundary; strides are not negative. (The rows of a fused q|k|v projection
- * are three such views of one buffer.) */
+ * boundary; strides are not negative, and rows that are written do not overlap
+ * (a zero stride is refused there; rows that are only read may share memory).
+ * (The rows of a fused q|k|v projection are three such views of one buffer.) */
 typedef struct mrtdf_rows {
   void* ptr;
   int64_t stride_l, stride_b, stride_h, stride_n;
@@ -576,7 +577,8 @@ int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* args, vo
  * `dtype`; out is of out_dtype (float32 for float32 x). The weights are not
  * rounded: sums of x times whole numbers are scaled in float32. 1 <= m <= 64,
  * k <= 2^17 a multiple of the group (32, 64 or 128), n <= 2^24; x's rows and
- * packed on 16-byte boundaries.
+ * packed on 16-byte boundaries. A row of x with an infinity or a NaN gives
+ * results that are not finite, and touches no other row.
  */
 typedef struct mrtdf_q4_args {
   size_t struct_bytes;
@@ -590,8 +592,8 @@ typedef struct mrtdf_q4_args {
   int64_t x_stride, out_stride;
   int32_t m, n, k, group, dtype, out_dtype, device;
 } mrtdf_q4_args;
-/* Workspace of a call with these sizes (x as the product takes it, some bytes
- * per element of x; 0 where x is small). args' pointers must be set as for the call, workspace
+/* Workspace of a call with these sizes (x as the product takes it and partial
+ * sums, up to 10 MB and some bytes per element of x; 0 where x is small). args' pointers must be set as for the call, workspace
  * aside. */
 int mrtdf_q4_linear_workspace(const mrtdf_q4_args* args, size_t* bytes);
 int mrtdf_q4_linear(const mrtdf_q4_args* args, void* stream);
@@ -600,7 +602,7 @@ int mrtdf_q4_linear(const mrtdf_q4_args* args, void* stream);
  * Weights (n, k) of `dtype` to the form that mrtdf_q4_linear takes: per group
  * of columns bias = min, scale = (max - min) / 15, both rounded to dtype, and
  * q = (w - bias) / scale with those two, rounded to the nearest (ties to even)
- * and clamped to 0 .. 15; a scale of 0 gives q = 0. Weights are finite.
+ * and clamped to 0 .. 15; a scale of 0 gives q = 0. Weights are finite, max - min too.
  */
 typedef struct mrtdf_q4_pack_args {
   size_t struct_bytes;

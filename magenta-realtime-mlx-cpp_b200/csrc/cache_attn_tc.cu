@@ -21,8 +21,8 @@
 //   warp 16    TMA producer: K and V tiles through a ring, 128-byte swizzle,
 //              over the items of the run without a stop;
 //   warp 17    MMA issuer: S = Q K^T into one of three TMEM buffers, two
-//              tiles ahead, then O_g += P V for the tile's group g, weights as two bf16 parts (16 bits of a
-//              weight; the second product is hidden too).
+//              tiles ahead, then O_g += P V for the tile's group g, weights as
+//              two bf16 parts (16 bits of a weight).
 //              V is an MN-major operand of 64-column parts kSub bytes apart.
 // A maximum is raised only when a tile exceeds it by 8 units of its scale.
 // The drafted rows are a tile of their own behind the cached ones.
@@ -31,6 +31,14 @@
 // rows behind the length are zeroed in the last cached tile, and in the drafted
 // tile single values that are not finite, which the rows that do see them take
 // from global memory at the end.
+//
+// Measured on a B200, us in a graph: 4 sequences x 8 kv heads of 128, 24 nodes of
+// four heads each (96 rows), 4097 to 16360 rows, 169 MB: 65 (2.6 TB/s, 270
+// TFLOP/s of real rows). A tile of 64 keys takes 0.95 us per SM, 0.75 of it its
+// products (two for the weights, since they keep 16 bits); the run's start (the
+// schedule and the queries to TMEM) 6, its end 4, the join of split items 3. With
+// heads of 64 a tile takes 0.86 us: the chain scores - maximum - exponentials -
+// weights - products of one tile, with two tiles in flight, not the products.
 #include <cuda.h>
 
 #include "cache_sched.cuh"

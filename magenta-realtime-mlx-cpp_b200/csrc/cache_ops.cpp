@@ -117,6 +117,20 @@ CacheView cache_view(const mrtdf_cache* c, const char* op, bool values) {
   return v;
 }
 
+// Rows that are written: a step of zero would put several into one.
+void apart(std::initializer_list<std::pair<int64_t, int64_t>> steps_and_extents, const char* op, const char* what) {
+  for (const auto& s : steps_and_extents)
+    if (s.second > 1 && s.first == 0) invalid(std::string(op) + ": rows of " + what + " are written and must not share memory (zero stride)");
+}
+void apart(const CacheView& c, const char* op) {
+  apart({{c.sl, c.layers}, {c.sb, c.batch}, {c.sh, c.kv_heads}, {c.st, c.capacity}}, op, "the cache");
+}
+
+// Addresses of elements of `esize` bytes.
+void check_element(const void* p, int esize, const char* op, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % esize) invalid(std::string(op) + ": " + what + " is not aligned to its elements");
+}
+
 void check_heads(const char* op, int heads, int kv_heads, int nodes) {
   if (heads < 1 || heads % kv_heads) invalid(std::string(op) + ": heads must be a multiple of kv_heads");
   if (nodes < 1) invalid(std::string(op) + ": nodes must be positive");
@@ -150,6 +164,7 @@ TreeParams tree_params(const mrtdf_cache* cache, const mrtdf_tree_args* a, const
   p.k_new = rows_view(a->k_new, 1, b, kv, n, es, op, "k_new");
   p.v_new = rows_view(a->v_new, 1, b, kv, n, es, op, "v_new");
   p.out = rows_view(a->out, 1, b, a->heads, n, es, op, "out");
+  apart({{p.out.sb, b}, {p.out.sh, a->heads}, {p.out.sn, n}}, op, "out");
   p.lse = a->lse;
   p.parents = a->parents;
   p.rel_bias = a->rel_bias;
@@ -172,6 +187,9 @@ Q4Params q4_params(const mrtdf_q4_args* a, const char* op) {
   if (!a->x || !a->packed || !a->scales || !a->biases || !a->out) invalid("q4_linear: NULL argument");
   if (!aligned16(a->x) || !aligned16(a->packed)) invalid("q4_linear: x and packed must be 16-byte aligned");
   if (a->device < 0) invalid("q4_linear: device is negative");
+  check_element(a->scales, es, op, "scales");
+  check_element(a->biases, es, op, "biases");
+  check_element(a->out, a->out_dtype == MRTDF_DTYPE_FP32 ? 4 : 2, op, "out");
   Q4Params p{};
   p.x = a->x;
   p.packed = static_cast<const uint8_t*>(a->packed);
@@ -269,6 +287,7 @@ int mrtdf_cache_commit(const mrtdf_cache* cache, const mrtdf_commit_args* a, voi
     if (a->next_pos_out && !p.c.next_pos) invalid("cache_commit: next_pos_out needs cache.next_pos");
     const int es = dtype_bytes(p.c.dtype, op), l = p.c.layers, b = p.c.batch, kv = p.c.kv_heads;
     if ((int64_t)l * kv * a->path_len >= (int64_t)1 << 26) out_of_range("cache_commit: too many rows");
+    apart(p.c, op);
     p.k_new = rows_view(a->k_new, l, b, kv, a->nodes, es, op, "k_new");
     p.v_new = rows_view(a->v_new, l, b, kv, a->nodes, es, op, "v_new");
     p.path = a->path;
@@ -296,6 +315,7 @@ int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* a, void*
     if (a->budget < 1) invalid("cache_evict: budget must be positive");
     if (a->recent < 0 || a->sinks < 0 || (int64_t)a->recent + a->sinks > a->budget)
       invalid("cache_evict: recent and sinks must be >= 0 and fit into the budget together");
+    apart(p.c, op);
     if (a->lens_out == p.c.lens) invalid("cache_evict: lens_out must be another buffer than lens");
     p.mass = a->mass;
     p.mass_out = a->mass_out;
@@ -347,6 +367,10 @@ int mrtdf_q4_quantize(const mrtdf_q4_pack_args* a, void* stream) {
     if (!a->w || !a->packed || !a->scales || !a->biases) invalid("q4_quantize: NULL argument");
     if (a->n > 1 && a->w_stride < a->k) invalid("q4_quantize: w_stride is less than k");
     if (a->device < 0) invalid("q4_quantize: device is negative");
+    const int es = dtype_bytes(a->dtype, op);
+    check_element(a->w, es, op, "w");
+    check_element(a->scales, es, op, "scales");
+    check_element(a->biases, es, op, "biases");
     Q4PackParams p{};
     p.w = a->w;
     p.packed = static_cast<uint8_t*>(a->packed);

@@ -729,6 +729,18 @@ def test_q4_infinite_scales_stay_in_their_rows(ops, m):
     assert torch.equal(y[:, keep], fine[:, keep])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("m", [3, 20])
+def test_q4_rows_that_are_not_finite_touch_no_other(ops, dtype, value, m):
+    x, packed, scales, biases = q4_case(m, dtype, m, 40, 256, 64)
+    want = ops.q4_linear(x, packed, scales, biases)
+    x[1, 70] = value
+    y = ops.q4_linear(x, packed, scales, biases)
+    keep = torch.arange(m, device=DEV) != 1
+    assert torch.equal(y[keep], want[keep]) and not bool(torch.isfinite(y[1]).any())
+
+
 def test_q4_out_types_views_and_streams(ops):
     x, packed, scales, biases = q4_case(5, BF, 6, 100, 256, 64)
     a = check_q4(ops, x, packed, scales, biases, out_dtype=F32)

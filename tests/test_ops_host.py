@@ -159,6 +159,30 @@ def test_workspace_follows_the_capacity(ops):
     assert c.run("tree")[0] == 1
 
 
+@pytest.mark.parametrize("field,extent", [("sl", "layers"), ("sb", "batch"), ("sh", "kv_heads"), ("st", "capacity")])
+def test_rows_that_are_written_do_not_share_memory(ops, field, extent):
+    """An expanded cache can be read (attention, weight), not written."""
+    for what in ("commit", "evict"):
+        c = Call(ops)
+        c.cache |= {field: 0, extent: max(2, c.cache[extent]), "pos": 256, "next_pos": 256}
+        c.commit |= dict(k_new=rows(sl=8192), v_new=rows(sl=8192), next_pos_out=512)
+        assert c.run(what)[0] == 1 and b"zero stride" in ops.lib().mrtdf_last_error()
+    c = Call(ops)
+    if field != "sl":
+        c.cache[field] = 0
+        assert c.run("workspace")[0] == 0
+        c.tree["out"] = rows(**{{"st": "sn"}.get(field, field): 0})
+        assert c.run("workspace")[0] == 1
+
+
+@pytest.mark.parametrize("what,field,value", [("q4", "scales", 257), ("q4", "biases", 257), ("q4", "out", 257), ("pack", "w", 257),
+                                              ("pack", "scales", 257), ("pack", "biases", 255)])
+def test_elements_are_aligned(ops, what, field, value):
+    c = Call(ops)
+    getattr(c, what)[field] = value
+    assert c.run(what)[0] == 1
+
+
 def test_strides_of_single_elements_do_not_matter(ops):
     c = Call(ops)
     c.cache |= dict(batch=1, sb=7, sl=3)
