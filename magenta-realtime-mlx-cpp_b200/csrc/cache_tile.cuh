@@ -137,29 +137,42 @@ __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<__nv_bfloat16
   }
 }
 
+// float32: three products of tf32 parts, the small ones apart. The tensor cores
+// cut off what does not fit an accumulator, always towards zero, so the large
+// products are summed over 32 columns at most before they are added, rounded, to
+// the score (chains over all 128 columns doubled the result's error).
 template <int D, int NT>
 __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<float, D>& q, uint32_t keys, int lane) {
   using R = Rows<float, D>;
+  constexpr int CHAIN = 4;
   const int m = lane >> 3, r = lane & 7;
   float low[NT][4] = {};
 #pragma unroll
-  for (int ks = 0; ks < D / 8; ++ks) {
-    uint32_t ah[4], al[4];
+  for (int k0 = 0; k0 < D / 8; k0 += CHAIN) {
+    float high[NT][4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split_tf32(q.a[ks][i], ah[i], al[i]);
+    for (int ks = k0; ks < k0 + CHAIN; ++ks) {
+      uint32_t ah[4], al[4];
 #pragma unroll
-    for (int jp = 0; jp < NT / 2; ++jp) {
-      uint32_t b[4], bh[4], bl[4];
-      ldsm_x4_g(b, keys + R::at(16 * jp + (m >> 1) * 8 + r, 2 * ks + (m & 1)));
+      for (int i = 0; i < 4; ++i) split_tf32(q.a[ks][i], ah[i], al[i]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split_tf32(b[i], bh[i], bl[i]);
+      for (int jp = 0; jp < NT / 2; ++jp) {
+        uint32_t b[4], bh[4], bl[4];
+        ldsm_x4_g(b, keys + R::at(16 * jp + (m >> 1) * 8 + r, 2 * ks + (m & 1)));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        mma_tf32(low[2 * jp + h], al, bh[2 * h], bh[2 * h + 1]);
-        mma_tf32(low[2 * jp + h], ah, bl[2 * h], bl[2 * h + 1]);
-        mma_tf32(s[2 * jp + h], ah, bh[2 * h], bh[2 * h + 1]);
+        for (int i = 0; i < 4; ++i) split_tf32(b[i], bh[i], bl[i]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mma_tf32(low[2 * jp + h], al, bh[2 * h], bh[2 * h + 1]);
+          mma_tf32(low[2 * jp + h], ah, bl[2 * h], bl[2 * h + 1]);
+          mma_tf32(high[2 * jp + h], ah, bh[2 * h], bh[2 * h + 1]);
+        }
       }
     }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] += high[j][e];
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j)
