@@ -165,6 +165,8 @@ TreeParams tree_params(const mrtdf_cache* cache, const mrtdf_tree_args* a, const
   p.v_new = rows_view(a->v_new, 1, b, kv, n, es, op, "v_new");
   p.out = rows_view(a->out, 1, b, a->heads, n, es, op, "out");
   apart({{p.out.sb, b}, {p.out.sh, a->heads}, {p.out.sn, n}}, op, "out");
+  if (p.out.ptr == p.q.ptr || p.out.ptr == p.k_new.ptr || p.out.ptr == p.v_new.ptr || p.out.ptr == p.c.k || p.out.ptr == p.c.v)
+    invalid(std::string(op) + ": out must be another buffer than the inputs");
   p.lse = a->lse;
   p.parents = a->parents;
   p.rel_bias = a->rel_bias;
@@ -187,6 +189,7 @@ Q4Params q4_params(const mrtdf_q4_args* a, const char* op) {
   if (!a->x || !a->packed || !a->scales || !a->biases || !a->out) invalid("q4_linear: NULL argument");
   if (!aligned16(a->x) || !aligned16(a->packed)) invalid("q4_linear: x and packed must be 16-byte aligned");
   if (a->device < 0) invalid("q4_linear: device is negative");
+  if (a->out == a->x) invalid(std::string(op) + ": out must be another buffer than x");
   check_element(a->scales, es, op, "scales");
   check_element(a->biases, es, op, "biases");
   check_element(a->out, a->out_dtype == MRTDF_DTYPE_FP32 ? 4 : 2, op, "out");
@@ -290,6 +293,8 @@ int mrtdf_cache_commit(const mrtdf_cache* cache, const mrtdf_commit_args* a, voi
     apart(p.c, op);
     p.k_new = rows_view(a->k_new, l, b, kv, a->nodes, es, op, "k_new");
     p.v_new = rows_view(a->v_new, l, b, kv, a->nodes, es, op, "v_new");
+    if (p.k_new.ptr == p.c.k || p.k_new.ptr == p.c.v || p.v_new.ptr == p.c.v || p.v_new.ptr == p.c.k)
+      invalid("cache_commit: the new rows must be another buffer than the cache");
     p.path = a->path;
     p.lens_out = a->lens_out;
     p.next_pos_out = a->next_pos_out;

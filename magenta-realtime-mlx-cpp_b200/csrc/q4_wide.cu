@@ -108,7 +108,9 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * C::kStage + C::kMerge);
   uint64_t* empty = full + ST;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ int abort_flag;
   if (tid == 0) {
+    abort_flag = 0;
     for (int i = 0; i < ST; ++i) {
       mbar_init(full + i, 1 + kScaleWarps);
       mbar_init(empty + i, C::CW);
@@ -120,6 +122,15 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
   const int u0 = q.start(blockIdx.x), u1 = q.start(blockIdx.x + 1);
   float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(p.ws) + q.passes * C::x_bytes(q.pairs)) +
                 (int64_t)blockIdx.x * 2 * C::ROWS * kBlock;
+
+  // A wait that runs out ends all of the CTA's: copies stop, the sums become NaN.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*(volatile int*)&abort_flag) return false;
+    if (mbar_wait_bounded(bar, parity, nullptr)) return true;
+    *(volatile int*)&abort_flag = 1;
+    return false;
+  };
 
   if (warp >= C::CW) {
     // One thread issues the copies.
@@ -151,6 +162,11 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
                2 * C::kXStep, full + a.st);
     };
     const int head = min(u1, u0 + ST);
+    int issued = head;  // stages [u0, issued)
+    // No copy may still be landing when the CTA exits.
+    auto landed = [&] {
+      for (int u = max(u0, issued - ST); u < issued; ++u) mbar_wait_bounded(full + (u - u0) % ST, (u - u0) / ST & 1, nullptr);
+    };
     At to_copy = begin();
     if (issues)
       for (int u = u0; u < head; ++u, next(to_copy)) weights(to_copy);
@@ -162,12 +178,13 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
     if (C::APART && warp == C::CW + kScaleWarps) {
       if (issues) {
         prologue();
-        for (int u = head, turn = 0; u < u1; ++u, next(to_copy)) {
-          mbar_wait_bounded(empty + to_copy.st, turn, nullptr);
+        for (int u = head, turn = 0; u < u1 && wait(empty + to_copy.st, turn); ++u, next(to_copy)) {
           weights(to_copy);
           rows_of_x(to_copy);
+          issued = u + 1;
           if (to_copy.st == ST - 1) turn ^= 1;
         }
+        landed();
       }
       return;
     }
@@ -214,16 +231,19 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
     for (int d = 0; d < kAhead; ++d) load(ahead[d], u0 + d);
     if (!C::APART && issues) prologue();
     int st = 0, turn = 0;
-    for (int u = u0; u < u1; u += kAhead) {
+    bool on = true;
+    for (int u = u0; u < u1 && on; u += kAhead) {
 #pragma unroll
       for (int d = 0; d < kAhead; ++d) {
         if (u + d >= u1) break;
         if (u + d >= head) {
-          mbar_wait_bounded(empty + st, turn, nullptr);
+          on = __all_sync(0xffffffffu, wait(empty + st, turn));
+          if (!on) break;
           if (!C::APART && issues) {
             weights(to_copy);
             rows_of_x(to_copy);
             next(to_copy);
+            issued = u + d + 1;
           }
         }
         auto* to = reinterpret_cast<ScalePair<T>*>(smem + st * C::kStage + C::kScales);
@@ -238,6 +258,7 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
         load(ahead[d], u + d + kAhead);
       }
     }
+    if (!C::APART && issues) landed();
   } else {
     const int wt = warp & 7, wk = warp >> 3, g = lane >> 2, c = lane & 3;
     const uint32_t swz = (uint32_t)(g >> 1 & 3) << 4;  // of rows g and g + 8
@@ -246,7 +267,7 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
     int item = u0 / q.pairs, pr = u0 - item * q.pairs, st = 0, phase = 0;
     bool whole = pr == 0;  // the row block from its first stage on
     for (int u = u0; u < u1; ++u) {
-      mbar_wait_bounded(full + st, phase, nullptr);
+      wait(full + st, phase);
       const uint32_t stage = base + st * C::kStage;
 #pragma unroll
       for (int half = 0; half < 2 / C::WK; ++half) {
@@ -298,6 +319,10 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
       }
       const bool ends = ++pr == q.pairs;
       if (ends || u + 1 == u1) {
+        if (*(volatile int*)&abort_flag) {
+#pragma unroll
+          for (int i = 0; i < NT * Y; ++i) y[i / Y][i % Y] = NAN;
+        }
         if (C::WK > 1) {  // the other warp's sums of these rows
           float* merge = reinterpret_cast<float*>(smem + ST * C::kStage) + wt * 32 + lane;
           if (wk) {

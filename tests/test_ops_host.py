@@ -43,16 +43,16 @@ class Call:
 
     def __init__(self, ops):
         self.ops = ops
-        self.cache = dict(size=_CACHE.size, k=256, v=256, sl=65536, sb=32768, sh=8192, st=64, layers=1, batch=2,
+        self.cache = dict(size=_CACHE.size, k=4096, v=8192, sl=65536, sb=32768, sh=8192, st=64, layers=1, batch=2,
                           kv_heads=2, capacity=128, head_dim=64, dtype=1, device=0, lens=256, pos=0, next_pos=0)
-        self.tree = dict(size=_TREE.size, q=rows(), k_new=rows(), v_new=rows(), out=rows(), lse=0, parents=0, rel_bias=0,
+        self.tree = dict(size=_TREE.size, q=rows(), k_new=rows(), v_new=rows(), out=rows(ptr=1024), lse=0, parents=0, rel_bias=0,
                          workspace=0, workspace_bytes=0, heads=4, nodes=8, rel_len=0, scale=1.0)
         self.mass = dict(size=_MASS.size, q=rows(), k_new=rows(), lse=256, path=256, rel_bias=0, mass=256, mass_out=256,
                          heads=4, nodes=8, path_len=4, rel_len=0, scale=1.0, decay=1.0)
         self.commit = dict(size=_COMMIT.size, k_new=rows(), v_new=rows(), path=256, lens_out=512, next_pos_out=0, nodes=8,
                            path_len=4)
         self.evict = dict(size=_EVICT.size, mass=256, mass_out=256, pos_out=256, lens_out=512, budget=64, recent=8, sinks=1)
-        self.q4 = dict(size=_Q4.size, x=256, packed=256, scales=256, biases=256, out=256, workspace=256, workspace_bytes=1 << 20,
+        self.q4 = dict(size=_Q4.size, x=256, packed=256, scales=256, biases=256, out=512, workspace=256, workspace_bytes=1 << 20,
                        x_stride=16384, out_stride=64, m=16,
                        n=64, k=16384, group=32, dtype=1, out_dtype=1, device=0)
         self.pack = dict(size=_PACK.size, w=256, packed=256, scales=256, biases=256, w_stride=128, n=4, k=128, group=32,
@@ -171,7 +171,7 @@ def test_rows_that_are_written_do_not_share_memory(ops, field, extent):
     if field != "sl":
         c.cache[field] = 0
         assert c.run("workspace")[0] == 0
-        c.tree["out"] = rows(**{{"st": "sn"}.get(field, field): 0})
+        c.tree["out"] = rows(ptr=1024, **{{"st": "sn"}.get(field, field): 0})
         assert c.run("workspace")[0] == 1
 
 
@@ -183,10 +183,19 @@ def test_elements_are_aligned(ops, what, field, value):
     assert c.run(what)[0] == 1
 
 
+def test_outputs_are_other_buffers_than_inputs(ops):
+    for what, change in (("tree", dict(out=rows())), ("tree", dict(out=rows(ptr=4096))), ("tree", dict(out=rows(ptr=8192))),
+                         ("q4", dict(out=256)), ("commit", dict(k_new=rows(ptr=4096))), ("commit", dict(v_new=rows(ptr=8192)))):
+        c = Call(ops)
+        getattr(c, what).update(change)
+        assert c.run("workspace" if what == "tree" else what)[0] == 1
+        assert b"another buffer" in ops.lib().mrtdf_last_error()
+
+
 def test_strides_of_single_elements_do_not_matter(ops):
     c = Call(ops)
     c.cache |= dict(batch=1, sb=7, sl=3)
-    c.tree |= dict(q=rows(sb=5, sl=1), nodes=1, k_new=rows(sn=3, sb=1), v_new=rows(sn=1, sb=9), out=rows(sn=2, sb=3))
+    c.tree |= dict(q=rows(sb=5, sl=1), nodes=1, k_new=rows(sn=3, sb=1), v_new=rows(sn=1, sb=9), out=rows(ptr=1024, sn=2, sb=3))
     c.tree["q"] = rows(sb=5, sn=9)
     assert c.run("workspace")[0] == 0
 
