@@ -559,9 +559,10 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
 // and 8 bytes of weight per cached row bound it. A warp owns 16 keys of a tile
 // and sums its columns over all rows, so every sum has one owner and one order.
 // 2 layers x 8 sequences x 8 kv heads x 3001 to 8190 rows of 128, bf16, five
-// nodes of four heads each: 50 us for 190 MB (3.8 TB/s; the exponentials of 32
-// padded rows, of which 20 count, go beside the keys); 2 x 16 heads of 64 over
-// 250 rows, float32: 6.7 us, latency.
+// nodes of four heads each: 41 us for 190 MB (4.7 TB/s; the exponentials of 32
+// padded rows, of which 20 count, go beside the keys; with the weights so far
+// asked for in the tile that adds to them, 50 us); 2 x 16 heads of 64 over 250 rows,
+// float32: 6.6 us, latency.
 constexpr int kMassRows = 64;  // query rows held in shared memory at a time
 
 // Rows of 512 bytes: two stages, so that two CTAs fit an SM.
@@ -717,24 +718,30 @@ __global__ __launch_bounds__(kThreads, mass_ctas<T, D>()) void cache_mass_kernel
       QFrag<T, D> q;
       if (here <= 16) q_from_smem<D>(q, smem_u32(q_s), lane);
 
+      // A lane's weights so far, keys 8 j + 2 c + e of a tile, in the lanes with
+      // g = 0: asked for a tile ahead.
+      auto before = [&](int t, float (*to)[2]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = t * kTile + warp * 16 + 8 * j + 2 * c + e;
+            to[j][e] = 0.f;
+            if (g == 0 && t < t1 && there && key < (rb ? len + count : len)) to[j][e] = (rb ? p.mass_out : p.mass)[row_at + key];
+          }
+      };
+      const float decay = rb ? 1.f : p.decay;
+      float ahead[2][2];
+      before(t0, ahead);
       for (int t = t0, st = 0, fill = kStages - 1; t < t1; ++t) {
+        float old[2][2] = {{ahead[0][0], ahead[0][1]}, {ahead[1][0], ahead[1][1]}};
+        before(t + 1, ahead);
         cp_async_wait<kStages - 2>();
         __syncwarp();
         if (t + kStages - 1 < t1) fetch(t + kStages - 1, fill);
         cp_async_commit();
         const int key0 = t * kTile + warp * 16;
         const uint32_t keys = ring + st * S::kStageBytes;
-        // Lane's weights: keys 8 j + 2 c + e, from the lanes with g = 0.
-        float old[2][2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int key = key0 + 8 * j + 2 * c + e;
-            old[j][e] = g == 0 && key < len + count && there
-                            ? (rb ? p.mass_out[row_at + key] : key < len ? p.decay * p.mass[row_at + key] : 0.f)
-                            : 0.f;
-          }
         float col[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
         const bool tail = key0 + 16 > len;
         for (int mt = 0; mt * 16 < here; ++mt) {
@@ -770,7 +777,8 @@ __global__ __launch_bounds__(kThreads, mass_ctas<T, D>()) void cache_mass_kernel
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) col[j][e] += __shfl_xor_sync(0xffffffffu, col[j][e], o);
             const int key = key0 + 8 * j + 2 * c + e;
-            if (g == 0 && key < len + count && there) p.mass_out[row_at + key] = old[j][e] + col[j][e];
+            if (g == 0 && key < len + count && there)
+              p.mass_out[row_at + key] = (rb || key < len ? decay * old[j][e] : 0.f) + col[j][e];
           }
         st = st + 1 == kStages ? 0 : st + 1;
         fill = fill + 1 == kStages ? 0 : fill + 1;
