@@ -160,6 +160,10 @@ __device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpre
 // Joins the partial rows of items that several CTAs worked on. A CTA's two
 // partial blocks of mb rows hold [head_dim / 4][row][4] sums, then the rows'
 // maxima (natural units) and sums of weights. A thread per row and four columns.
+// A part that a row saw nothing in has the maximum -inf and the sum 0. One whose
+// scores are all NaN has the maximum -inf too, since a maximum passes NaN over,
+// but a sum of NaN, which makes the row NaN as it does where one CTA has the item;
+// so does a NaN value whose weight is 0 beside another part's.
 // blockIdx.x is an item, or where there are more items than CTAs, a CTA whose run
 // may begin inside one (the first such run of an item joins it).
 inline bool join_by_item(const TreeParams& p) { return p.c.batch * p.c.kv_heads * p.row_blocks <= p.grid; }
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void tree_join_kernel(const __grid_consta
       const float* src = part(c);
       const float f = ex2((src[mb * D + r] - u) * kLog2e), l = src[mb * D + mb + r];
       const float4 v = *reinterpret_cast<const float4*>(src + (quad * mb + r) * 4);
-      if (f == 0.f) continue;  // an empty part's sums may be anything
+      if (l == 0.f) continue;  // an empty part's columns may be anything
       sum += l * f;
       acc.x += v.x * f;
       acc.y += v.y * f;

@@ -1,0 +1,65 @@
+"""The operators on device buffers (mrtops.py) where values are not finite, very
+large, or all of one sign. Oracles and tolerances: test_ops_gpu.py."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_ops_gpu import BF, DEV, F32, attend, ints, near, normal, ops, tree_inputs  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+# dtype, D, heads, kv heads, nodes: few rows and many (the tcgen05 kernel where
+# the cache is long and bf16).
+TREES = [(BF, 64, 2, 1, 3), (F32, 64, 2, 1, 3), (F32, 128, 4, 2, 5), (BF, 128, 16, 1, 8), (BF, 64, 16, 1, 8), (F32, 64, 16, 1, 8)]
+
+
+@pytest.mark.parametrize("dtype,D,H,KV,N", TREES)
+@pytest.mark.parametrize("cap", [200, 6000])
+def test_tree_nan_query_gives_nan_however_it_is_split(ops, dtype, D, H, KV, N, cap):
+    """A row of NaN scores is NaN, in whole items and in those that several CTAs
+    share; the rows beside it are untouched."""
+    x = tree_inputs(3, dtype, 1, H, KV, N, D, cap)
+    lens = ints([cap - 5])
+    wo, wl, to, tl = attend(*x, lens)
+    x[0][0, 1, 0, 7] = math.nan
+    out, lse = ops.tree_attention(*x, lens)
+    assert bool(torch.isnan(out[0, 1, 0]).all()) and bool(torch.isnan(lse[0, 1, 0]))
+    wo[0, 1, 0], wl[0, 1, 0] = 0.0, 0.0
+    out[0, 1, 0], lse[0, 1, 0] = 0.0, 0.0
+    near(out, wo, to)
+    near(lse, wl, tl)
+
+
+@pytest.mark.parametrize("dtype,D,H,KV,N", TREES)
+@pytest.mark.parametrize("cap,first,last", [(200, 70, 130), (6000, 1500, 4500), (6000, 0, 6000)])
+def test_tree_nan_keys_that_rows_see_give_nan(ops, dtype, D, H, KV, N, cap, first, last):
+    """Keys that are NaN over more than a CTA's share of the cache."""
+    x = tree_inputs(4, dtype, 2, H, KV, N, D, cap)
+    x[3][0, :, first:last, 3] = math.nan
+    lens = ints([cap, cap])
+    wo, wl, to, tl = attend(*(t[1:] for t in x), lens[1:])
+    out, lse = ops.tree_attention(*x, lens)
+    assert bool(torch.isnan(out[0]).all()) and bool(torch.isnan(lse[0]).all())
+    near(out[1:], wo, to)
+    near(lse[1:], wl, tl)
+
+
+@pytest.mark.parametrize("dtype,D,H,KV,N", TREES)
+@pytest.mark.parametrize("cap", [200, 6000])
+def test_tree_nan_value_of_a_far_smaller_weight(ops, dtype, D, H, KV, N, cap):
+    """A NaN value that a row sees with a weight that underflows: 0 x NaN, in the
+    same CTA as the large weights or in another."""
+    x = tree_inputs(5, dtype, 1, H, KV, N, D, cap)
+    x[0][:], x[3][:, :, : cap // 2] = 1.0, -320.0 / D
+    lens = ints([cap])
+    wo, wl, to, tl = attend(*x, lens)
+    x[4][0, :, 7, 3] = math.nan
+    out, lse = ops.tree_attention(*x, lens)
+    near(lse, wl, tl)
+    assert bool(torch.isnan(out[..., 3]).all())
+    out[..., 3], wo[..., 3] = 0.0, 0.0
+    near(out, wo, to)
