@@ -502,6 +502,11 @@ typedef struct mrtdf_tree_args {
 int mrtdf_tree_attention_workspace(const mrtdf_cache* cache, const mrtdf_tree_args* args, size_t* bytes);
 int mrtdf_tree_attention(const mrtdf_cache* cache, const mrtdf_tree_args* args, void* stream);
 
+/* Failure-detection check: the same call, but a wait of its kernels for a copy
+ * or a product looks once and gives up instead of after 0.5 s. The call ends as
+ * one does whose wait runs out; its results mean nothing. */
+int mrtdf_check_tree_attention_wait(const mrtdf_cache* cache, const mrtdf_tree_args* args, void* stream);
+
 /*
  * The attention weight that each cached row collects (what mrtdf_cache_evict
  * ranks rows by). path[b] lists the accepted nodes of sequence b, increasing

@@ -168,9 +168,13 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
   Cursor<true> cur;
   cur.seek(w0, lens, first, batch, blocks, nodes);
 
+  // A wait that runs out makes all of the CTA's later ones give up at once. The
+  // copies and the products stop there; the softmax warps go on to the end with
+  // what they find, since they meet at barriers (the two warps of a row in every
+  // tile, all of them at an item's ends) and one that left would keep the others.
   auto wait = [&](uint64_t* b, uint32_t parity) -> bool {
     if (*(volatile int*)&abort_flag) return false;
-    if (mbar_wait_bounded(b, parity, nullptr)) return true;
+    if (p.wait_once ? mbar_test_wait(b, parity) : mbar_wait_bounded(b, parity, nullptr)) return true;
     *(volatile int*)&abort_flag = 1;
     return false;
   };
@@ -349,9 +353,8 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
           near = __any_sync(0xffffffffu, k < valid && (int)((unsigned)next - (unsigned)mine) < p.rel_len - 1);
         }
         const int buf = it % kBufs;
-        if (ok) ok = wait(s_full + buf, (uint32_t)((it / kBufs) & 1));
-        // The TMEM accesses below are .sync.aligned: decide warp-uniformly.
-        if (!(ok = __all_sync(0xffffffffu, ok) != 0)) break;
+        // The TMEM accesses below are .sync.aligned: the warp goes on together.
+        ok = __all_sync(0xffffffffu, ok && wait(s_full + buf, (uint32_t)((it / kBufs) & 1))) != 0;
         tc_fence_after();
         const uint32_t scores = tmem + lane_base + (uint32_t)(buf * 64);
         float x[32];
@@ -362,8 +365,8 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         }
         // Values that must not meet the products.
         const bool cleaned = fresh || (tile + 1) * kTile > len;
-        if (cleaned) {
-          if (!(ok = __all_sync(0xffffffffu, wait(kv_full + st, (uint32_t)((it / NS) & 1))) != 0)) break;
+        if (cleaned) ok = __all_sync(0xffffffffu, ok && wait(kv_full + st, (uint32_t)((it / NS) & 1))) != 0;
+        if (cleaned && ok) {
           uint8_t* vs = smem + st * 2 * C::kKvBytes + C::kKvBytes;
           for (int x4 = half * kRows + row; x4 < kTile * (D / 8); x4 += 2 * kRows) {
             const int r = x4 / (D / 8), ch = x4 % (D / 8);
@@ -436,7 +439,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
           if (__any_sync(0xffffffffu, scale)) {
             // O holds products made with the old maximum: scale it once the
             // last of them (this group's tile before) has retired.
-            if (!(ok = __all_sync(0xffffffffu, wait(p_empty + (it - 2) % kBufs, (uint32_t)(((it - 2) / kBufs) & 1))) != 0)) break;
+            ok = __all_sync(0xffffffffu, ok && wait(p_empty + (it - 2) % kBufs, (uint32_t)(((it - 2) / kBufs) & 1))) != 0;
             tc_fence_after();
 #pragma unroll
             for (int cc = 0; cc < D / 2; cc += 16) {
@@ -472,8 +475,7 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
         warp_arrive(p_full + buf);
       }
       i += n;
-      if (ok) ok = wait(o_done, (uint32_t)(seg & 1));
-      ok = __all_sync(0xffffffffu, ok) != 0;
+      ok = __all_sync(0xffffffffu, ok && wait(o_done, (uint32_t)(seg & 1))) != 0;
       // Join the groups; every softmax thread passes here once per item.
       if (half == 0) xm[group][row] = m;
       xl[part4][row] = l;

@@ -209,6 +209,22 @@ Q4Params q4_params(const mrtdf_q4_args* a, const char* op) {
   return p;
 }
 
+void run_tree_attention(const mrtdf_cache* cache, const mrtdf_tree_args* args, bool wait_once, void* stream, const char* op) {
+  TreeParams p = tree_params(cache, args, op);
+  p.wait_once = wait_once;
+  size_t floats = 0;
+  cuda_check(plan_tree_attention(p, op_sm_count(cache->device), &floats), op);
+  if (floats) {
+    if (!args->workspace || args->workspace_bytes < floats * sizeof(float))
+      invalid(std::string(op) + ": the workspace is smaller than mrtdf_tree_attention_workspace says (" +
+              std::to_string(floats * sizeof(float)) + " bytes)");
+    if (!aligned16(args->workspace)) invalid(std::string(op) + ": the workspace must be 16-byte aligned");
+    p.ws = static_cast<float*>(args->workspace);
+  }
+  DeviceScope on(cache->device, op);
+  cuda_check(launch_tree_attention(p, static_cast<cudaStream_t>(stream)), op);
+}
+
 }  // namespace
 
 extern "C" {
@@ -225,21 +241,11 @@ int mrtdf_tree_attention_workspace(const mrtdf_cache* cache, const mrtdf_tree_ar
 }
 
 int mrtdf_tree_attention(const mrtdf_cache* cache, const mrtdf_tree_args* args, void* stream) {
-  return guarded([&] {
-    const char* op = "tree_attention";
-    TreeParams p = tree_params(cache, args, op);
-    size_t floats = 0;
-    cuda_check(plan_tree_attention(p, op_sm_count(cache->device), &floats), op);
-    if (floats) {
-      if (!args->workspace || args->workspace_bytes < floats * sizeof(float))
-        invalid("tree_attention: the workspace is smaller than mrtdf_tree_attention_workspace says (" +
-                std::to_string(floats * sizeof(float)) + " bytes)");
-      if (!aligned16(args->workspace)) invalid("tree_attention: the workspace must be 16-byte aligned");
-      p.ws = static_cast<float*>(args->workspace);
-    }
-    DeviceScope on(cache->device, op);
-    cuda_check(launch_tree_attention(p, static_cast<cudaStream_t>(stream)), op);
-  });
+  return guarded([&] { run_tree_attention(cache, args, false, stream, "tree_attention"); });
+}
+
+int mrtdf_check_tree_attention_wait(const mrtdf_cache* cache, const mrtdf_tree_args* args, void* stream) {
+  return guarded([&] { run_tree_attention(cache, args, true, stream, "check_tree_attention_wait"); });
 }
 
 int mrtdf_cache_mass(const mrtdf_cache* cache, const mrtdf_mass_args* a, void* stream) {

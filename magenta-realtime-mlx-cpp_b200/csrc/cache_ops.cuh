@@ -61,6 +61,7 @@ struct TreeParams {
   int row_blocks; // blocks of query rows per (sequence, kv head)
   int tc;         // 1: the tcgen05 kernel
   int stream;     // 1: equal runs of key tiles per CTA, joined afterwards; 0: whole items
+  int wait_once;  // 1: a device wait looks once and gives up (failure detection)
 };
 
 struct MassParams {
