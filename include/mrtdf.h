@@ -407,7 +407,9 @@ int mrtdf_resolve_inference_bundle(const char* cache_root, const char* tag, mrtd
  * (depthformer/decode.cpp:150-237) drafts one chain and re-attends with the
  * single-chain kernels. Each call checks its arguments on the host, queues its
  * kernels on `stream` (a cudaStream_t, NULL = the legacy default stream) of
- * `device` and returns without waiting. It allocates nothing, keeps nothing
+ * `device` and returns without waiting. A kernel's own waits for its copies and
+ * products are bounded (0.5 s); where one runs out the kernel ends all the same
+ * and the result rows that it was working on are NaN. It allocates nothing, keeps nothing
  * between calls and may be captured into a CUDA graph; calls on different
  * streams or from different threads may overlap as long as no buffer that one
  * of them writes (workspaces included) is used by another. What a call writes
@@ -503,8 +505,8 @@ int mrtdf_tree_attention_workspace(const mrtdf_cache* cache, const mrtdf_tree_ar
 int mrtdf_tree_attention(const mrtdf_cache* cache, const mrtdf_tree_args* args, void* stream);
 
 /* Failure-detection check: the same call, but a wait of its kernels for a copy
- * or a product looks once and gives up instead of after 0.5 s. The call ends as
- * one does whose wait runs out; its results mean nothing. */
+ * or a product looks once and gives up instead of after 0.5 s. Rows of out and
+ * lse are then NaN as a whole, or right where no wait of theirs ran out. */
 int mrtdf_check_tree_attention_wait(const mrtdf_cache* cache, const mrtdf_tree_args* args, void* stream);
 
 /*

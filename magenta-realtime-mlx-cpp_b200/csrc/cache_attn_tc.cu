@@ -290,6 +290,19 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       if (lane == 0) arrive(b);
     };
     auto soft_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory"); };
+    // The same barrier; whether `v` holds in all of the threads.
+    auto soft_all = [](bool v) -> bool {
+      uint32_t all;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\t"
+          "setp.ne.u32 p, %1, 0;\n\t"
+          "bar.red.and.pred q, 1, %2, p;\n\t"
+          "selp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(all)
+          : "r"((uint32_t)v), "n"(kSoft)
+          : "memory");
+      return all != 0;
+    };
     bool ok = true;
     int i = 0, masks_of = -1;
     for (int seg = 0; cur.w < w1; ++seg) {
@@ -479,7 +492,9 @@ __global__ __launch_bounds__(kTcThreads, 1) void tree_attn_tc_kernel(const __gri
       // Join the groups; every softmax thread passes here once per item.
       if (half == 0) xm[group][row] = m;
       xl[part4][row] = l;
-      soft_sync();
+      // A row's columns, its sum and its parts' joins go by several threads: where
+      // one has given up, all of them write NaN (also where nothing was summed yet).
+      ok = soft_all(ok);
       const float m0 = xm[0][row], m1 = xm[1][row], mx = fmaxf(m0, m1), u = mx == -INFINITY ? 0.f : mx;
       const float a0 = weight(m0 - u), a1 = weight(m1 - u), sum = (xl[0][row] + xl[1][row]) * a0 + (xl[2][row] + xl[3][row]) * a1;
       const float mn = POW2 ? mx * kLn2 : mx;

@@ -61,3 +61,23 @@ def test_tree_ends_when_waits_run_out(ops, D, bias, B, H, KV, N, cap):
     assert time.perf_counter() - begin < 0.4  # less than one wait's limit
     small = [t[:1] for t in x]
     check_tree(ops, small, lens[:1], None, scale=0.125, **kw)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bias", [0, 32])
+@pytest.mark.parametrize("B,H,KV,N,cap", TREES)
+def test_tree_rows_whose_waits_ran_out_are_nan(ops, D, bias, B, H, KV, N, cap):
+    """In whole items and in those that several CTAs share: a row is NaN, its lse
+    too, or as without the hurry. None is zeros or a softmax over a part."""
+    x = tree_inputs(1, BF, B, H, KV, N, D, cap)
+    lens = ints([cap - 3 * b for b in range(B)])
+    kw = dict(rel_bias=normal(2, H, bias)) if bias else {}
+    want, want_lse = ops.tree_attention(*x, lens, scale=0.125, **kw)
+    failed = 0
+    for _ in range(3):
+        out, lse = hurried_tree(ops, *x, lens, **kw)
+        gone = torch.isnan(lse)
+        assert torch.equal(torch.isnan(out), gone[..., None].expand_as(out))
+        assert torch.equal(out[~gone], want[~gone]) and torch.equal(lse[~gone], want_lse[~gone])
+        failed += int(gone.sum())
+    assert failed
