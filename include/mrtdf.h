@@ -607,6 +607,11 @@ typedef struct mrtdf_q4_args {
 int mrtdf_q4_linear_workspace(const mrtdf_q4_args* args, size_t* bytes);
 int mrtdf_q4_linear(const mrtdf_q4_args* args, void* stream);
 
+/* Failure-detection check: the same call, but a wait of its kernel for a free
+ * place to copy to looks once and gives up, where the call streams x. Results
+ * are NaN or right, one by one. */
+int mrtdf_check_q4_linear_wait(const mrtdf_q4_args* args, void* stream);
+
 /*
  * Weights (n, k) of `dtype` to the form that mrtdf_q4_linear takes: per group
  * of columns bias = min, scale = (max - min) / 15, both rounded to dtype, and

@@ -209,6 +209,22 @@ Q4Params q4_params(const mrtdf_q4_args* a, const char* op) {
   return p;
 }
 
+void run_q4_linear(const mrtdf_q4_args* a, bool wait_once, void* stream, const char* op) {
+  Q4Params p = q4_params(a, op);
+  p.wait_once = wait_once;
+  size_t need = 0;
+  const int sms = op_sm_count(a->device);
+  cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, &need, nullptr), op);
+  if (need) {
+    if (!a->workspace || a->workspace_bytes < need)
+      invalid("q4_linear: the workspace is smaller than mrtdf_q4_linear_workspace says (" + std::to_string(need) + " bytes)");
+    if (!aligned16(a->workspace)) invalid("q4_linear: the workspace must be 16-byte aligned");
+    p.ws = a->workspace;
+  }
+  DeviceScope on(a->device, op);
+  cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, nullptr, static_cast<cudaStream_t>(stream)), op);
+}
+
 void run_tree_attention(const mrtdf_cache* cache, const mrtdf_tree_args* args, bool wait_once, void* stream, const char* op) {
   TreeParams p = tree_params(cache, args, op);
   p.wait_once = wait_once;
@@ -349,21 +365,11 @@ int mrtdf_q4_linear_workspace(const mrtdf_q4_args* a, size_t* bytes) {
 }
 
 int mrtdf_q4_linear(const mrtdf_q4_args* a, void* stream) {
-  return guarded([&] {
-    const char* op = "q4_linear";
-    Q4Params p = q4_params(a, op);
-    size_t need = 0;
-    const int sms = op_sm_count(a->device);
-    cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, &need, nullptr), op);
-    if (need) {
-      if (!a->workspace || a->workspace_bytes < need)
-        invalid("q4_linear: the workspace is smaller than mrtdf_q4_linear_workspace says (" + std::to_string(need) + " bytes)");
-      if (!aligned16(a->workspace)) invalid("q4_linear: the workspace must be 16-byte aligned");
-      p.ws = a->workspace;
-    }
-    DeviceScope on(a->device, op);
-    cuda_check(launch_q4_linear(p, a->dtype, a->out_dtype, sms, nullptr, static_cast<cudaStream_t>(stream)), op);
-  });
+  return guarded([&] { run_q4_linear(a, false, stream, "q4_linear"); });
+}
+
+int mrtdf_check_q4_linear_wait(const mrtdf_q4_args* a, void* stream) {
+  return guarded([&] { run_q4_linear(a, true, stream, "check_q4_linear_wait"); });
 }
 
 int mrtdf_q4_quantize(const mrtdf_q4_pack_args* a, void* stream) {

@@ -19,6 +19,7 @@ struct Q4Params {
   void* out;               // (m, n), row stride out_stride elements
   int64_t x_stride, out_stride;
   int m, n, k, group;
+  int wait_once;  // 1: a wait of the copying warps looks once and gives up (failure detection)
 };
 
 struct Q4PackParams {

@@ -124,10 +124,12 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
                 (int64_t)blockIdx.x * 2 * C::ROWS * kBlock;
 
   // A wait that runs out ends all of the CTA's: copies stop, the sums become NaN.
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (mbar_try_wait(bar, parity)) return true;
+  // `once`: it looks once and gives up (the waits for a free place in the ring,
+  // when p.wait_once asks for it; in the products' own the test costs 1 to 2.5 %).
+  auto wait = [&](uint64_t* bar, uint32_t parity, bool once = false) {
+    if (once ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)) return true;
     if (*(volatile int*)&abort_flag) return false;
-    if (mbar_wait_bounded(bar, parity, nullptr)) return true;
+    if (!once && mbar_wait_bounded(bar, parity, nullptr)) return true;
     *(volatile int*)&abort_flag = 1;
     return false;
   };
@@ -178,7 +180,7 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
     if (C::APART && warp == C::CW + kScaleWarps) {
       if (issues) {
         prologue();
-        for (int u = head, turn = 0; u < u1 && wait(empty + to_copy.st, turn); ++u, next(to_copy)) {
+        for (int u = head, turn = 0; u < u1 && wait(empty + to_copy.st, turn, p.wait_once); ++u, next(to_copy)) {
           weights(to_copy);
           rows_of_x(to_copy);
           issued = u + 1;
@@ -237,7 +239,7 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
       for (int d = 0; d < kAhead; ++d) {
         if (u + d >= u1) break;
         if (u + d >= head) {
-          on = __all_sync(0xffffffffu, wait(empty + st, turn));
+          on = __all_sync(0xffffffffu, wait(empty + st, turn, p.wait_once));
           if (!on) break;
           if (!C::APART && issues) {
             weights(to_copy);
@@ -266,8 +268,9 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
     float y[NT][Y] = {};
     int item = u0 / q.pairs, pr = u0 - item * q.pairs, st = 0, phase = 0;
     bool whole = pr == 0;  // the row block from its first stage on
+    bool on = true;        // after a wait that ran out no other is begun: each may take the hardware's time for one look
     for (int u = u0; u < u1; ++u) {
-      wait(full + st, phase);
+      on = on && wait(full + st, phase);
       const uint32_t stage = base + st * C::kStage;
 #pragma unroll
       for (int half = 0; half < 2 / C::WK; ++half) {

@@ -45,7 +45,8 @@ EXPORTS = [
     "mrtdf_context_roll", "mrtdf_llm_to_rvq", "mrtdf_rvq_to_llm", "mrtdf_resolve_inference_bundle",
     # operators on device buffers (bound in mrtops.py)
     "mrtdf_stream_cache", "mrtdf_tree_attention_workspace", "mrtdf_tree_attention",
-    "mrtdf_check_tree_attention_wait", "mrtdf_cache_mass", "mrtdf_cache_commit", "mrtdf_cache_evict", "mrtdf_q4_linear_workspace", "mrtdf_q4_linear", "mrtdf_q4_quantize",
+    "mrtdf_check_tree_attention_wait", "mrtdf_cache_mass", "mrtdf_cache_commit", "mrtdf_cache_evict", "mrtdf_q4_linear_workspace", "mrtdf_q4_linear",
+    "mrtdf_check_q4_linear_wait", "mrtdf_q4_quantize",
 ]
 
 

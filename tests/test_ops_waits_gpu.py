@@ -10,8 +10,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_ops_gpu import BF, DEV, attend, check_tree, ints, near, normal, ops, tree_inputs  # noqa: E402,F401
-from test_ops_host import _CACHE, _TREE  # noqa: E402
+from test_ops_gpu import BF, DEV, F32, check_q4, check_tree, ints, normal, ops, q4_case, tree_inputs  # noqa: E402,F401
+from test_ops_host import _CACHE, _Q4, _TREE  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,36 @@ def test_tree_rows_whose_waits_ran_out_are_nan(ops, D, bias, B, H, KV, N, cap):
         assert torch.equal(out[~gone], want[~gone]) and torch.equal(lse[~gone], want_lse[~gone])
         failed += int(gone.sum())
     assert failed
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,n,k,group", [(8, 10000, 8192, 128), (33, 20000, 4096, 32), (16, 700, 131072, 64)])
+def test_q4_ends_and_shows_waits_that_ran_out(ops, dtype, m, n, k, group):
+    """Row blocks that one CTA has and those that several share; more stages per CTA
+    than its ring holds, so that its copies have to wait for a free place."""
+    x, packed, scales, biases = q4_case(m, dtype, m, n, k, group)
+    want = ops.q4_linear(x, packed, scales, biases, out_dtype=F32)
+    L, need = ops.lib(), ctypes.c_size_t()
+    L.mrtdf_q4_linear_workspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_size_t)]
+    L.mrtdf_check_q4_linear_wait.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+    out = torch.zeros(m, n, device=DEV)
+
+    def args(ws, size):
+        return _Q4.pack(_Q4.size, x.data_ptr(), packed.data_ptr(), scales.data_ptr(), biases.data_ptr(), out.data_ptr(), ws, size,
+                        k, n, m, n, k, group, int(dtype is BF), 0, 0)
+
+    assert L.mrtdf_q4_linear_workspace(args(0, 0), ctypes.byref(need)) == 0 and need.value
+    ws = torch.zeros(need.value, dtype=torch.uint8, device=DEV)
+    failed = 0
+    for _ in range(3):
+        torch.cuda.synchronize()
+        begin = time.perf_counter()
+        rc = L.mrtdf_check_q4_linear_wait(args(ws.data_ptr(), need.value), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, L.mrtdf_last_error()
+        torch.cuda.synchronize()
+        assert time.perf_counter() - begin < 2.0
+        gone = torch.isnan(out)
+        assert torch.equal(out[~gone], want[~gone])
+        failed += int(gone.sum())
+    assert failed
+    assert torch.equal(check_q4(ops, x, packed, scales, biases, out_dtype=F32), want)
