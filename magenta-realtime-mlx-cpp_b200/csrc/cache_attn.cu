@@ -752,6 +752,9 @@ __global__ __launch_bounds__(kThreads, mass_ctas<T, D>()) void cache_mass_kernel
           for (int h = 0; h < 2; ++h) {
             const int row = mt * 16 + g + 8 * h, i = BIAS || tail ? node_s[row] : 0;
             const float lse = lse_s[row];
+            // A row that gives nothing is left out by a choice: its weight would
+            // be exp(x - inf), NaN where a key makes x one (0 x inf among them).
+            const bool gives = lse != INFINITY;
             const float* tab = BIAS ? p.rel_bias + (int64_t)(kvh * heads_per + head_s[row]) * p.rel_len : nullptr;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
@@ -766,7 +769,7 @@ __global__ __launch_bounds__(kThreads, mass_ctas<T, D>()) void cache_mass_kernel
                   x += __ldg(tab + min(max((int)((unsigned)(next + i) - (unsigned)at), 0), p.rel_len - 1));
                 }
                 const float w = ex2(POW2 ? x - lse : (x - lse) * kLog2e);
-                col[j][e] += !tail || key0 + k - len <= i ? w : 0.f;
+                col[j][e] += gives && (!tail || key0 + k - len <= i) ? w : 0.f;
               }
           }
         }

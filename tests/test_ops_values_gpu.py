@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_ops_gpu import BF, DEV, F32, attend, ints, near, normal, ops, tree_inputs  # noqa: E402,F401
+from test_ops_gpu import BF, DEV, F32, attend, collected, ints, near, normal, ops, tree_inputs  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,42 @@ def test_tree_nan_value_of_a_far_smaller_weight(ops, dtype, D, H, KV, N, cap):
     assert bool(torch.isnan(out[..., 3]).all())
     out[..., 3], wo[..., 3] = 0.0, 0.0
     near(out, wo, to)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("bias", [0, 16])
+@pytest.mark.parametrize("cap", [60, 300])
+def test_mass_rows_that_count_for_nothing(ops, dtype, bias, cap):
+    """Rows with lse = -inf add nothing whatever their scores are; nor do the
+    rows that fill a product up."""
+    L, B, H, KV, N, D = 1, 2, 3, 1, 5, 64
+    q, k, kn = normal(1, L, B, H, N, D, dtype=dtype, std=0.2), normal(2, L, B, KV, cap, D, dtype=dtype), normal(3, L, B, KV, N, D, dtype=dtype)
+    lse = torch.full((L, B, H, N), -math.inf, device=DEV)
+    lse[0, 1] = 3.0  # the second sequence's rows count
+    k[0, 0, 0, 7, 3], k[0, 0, 0, 20] = math.nan, math.inf
+    kn[0, 0, 0, 1] = math.nan
+    mass, path = normal(5, L, B, KV, cap).abs(), ints([[1, 4, -1], [0, 2, 3]])
+    lens = ints([cap - 10, cap - 20])
+    kw = dict(decay=0.5)
+    if bias:
+        kw |= dict(rel_bias=normal(7, H, bias))
+    got = ops.cache_mass(q, lse, kn, k, lens, path, mass, mass_out=torch.full_like(mass, -7.0), **kw)
+    t = cap - 10
+    assert torch.equal(got[0, 0, 0, :t], 0.5 * mass[0, 0, 0, :t])
+    assert not got[0, 0, 0, t:t + 2].any() and bool((got[0, 0, 0, t + 2:] == -7).all())
+    k[0, 0], kn[0, 0] = 0.0, 0.0
+    want, tol = collected(q, lse, kn, k, lens, path, mass, torch.full_like(mass, -7.0), **kw)
+    near(got[:, 1], want[:, 1], tol[:, 1])
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_mass_of_an_infinite_key_is_its_own_rows(ops, sign):
+    """A key with an infinity weighs what the real rows say: exp(-inf) = 0 or
+    infinity, not what a row of zeros would make of it."""
+    q, k, kn = normal(1, 1, 1, 2, 3, 64, dtype=BF), normal(2, 1, 1, 1, 200, 64, dtype=BF), normal(3, 1, 1, 1, 3, 64, dtype=BF)
+    q[..., 9] = 0.5
+    k[0, 0, 0, 11, 9] = -sign * math.inf
+    mass, lse = torch.ones(1, 1, 1, 200, device=DEV), torch.full((1, 1, 2, 3), 5.0, device=DEV)
+    got = ops.cache_mass(q, lse, kn, k, ints([150]), ints([[0, 2]]), mass.clone())
+    assert float(got[0, 0, 0, 11]) == (1.0 if sign > 0 else math.inf)
+    assert bool(torch.isfinite(got[0, 0, 0, 12:]).all())
