@@ -9,13 +9,12 @@
 // per output) and, next to it, by the instructions that unpack the weights. A
 // warp takes 16 output rows as the M side of m16n8k16 (fp16), the rows of x
 // are its eight columns; weights go from global memory through a private
-// cp.async ring to registers. fp16 has ten mantissa bits, so two nibbles of a
-// 16-bit half become numbers without a shift: w & 0x000f000f | 0x64006400 is
-// the pair 1024 + q, w & 0x00f000f0 | 0x64006400 the pair 1024 + 16 q (exact).
-//   float32 results: one more instruction each makes them q - 8 (exact).
-//   bf16 results: they stay, the odd columns of x are divided by 16, and the
-//   sums 1024 X_even + 64 X_odd are taken off in float32. That loses seven bits
-//   of float32, nothing in a bf16 result: 5 instructions per 8 weights, not 9.
+// cp.async ring to registers, where two nibbles of a 16-bit half become q - 8 in
+// two instructions and without a shift (unpack, q4_tile.cuh). Without the second,
+// an offset of 1024 per weight goes through the products' sums and comes off
+// afterwards; the matrix instructions cut sums off towards zero, so x of one sign
+// (after a gated activation) then put every result 2.3e-4 of its size too low (16384
+// x 8192, 8 rows: 24.2 us, 22.8 with the offset).
 // x is brought to fp16 by a power of two per row and group that puts the
 // group's largest |x| into [2^14, 2^15): bf16 x keeps all its bits (smaller
 // ones down to 2^-31 of the largest), float32 x becomes two columns, x = hi + lo
@@ -90,7 +89,6 @@ template <typename T, typename O, int G>
 __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __grid_constant__ Q4Params p,
                                                                       const __grid_constant__ Q4Plan q) {
   constexpr int WL = G / 32, GS = kStep / G, P = Parts<T>::N, ROWS = kCols / P, LD = ROWS + 1;  // rows of x
-  constexpr bool EIGHT = sizeof(O) == 4;
   extern __shared__ __align__(128) uint8_t smem[];
   const Q4Smem<T, G> at(q);
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5;
@@ -182,7 +180,7 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
   float4* factor = reinterpret_cast<float4*>(smem + at.factors);
   for (int i0 = tid; i0 - lane < all_words; i0 += threads) {
     const int m = i0 / words, wd = i0 - m * words;
-    bring_x<T, G, EIGHT>(
+    bring_x<T, G>(
         p, i0 < all_words ? m : -1, k0 + wd * 8,
         [&](int h, uint4 w) {
           if (i0 < all_words) *reinterpret_cast<uint4*>(smem + at.x + (m * P + h) * at.x_bytes + word_at<WL>(wd) * 16) = w;
@@ -227,10 +225,10 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
 #pragma unroll
         for (int i = 0; i < WL; ++i) {
           uint32_t a0[4], a1[4];
-          unpack<EIGHT>(w0[i], a0[0], a0[2]);
-          unpack<EIGHT>(w1[i], a0[1], a0[3]);
-          unpack<EIGHT>(w0[i] >> 8, a1[0], a1[2]);
-          unpack<EIGHT>(w1[i] >> 8, a1[1], a1[3]);
+          unpack(w0[i], a0[0], a0[2]);
+          unpack(w1[i], a0[1], a0[3]);
+          unpack(w0[i] >> 8, a1[0], a1[2]);
+          unpack(w1[i] >> 8, a1[1], a1[3]);
           const uint4 b = lds128(xa + gi * (WL * 64) + i * 64);
           if (i == 0) {
             mma_f16_first(acc, a0, b.x, b.y);

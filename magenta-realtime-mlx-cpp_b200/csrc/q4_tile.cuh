@@ -42,19 +42,18 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
   return v;
 }
 
-// The column pairs (0, 4), (1, 5) of w, or with w >> 8 (2, 6), (3, 7): q - 8
-// (EIGHT), or 1024 + q and 1024 + 16 q.
-template <bool EIGHT>
+// q - 8 of the column pairs (0, 4), (1, 5) of w, or with w >> 8 (2, 6), (3, 7). The
+// nibbles go under the bits of 1024 (an fp16 whose last place is 1, a published
+// way to make small integers floating): 1024 + q and 1024 + 16 q, exactly, then
+// - 1032 and / 16 - 72, exactly too.
 __device__ __forceinline__ void unpack(uint32_t w, uint32_t& even, uint32_t& odd) {
   // (w & mask) | magic in one instruction each
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(even) : "r"(w), "n"(0x000f000f), "r"(0x64006400u));
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(odd) : "r"(w), "n"(0x00f000f0), "r"(0x64006400u));
-  if (EIGHT) {
-    const __half2 e = __hadd2(*reinterpret_cast<const __half2*>(&even), __float2half2_rn(-1032.f));
-    const __half2 o = __hfma2(*reinterpret_cast<const __half2*>(&odd), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
-    even = *reinterpret_cast<const uint32_t*>(&e);
-    odd = *reinterpret_cast<const uint32_t*>(&o);
-  }
+  const __half2 e = __hadd2(*reinterpret_cast<const __half2*>(&even), __float2half2_rn(-1032.f));
+  const __half2 o = __hfma2(*reinterpret_cast<const __half2*>(&odd), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+  even = *reinterpret_cast<const uint32_t*>(&e);
+  odd = *reinterpret_cast<const uint32_t*>(&o);
 }
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -107,7 +106,7 @@ struct Parts<float> {
 // 4 WL neighbouring lanes, all lanes of a warp together. put(h, words) gets the
 // lane's eight values of part h, sums(h, {factor, addend, X, 0}) the group's.
 // Rows that do not exist (m < 0) and columns past k are zero.
-template <typename T, int G, bool EIGHT, typename Put, typename Sums>
+template <typename T, int G, typename Put, typename Sums>
 __device__ __forceinline__ void bring_x(const Q4Params& p, int m, int kk, Put&& put, Sums&& sums) {
   constexpr int WL = G / 32, P = Parts<T>::N, V = 8 * (int)sizeof(T) / 16;
   float v[8], big = 0.f;
@@ -137,19 +136,12 @@ __device__ __forceinline__ void bring_x(const Q4Params& p, int m, int kk, Put&& 
       f[e] = t2.x;
       f[e + 4] = t2.y;
     }
-    float even = (f[0] + f[4]) + (f[2] + f[6]), odd = (f[1] + f[5]) + (f[3] + f[7]);
+    float sum = ((f[0] + f[4]) + (f[2] + f[6])) + ((f[1] + f[5]) + (f[3] + f[7]));
 #pragma unroll
-    for (int o = 1; o < 4 * WL; o <<= 1) {
-      even += __shfl_xor_sync(0xffffffffu, even, o);
-      odd += __shfl_xor_sync(0xffffffffu, odd, o);
-    }
-    if (!EIGHT) {
-      w[1] = pack_f16(f[1] * 0.0625f, f[5] * 0.0625f);
-      w[3] = pack_f16(f[3] * 0.0625f, f[7] * 0.0625f);
-    }
+    for (int o = 1; o < 4 * WL; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     put(h, make_uint4(w[0], w[1], w[2], w[3]));
-    const float sum = down * (even + odd);
-    sums(h, make_float4(down, EIGHT ? 8.f * sum : -down * (1024.f * even + 64.f * odd), sum, 0.f));
+    sum *= down;
+    sums(h, make_float4(down, 8.f * sum, sum, 0.f));
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] -= f[e];
   }

@@ -61,7 +61,7 @@ struct Runs {
   __host__ __device__ int owner(int u) const { return (int)((((int64_t)u + 1) * grid - 1) / total); }
 };
 
-template <typename T, int G, int NT, bool EIGHT>
+template <typename T, int G, int NT>
 __global__ __launch_bounds__(128) void q4_wide_prepare_kernel(const __grid_constant__ Q4Params p, int pairs, int rows) {
   using C = Wide<T, G, NT>;
   constexpr int WL = G / 32, P = C::P;
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(128) void q4_wide_prepare_kernel(const __grid_const
   if (i - lane >= all) return;
   const int m = i / words, wd = i - m * words, in = wd % (4 * WL), gi = wd % 16 / (4 * WL);
   uint8_t* step = out + (int64_t)(wd / 16) * C::kXStep;
-  bring_x<T, G, EIGHT>(
+  bring_x<T, G>(
       p, i < all && m < rows && m0 + m < p.m ? m0 + m : -1, wd * 8,
       [&](int h, uint4 w) {
         const int col = m * P + h;
@@ -102,7 +102,6 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
                                                                               const __grid_constant__ Runs q) {
   using C = Wide<T, G, NT>;
   constexpr int WL = G / 32, GS = C::GS, P = C::P, Y = C::Y, COLS = C::COLS, ST = C::kStages;
-  constexpr bool EIGHT = sizeof(O) == 4;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((512 - (smem_u32(raw) & 511)) & 511);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * C::kStage + C::kMerge);
@@ -290,10 +289,10 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
 #pragma unroll
           for (int i = 0; i < WL; ++i) {
             uint32_t a0[4], a1[4];
-            unpack<EIGHT>(w0[i], a0[0], a0[2]);
-            unpack<EIGHT>(w1[i], a0[1], a0[3]);
-            unpack<EIGHT>(w0[i] >> 8, a1[0], a1[2]);
-            unpack<EIGHT>(w1[i] >> 8, a1[1], a1[3]);
+            unpack(w0[i], a0[0], a0[2]);
+            unpack(w1[i], a0[1], a0[3]);
+            unpack(w0[i] >> 8, a1[0], a1[2]);
+            unpack(w1[i] >> 8, a1[1], a1[3]);
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               const uint4 b = lds128(xa + ((gi * WL + i) * NT + j) * 512);
@@ -403,7 +402,7 @@ cudaError_t wide_run(const Q4Params& p, int sms, size_t* ws_bytes, cudaStream_t 
   cudaError_t e = allow_smem<K>();
   if (e != cudaSuccess) return e;
   const int words = q.pairs * 2 * (kStep / 8) * C::ROWS;
-  q4_wide_prepare_kernel<T, G, NT, sizeof(O) == 4><<<dim3((words + 127) / 128, q.passes), 128, 0, s>>>(p, q.pairs, q.rows);
+  q4_wide_prepare_kernel<T, G, NT><<<dim3((words + 127) / 128, q.passes), 128, 0, s>>>(p, q.pairs, q.rows);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr;

@@ -8,7 +8,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_ops_gpu import BF, DEV, F32, attend, collected, ints, near, normal, ops, tree_inputs  # noqa: E402,F401
+from test_ops_gpu import (  # noqa: E402,F401
+    BF, DEV, F32, attend, check_q4, collected, half_step, ints, near, normal, ops, q4_case, tree_inputs, unpack)
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +103,23 @@ def test_mass_of_an_infinite_key_is_its_own_rows(ops, sign):
     got = ops.cache_mass(q, lse, kn, k, ints([150]), ints([[0, 2]]), mass.clone())
     assert float(got[0, 0, 0, 11]) == (1.0 if sign > 0 else math.inf)
     assert bool(torch.isfinite(got[0, 0, 0, 12:]).all())
+
+
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("m,n,k,group", [(4, 4096, 1024, 64), (8, 4096, 8192, 128), (32, 2048, 8192, 32)])
+def test_q4_values_of_one_sign_lean_to_no_side(ops, dtype, out, m, n, k, group):
+    """x of one sign, weights of both: what the sums lose may not pile up on one
+    side. Rounding the count = m n results moves each by up to u = half a step of
+    itself, evenly to both sides, their mean by 6 u / sqrt(3 count) of their root
+    mean square at most. In the products of a group with q - 8 up to group / 16
+    steps follow one another, each cut off towards zero by 2^-23 of a sum that is
+    no larger than |x| |s (q - 8)| over the group; the rest is rounded evenly."""
+    x, packed, scales, biases = q4_case(m, dtype, m, n, k, group)
+    x = x.abs()
+    y = check_q4(ops, x, packed, scales, biases, out_dtype=out)
+    s, b = (t.cpu().double().repeat_interleave(group, 1) for t in (scales, biases))
+    q, xd = unpack(packed), x.cpu().double()
+    want, size = xd @ (s * q + b).T, xd @ (s * (q - 8).abs()).T
+    rms = float(want.square().mean().sqrt())
+    lean = float((y.cpu().double() - want).mean())
+    assert abs(lean) <= 6 * half_step(out) / math.sqrt(3 * m * n) * rms + group / 16 * 2.0**-23 * float(size.mean()) + 2.0**-22 * rms
