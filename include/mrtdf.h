@@ -587,7 +587,9 @@ int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* args, vo
  * rounded: sums of x times whole numbers are scaled in float32. 1 <= m <= 64,
  * k <= 2^17 a multiple of the group (32, 64 or 128), n <= 2^24; x's rows and
  * packed on 16-byte boundaries. A row of x with an infinity or a NaN gives
- * results that are not finite, and touches no other row.
+ * results that are not finite, and touches no other row. Finite x gives finite
+ * results where x times the weights, summed, fits float32 (scales and biases
+ * below 2^100).
  */
 typedef struct mrtdf_q4_args {
   size_t struct_bytes;

@@ -18,7 +18,7 @@
 // x is brought to fp16 by a power of two per row and group that puts the
 // group's largest |x| into [2^14, 2^15): bf16 x keeps all its bits (smaller
 // ones down to 2^-31 of the largest), float32 x becomes two columns, x = hi + lo
-// with 22 bits. The factor multiplies the group's float32 sum. Here every CTA
+// with 22 bits. The factor multiplies the group's float32 sum at the end. Here every CTA
 // does that for itself, which is right for small x only: for more, and for what
 // does not fit the shared memory, see q4_wide.cu.
 //
@@ -59,7 +59,7 @@ struct Q4Smem {
     x_bytes = q.slab * kStep * 2 + 64;
     x = q.warps * q.wk * kRing * kStageBytes;
     factors = x + kCols * x_bytes;
-    scales = factors + (q.slab * kStep / G) * kCols * 16;
+    scales = factors + (q.slab * kStep / G) * kCols * 8;
     part = scales + (q.slab * kStep / G) * q.tiles * 16 * 2 * (int)sizeof(T);
     const int units = q.tiles > q.warps * q.wk ? q.tiles : q.warps * q.wk;
     bytes = part + units * 16 * (kCols / Parts<T>::N + 1) * 4;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
     }
   }
   const int words = steps * (kStep / 8), all_words = words * p.m, spare = kCols - p.m * P;
-  float4* factor = reinterpret_cast<float4*>(smem + at.factors);
+  float2* factor = reinterpret_cast<float2*>(smem + at.factors);
   for (int i0 = tid; i0 - lane < all_words; i0 += threads) {
     const int m = i0 / words, wd = i0 - m * words;
     bring_x<T, G>(
@@ -185,23 +185,23 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
         [&](int h, uint4 w) {
           if (i0 < all_words) *reinterpret_cast<uint4*>(smem + at.x + (m * P + h) * at.x_bytes + word_at<WL>(wd) * 16) = w;
         },
-        [&](int h, float4 f) {
+        [&](int h, float2 f) {
           if (i0 < all_words && wd % (4 * WL) == 0) factor[wd / (4 * WL) * kCols + m * P + h] = f;
         });
   }
   for (int i = tid; i < words * spare; i += threads)  // columns without a row of x
     *reinterpret_cast<uint4*>(smem + at.x + (kCols - spare + i / words) * at.x_bytes + (i % words) * 16) = make_uint4(0, 0, 0, 0);
   for (int i = tid; i < gn * spare; i += threads)
-    factor[i / spare * kCols + kCols - spare + i % spare] = make_float4(0.f, 0.f, 0.f, 0.f);
+    factor[i / spare * kCols + kCols - spare + i % spare] = make_float2(0.f, 0.f);
   __syncthreads();
 
   float y[4 / P] = {};
   // Shared addresses of this lane's operands in the unit's step.
   const uint32_t swz = (uint32_t)(g >> 1 & 3) << 4;  // of rows g and g + 8
   const uint32_t x_first = smem_u32(smem + at.x) + g * at.x_bytes + c * 16 + wk * 2 * GS * (WL * 64);
-  const uint32_t f_first = smem_u32(smem + at.factors) + (wk * 2 * GS * kCols + 2 * c) * 16;
+  const uint32_t f_first = smem_u32(smem + at.factors) + (wk * 2 * GS * kCols + 2 * c) * 8;
   const uint32_t s_first = smem_u32(sb) + (wk * 2 * GS * stride + wt * 16 + g) * 2 * (int)sizeof(T);
-  const uint32_t x_step = GS * (WL * 64), fa_step = GS * kCols * 16, skip = 2 * q.wk - 2, s_group = stride * 2 * (int)sizeof(T);
+  const uint32_t x_step = GS * (WL * 64), fa_step = GS * kCols * 8, skip = 2 * q.wk - 2, s_group = stride * 2 * (int)sizeof(T);
   uint32_t xa = x_first, fa = f_first, sa = s_first, row = ring + g * (kStep / 2), st = 0;
   int tile = wt, step = 0;
   for (int t = 0; t < units; ++t) {
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kMaxWarps * 32, 1) void q4_linear_kernel(const __gr
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += acd[e];
-        add_group<P>(y, acc, lds128(fa + gi * kCols * 16), lds128(fa + gi * kCols * 16 + 16), s0, b0, s1, b1);
+        add_group<P>(y, acc, lds128(fa + gi * kCols * 8), s0, b0, s1, b1);
       }
       xa += x_step;
       fa += fa_step;

@@ -104,7 +104,8 @@ struct Parts<float> {
 };
 // x to fp16: 8 columns from kk on (one word of weights) per lane, a group by
 // 4 WL neighbouring lanes, all lanes of a warp together. put(h, words) gets the
-// lane's eight values of part h, sums(h, {factor, addend, X, 0}) the group's.
+// lane's eight values of part h, sums(h, {factor, X}) the group's power of two and
+// sum, the latter of the values as the product takes them: x is both multiplied.
 // Rows that do not exist (m < 0) and columns past k are zero.
 template <typename T, int G, typename Put, typename Sums>
 __device__ __forceinline__ void bring_x(const Q4Params& p, int m, int kk, Put&& put, Sums&& sums) {
@@ -140,30 +141,32 @@ __device__ __forceinline__ void bring_x(const Q4Params& p, int m, int kk, Put&& 
 #pragma unroll
     for (int o = 1; o < 4 * WL; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     put(h, make_uint4(w[0], w[1], w[2], w[3]));
-    sum *= down;
-    sums(h, make_float4(down, 8.f * sum, sum, 0.f));
+    sums(h, make_float2(down, sum));
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] -= f[e];
   }
 }
 
-// A group's products, scaled, onto y: rows g and g + 8 of the weights and
-// columns 2 c, 2 c + 1 with the factors u and v. The two are two rows of x
+// A group's products, scaled, onto y: rows g and g + 8 of the weights and columns
+// 2 c, 2 c + 1, whose factors and sums {f, X} are in `u`. The two are two rows of x
 // (y[0], y[1] of row g, y[2], y[3] of row g + 8), or the parts of one (y[0] and
-// y[1]), which are added before a scale meets them.
+// y[1]; one factor), which are added before a scale meets them.
+//   y += f (s (acc + 8 X) + b X)
+// The power of two comes last: s and b shrink the sums first, so nothing on the
+// way to a finite y is too large for float32 (|x| near its largest number
+// included) as long as s and b are below 2^100.
 template <int P>
-__device__ __forceinline__ void add_group(float* y, const float* acc, uint4 u, uint4 v, float s0, float b0, float s1, float b1) {
-  const float fu = __uint_as_float(u.x), ou = __uint_as_float(u.y), xu = __uint_as_float(u.z);
-  const float fv = __uint_as_float(v.x), ov = __uint_as_float(v.y), xv = __uint_as_float(v.z);
+__device__ __forceinline__ void add_group(float* y, const float* acc, uint4 u, float s0, float b0, float s1, float b1) {
+  const float fu = __uint_as_float(u.x), xu = __uint_as_float(u.y), fv = __uint_as_float(u.z), xv = __uint_as_float(u.w);
+  auto add = [](float y, float f, float acc, float x, float s, float b) { return fmaf(f, fmaf(s, fmaf(8.f, x, acc), b * x), y); };
   if constexpr (P == 2) {
-    const float o = ou + ov, x = xu + xv;
-    y[0] = fmaf(s0, fmaf(fu, acc[0], fmaf(fv, acc[1], o)), fmaf(b0, x, y[0]));
-    y[1] = fmaf(s1, fmaf(fu, acc[2], fmaf(fv, acc[3], o)), fmaf(b1, x, y[1]));
+    y[0] = add(y[0], fu, acc[0] + acc[1], xu + xv, s0, b0);
+    y[1] = add(y[1], fu, acc[2] + acc[3], xu + xv, s1, b1);
   } else {
-    y[0] = fmaf(s0, fmaf(fu, acc[0], ou), fmaf(b0, xu, y[0]));
-    y[1] = fmaf(s0, fmaf(fv, acc[1], ov), fmaf(b0, xv, y[1]));
-    y[2] = fmaf(s1, fmaf(fu, acc[2], ou), fmaf(b1, xu, y[2]));
-    y[3] = fmaf(s1, fmaf(fv, acc[3], ov), fmaf(b1, xv, y[3]));
+    y[0] = add(y[0], fu, acc[0], xu, s0, b0);
+    y[1] = add(y[1], fv, acc[1], xv, s0, b0);
+    y[2] = add(y[2], fu, acc[2], xu, s1, b1);
+    y[3] = add(y[3], fv, acc[3], xv, s1, b1);
   }
 }
 

@@ -41,7 +41,7 @@ struct Wide {
   static constexpr bool APART = NT <= 2;  // a warp of its own issues the copies: the loaders would be too slow for both
   static constexpr int kThreads = (CW + kScaleWarps + APART) * 32;
   static constexpr bool TWO = NT <= 2;  // two chains of products, where there are few to overlap
-  static constexpr int kXStep = COLS * 256 + GS * COLS * 16;  // bytes of x and its factors per step
+  static constexpr int kXStep = COLS * 256 + GS * COLS * 8;  // bytes of x and its factors per step
   static constexpr int kX = 2 * kBoxBytes, kScales = kX + 2 * kXStep;
   static constexpr int kStage = (kScales + 2 * GS * kBlock * 2 * (int)sizeof(T) + 511) / 512 * 512;
   static constexpr int kMerge = WK > 1 ? 8 * 32 * NT * Y * 4 : 0;
@@ -79,8 +79,8 @@ __global__ __launch_bounds__(128) void q4_wide_prepare_kernel(const __grid_const
         if (i < all)
           *reinterpret_cast<uint4*>(step + (((gi * WL + in % WL) * NT + col / 8) * 32 + col % 8 * 4 + in / WL) * 16) = w;
       },
-      [&](int h, float4 f) {
-        if (i < all && in == 0) *reinterpret_cast<float4*>(step + C::COLS * 256 + (gi * C::COLS + m * P + h) * 16) = f;
+      [&](int h, float2 f) {
+        if (i < all && in == 0) *reinterpret_cast<float2*>(step + C::COLS * 256 + (gi * C::COLS + m * P + h) * 8) = f;
       });
 }
 
@@ -275,7 +275,7 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
       for (int half = 0; half < 2 / C::WK; ++half) {
         const int sub = C::WK > 1 ? wk : half;
         const uint32_t row = stage + sub * kBoxBytes + (wt * 16 + g) * (kStep / 2), xa = stage + C::kX + sub * C::kXStep + lane * 16;
-        const uint32_t fa = stage + C::kX + sub * C::kXStep + COLS * 256 + 2 * c * 16;
+        const uint32_t fa = stage + C::kX + sub * C::kXStep + COLS * 256 + 2 * c * 8;
         const uint32_t sa = stage + C::kScales + (sub * GS * kBlock + wt * 16 + g) * 2 * (int)sizeof(T);
 #pragma unroll
         for (int gi = 0; gi < GS; ++gi) {
@@ -309,7 +309,7 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[j][e] += acd[j][e];
             }
-            add_group<P>(y[j], acc[j], lds128(fa + (gi * COLS + j * 8) * 16), lds128(fa + (gi * COLS + j * 8) * 16 + 16), s0, b0, s1, b1);
+            add_group<P>(y[j], acc[j], lds128(fa + (gi * COLS + j * 8) * 8), s0, b0, s1, b1);
           }
         }
       }

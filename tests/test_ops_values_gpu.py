@@ -123,3 +123,15 @@ def test_q4_values_of_one_sign_lean_to_no_side(ops, dtype, out, m, n, k, group):
     rms = float(want.square().mean().sqrt())
     lean = float((y.cpu().double() - want).mean())
     assert abs(lean) <= 6 * half_step(out) / math.sqrt(3 * m * n) * rms + group / 16 * 2.0**-23 * float(size.mean()) + 2.0**-22 * rms
+
+
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("m", [1, 4, 8, 33])
+@pytest.mark.parametrize("value,size", [(1e36, 1), (2e38, 1), (2e37, 128)])
+def test_q4_large_finite_values(ops, dtype, out, m, value, size):
+    """x near the largest number of its type, one value of a group or all of
+    them: results that are finite come out finite."""
+    x, packed, scales, biases = q4_case(m, dtype, m, 50, 384, 128)
+    x[m // 2, 128:128 + size] = value
+    y = check_q4(ops, x, packed, scales, biases, out_dtype=out)
+    assert bool(torch.isfinite(y).all())
