@@ -147,6 +147,8 @@ def q4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, biase
 def q4_quantize(w: torch.Tensor, group: int = 64) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(packed, scales, biases) of float32 or bfloat16 weights (n, k), as
     q4_linear takes them (mrtdf_q4_quantize)."""
+    if w.requires_grad and torch.is_grad_enabled():
+        _invalid("w requires a gradient, which the operators do not give")
     if w.dim() != 2 or w.stride(1) != 1:
         _invalid("w must be (n, k) with contiguous rows")
     n, k = w.shape
