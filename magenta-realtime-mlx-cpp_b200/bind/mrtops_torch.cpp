@@ -13,6 +13,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -52,6 +53,8 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
 void no_gradient(const at::Tensor& t, const char* name) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     invalid(std::string(name) + " requires a gradient, which the operators do not give");
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    invalid(std::string(name) + " has a forward-mode tangent, which the operators do not carry on");
 }
 
 int dtype_of(const at::Tensor& t, const char* name) {

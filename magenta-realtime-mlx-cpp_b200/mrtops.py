@@ -13,7 +13,8 @@ device and returns without waiting; it may be captured into a CUDA graph.
 Outputs that are not given are new tensors, workspaces come from torch's
 allocator per call, so calls on several streams do not share any. float32 and
 bfloat16; the operators have no gradients (an input that requires one is
-refused while gradients are on). Errors raise ``mrtdf.MrtdfError``.
+refused while gradients are on, one with a forward-mode tangent while those
+are). Errors raise ``mrtdf.MrtdfError``.
 """
 from __future__ import annotations
 
@@ -149,6 +150,8 @@ def q4_quantize(w: torch.Tensor, group: int = 64) -> Tuple[torch.Tensor, torch.T
     q4_linear takes them (mrtdf_q4_quantize)."""
     if w.requires_grad and torch.is_grad_enabled():
         _invalid("w requires a gradient, which the operators do not give")
+    if torch.autograd.forward_ad.unpack_dual(w).tangent is not None:
+        _invalid("w has a forward-mode tangent, which the operators do not carry on")
     if w.dim() != 2 or w.stride(1) != 1:
         _invalid("w must be (n, k) with contiguous rows")
     n, k = w.shape
