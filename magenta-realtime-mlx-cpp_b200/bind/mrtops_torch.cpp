@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/mrtdf.h"
@@ -55,6 +56,13 @@ void no_gradient(const at::Tensor& t, const char* name) {
     invalid(std::string(name) + " requires a gradient, which the operators do not give");
   if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
     invalid(std::string(name) + " has a forward-mode tangent, which the operators do not carry on");
+}
+
+// What a call has written counts as modified in place: a backward pass that saved
+// it before reports that instead of using the new values.
+void written(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 int dtype_of(const at::Tensor& t, const char* name) {
@@ -265,6 +273,8 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       t.workspace_bytes = ws.nbytes();
     }
     check(mrtdf_tree_attention(&c, &t, stream_of(d)));
+    written({&out, &lse});
+    if (ws.defined()) written({&ws});
     return pair(a[11] == Py_None ? wrap(out) : given(a[11]), a[12] == Py_None ? wrap(lse) : given(a[12]));
   });
 }
@@ -315,6 +325,7 @@ PyObject* cache_mass(PyObject*, PyObject* const* a, Py_ssize_t n) {
     m.scale = number(a[7], "scale");
     m.decay = number(a[11], "decay");
     check(mrtdf_cache_mass(&c, &m, stream_of(d)));
+    written({&tensor(to, "mass_out")});
     return given(to);
   });
 }
@@ -347,6 +358,9 @@ PyObject* cache_commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
     m.nodes = small(nodes, "nodes");
     m.path_len = small(path.size(1), "path_len");
     check(mrtdf_cache_commit(&c, &m, stream_of(d)));
+    written({&k, &v, &lens});
+    if (positions) written({&next});
+    if (a[6] != Py_None) written({&tensor(a[6], "pos")});
     return pair(a[8] == Py_None ? wrap(lens) : given(a[8]),
                 a[9] != Py_None || !positions ? given(a[9]) : wrap(next));
   });
@@ -364,14 +378,16 @@ PyObject* cache_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     mrtdf_evict_args m{};
     m.struct_bytes = sizeof(m);
     m.mass = flat<float>(tensor(a[3], "mass"), shape, at::kFloat, d, "mass");
-    m.mass_out = flat<float>(tensor(a[9] == Py_None ? a[3] : a[9], "mass_out"), shape, at::kFloat, d, "mass_out");
-    m.pos_out = flat<int32_t>(tensor(a[10] == Py_None ? a[4] : a[10], "pos_out"), shape, at::kInt, d, "pos_out");
+    const at::Tensor &mass_out = tensor(a[9] == Py_None ? a[3] : a[9], "mass_out"), &pos_out = tensor(a[10] == Py_None ? a[4] : a[10], "pos_out");
+    m.mass_out = flat<float>(mass_out, shape, at::kFloat, d, "mass_out");
+    m.pos_out = flat<int32_t>(pos_out, shape, at::kInt, d, "pos_out");
     at::Tensor lens = a[11] == Py_None ? fresh(one, at::kInt, d) : tensor(a[11], "lens_out");
     m.lens_out = flat<int32_t>(lens, one, at::kInt, d, "lens_out");
     m.budget = whole(a[6], "budget");
     m.recent = whole(a[7], "recent");
     m.sinks = whole(a[8], "sinks");
     check(mrtdf_cache_evict(&c, &m, stream_of(d)));
+    written({&k, &v, &mass_out, &pos_out, &lens});
     return a[11] == Py_None ? wrap(lens) : given(a[11]);
   });
 }
@@ -419,6 +435,7 @@ PyObject* q4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
       m.workspace_bytes = need;
     }
     check(mrtdf_q4_linear(&m, stream_of(d)));
+    written({&out});
     return a[4] == Py_None ? wrap(out) : given(a[4]);
   });
 }
