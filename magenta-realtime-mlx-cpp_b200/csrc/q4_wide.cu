@@ -365,11 +365,13 @@ template <typename T, typename O, int G, int NT>
 __global__ __launch_bounds__(256) void q4_wide_join_kernel(const __grid_constant__ Q4Params p, const __grid_constant__ Runs q) {
   using C = Wide<T, G, NT>;
   const int c = blockIdx.x + 1, u = q.start(c), item = u / q.pairs, first = item * q.pairs;
-  if (u == first || q.start(c - 1) > first) return;
+  const bool joins = u != first && q.start(c - 1) <= first;
   const int last = q.owner(first + q.pairs - 1), m0 = item % q.passes * q.rows, n0 = item / q.passes * kBlock;
   const int m = blockIdx.y * 2 + (threadIdx.x >> 7), r = threadIdx.x & 127;
+  // Every CTA waits, those without work too: the join is done when the products
+  // are, and so what comes next on the stream may use them.
   pdl_wait();
-  if (m >= q.rows || m0 + m >= p.m || n0 + r >= p.n) return;
+  if (!joins || m >= q.rows || m0 + m >= p.m || n0 + r >= p.n) return;
   const float* part = reinterpret_cast<const float*>(static_cast<const uint8_t*>(p.ws) + q.passes * C::x_bytes(q.pairs)) + m * kBlock + r;
   float sum = 0.f;
   for (int o = c - 1; o <= last; ++o) sum += part[((int64_t)o * 2 + (o == c - 1 && q.start(o) != first)) * C::ROWS * kBlock];
@@ -416,7 +418,8 @@ cudaError_t wide_run(const Q4Params& p, int sms, size_t* ws_bytes, cudaStream_t 
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, K, map, p, q);
-  if (e != cudaSuccess || q.grid == 1 || (q.total % q.grid == 0 && q.total / q.grid % q.pairs == 0)) return e;
+  // A row block is one CTA's alone where runs end with it.
+  if (e != cudaSuccess || q.grid == 1 || q.pairs == 1 || (q.total % q.grid == 0 && q.total / q.grid % q.pairs == 0)) return e;
   cfg.gridDim = dim3(q.grid - 1, (q.rows + 1) / 2);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;

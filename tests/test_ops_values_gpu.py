@@ -135,3 +135,19 @@ def test_q4_large_finite_values(ops, dtype, out, m, value, size):
     x[m // 2, 128:128 + size] = value
     y = check_q4(ops, x, packed, scales, biases, out_dtype=out)
     assert bool(torch.isfinite(y).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,n,k,group", [(64, 1 << 17, 256, 32), (33, 100000, 128, 64), (64, 1 << 17, 512, 32)])
+def test_q4_is_done_when_the_next_kernel_starts(ops, dtype, m, n, k, group):
+    """The stream goes on when the result is whole, also where no row block is
+    shared and nothing is joined (k up to 256)."""
+    x, packed, scales, biases = q4_case(m, dtype, m, n, k, group)
+    want = ops.q4_linear(x, packed, scales, biases, out_dtype=F32)
+    torch.cuda.synchronize()
+    out = torch.empty(m, n, device=DEV)
+    for _ in range(20):
+        out.fill_(math.nan)
+        ops.q4_linear(x, packed, scales, biases, out=out)
+        assert not int(out.isnan().sum())
+    assert torch.equal(out, want)
