@@ -413,8 +413,9 @@ int mrtdf_resolve_inference_bundle(const char* cache_root, const char* tag, mrtd
  * between calls and may be captured into a CUDA graph; calls on different
  * streams or from different threads may overlap as long as no buffer that one
  * of them writes (workspaces included) is used by another. What a call writes
- * overlaps nothing that it reads, except where an operator says so (drafted rows
- * are not views of the cache's own rows; the same address is refused). The caller's
+ * overlaps nothing else that it reads or writes, except where an operator says so
+ * (drafted rows are not views of the cache's own rows; buffers of the same address
+ * are refused). The caller's
  * current device is as before when a call returns. Nothing on the host sees
  * the values in device memory: what a kernel does with a length, a parent, a
  * path or a position that makes no sense is said with each operator, and none

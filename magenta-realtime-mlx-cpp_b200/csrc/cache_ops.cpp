@@ -2,6 +2,7 @@
 // "operators"): argument checks, the device switch and the launches. Nothing
 // here allocates, synchronises or reads device memory.
 #include <atomic>
+#include <initializer_list>
 #include <string>
 
 #include "cache_ops.cuh"
@@ -126,6 +127,12 @@ void apart(const CacheView& c, const char* op) {
   apart({{c.sl, c.layers}, {c.sb, c.batch}, {c.sh, c.kv_heads}, {c.st, c.capacity}}, op, "the cache");
 }
 
+// A buffer that is written is none of the others of the call (NULL ones aside).
+void own_buffer(const void* written, std::initializer_list<const void*> others, const char* op, const char* what) {
+  for (const void* o : others)
+    if (written && written == o) invalid(std::string(op) + ": " + what + " must be another buffer than the other operands");
+}
+
 // Addresses of elements of `esize` bytes.
 void check_element(const void* p, int esize, const char* op, const char* what) {
   if (reinterpret_cast<uintptr_t>(p) % esize) invalid(std::string(op) + ": " + what + " is not aligned to its elements");
@@ -165,8 +172,11 @@ TreeParams tree_params(const mrtdf_cache* cache, const mrtdf_tree_args* a, const
   p.v_new = rows_view(a->v_new, 1, b, kv, n, es, op, "v_new");
   p.out = rows_view(a->out, 1, b, a->heads, n, es, op, "out");
   apart({{p.out.sb, b}, {p.out.sh, a->heads}, {p.out.sn, n}}, op, "out");
-  if (p.out.ptr == p.q.ptr || p.out.ptr == p.k_new.ptr || p.out.ptr == p.v_new.ptr || p.out.ptr == p.c.k || p.out.ptr == p.c.v)
-    invalid(std::string(op) + ": out must be another buffer than the inputs");
+  const std::initializer_list<const void*> read = {p.q.ptr, p.k_new.ptr, p.v_new.ptr, p.c.k, p.c.v, p.c.lens, p.c.pos, p.c.next_pos,
+                                                    a->parents, a->rel_bias};
+  own_buffer(p.out.ptr, read, op, "out");
+  own_buffer(a->lse, read, op, "lse");
+  own_buffer(a->lse, {p.out.ptr}, op, "lse");
   p.lse = a->lse;
   p.parents = a->parents;
   p.rel_bias = a->rel_bias;
@@ -189,7 +199,7 @@ Q4Params q4_params(const mrtdf_q4_args* a, const char* op) {
   if (!a->x || !a->packed || !a->scales || !a->biases || !a->out) invalid("q4_linear: NULL argument");
   if (!aligned16(a->x) || !aligned16(a->packed)) invalid("q4_linear: x and packed must be 16-byte aligned");
   if (a->device < 0) invalid("q4_linear: device is negative");
-  if (a->out == a->x) invalid(std::string(op) + ": out must be another buffer than x");
+  own_buffer(a->out, {a->x, a->packed, a->scales, a->biases}, op, "out");
   check_element(a->scales, es, op, "scales");
   check_element(a->biases, es, op, "biases");
   check_element(a->out, a->out_dtype == MRTDF_DTYPE_FP32 ? 4 : 2, op, "out");
@@ -280,6 +290,7 @@ int mrtdf_cache_mass(const mrtdf_cache* cache, const mrtdf_mass_args* a, void* s
     const int es = dtype_bytes(p.c.dtype, op), l = p.c.layers, b = p.c.batch;
     p.q = rows_view(a->q, l, b, a->heads, a->nodes, es, op, "q");
     p.k_new = rows_view(a->k_new, l, b, p.c.kv_heads, a->nodes, es, op, "k_new");
+    own_buffer(a->mass_out, {p.q.ptr, p.k_new.ptr, p.c.k, p.c.lens, p.c.pos, p.c.next_pos, a->lse, a->path, a->rel_bias}, op, "mass_out");
     p.lse = a->lse;
     p.path = a->path;
     p.rel_bias = a->rel_bias;
@@ -307,8 +318,6 @@ int mrtdf_cache_commit(const mrtdf_cache* cache, const mrtdf_commit_args* a, voi
     if (a->nodes > kOpMaxNodes) out_of_range("cache_commit: at most 64 nodes");
     if (a->path_len < 1 || a->path_len > a->nodes) invalid("cache_commit: path_len must be 1 .. nodes");
     if (!a->path || !a->lens_out) invalid("cache_commit: path and lens_out must not be NULL");
-    if (a->lens_out == p.c.lens || (a->next_pos_out && a->next_pos_out == p.c.next_pos))
-      invalid("cache_commit: lens_out and next_pos_out must be other buffers than lens and next_pos");
     if (a->next_pos_out && !p.c.next_pos) invalid("cache_commit: next_pos_out needs cache.next_pos");
     const int es = dtype_bytes(p.c.dtype, op), l = p.c.layers, b = p.c.batch, kv = p.c.kv_heads;
     if ((int64_t)l * kv * a->path_len >= (int64_t)1 << 26) out_of_range("cache_commit: too many rows");
@@ -317,6 +326,11 @@ int mrtdf_cache_commit(const mrtdf_cache* cache, const mrtdf_commit_args* a, voi
     p.v_new = rows_view(a->v_new, l, b, kv, a->nodes, es, op, "v_new");
     if (p.k_new.ptr == p.c.k || p.k_new.ptr == p.c.v || p.v_new.ptr == p.c.v || p.v_new.ptr == p.c.k)
       invalid("cache_commit: the new rows must be another buffer than the cache");
+    const std::initializer_list<const void*> read = {p.c.lens, p.c.next_pos, p.c.pos, a->path, p.c.k, p.c.v, p.k_new.ptr, p.v_new.ptr};
+    own_buffer(a->lens_out, read, op, "lens_out");
+    own_buffer(a->next_pos_out, read, op, "next_pos_out");
+    own_buffer(a->next_pos_out, {a->lens_out}, op, "next_pos_out");
+    own_buffer(p.c.pos, {p.c.lens, p.c.next_pos, a->path}, op, "pos");
     p.path = a->path;
     p.lens_out = a->lens_out;
     p.next_pos_out = a->next_pos_out;
@@ -343,7 +357,9 @@ int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* a, void*
     if (a->recent < 0 || a->sinks < 0 || (int64_t)a->recent + a->sinks > a->budget)
       invalid("cache_evict: recent and sinks must be >= 0 and fit into the budget together");
     apart(p.c, op);
-    if (a->lens_out == p.c.lens) invalid("cache_evict: lens_out must be another buffer than lens");
+    own_buffer(a->lens_out, {p.c.lens, p.c.next_pos, p.c.pos, p.c.k, p.c.v, a->mass, a->mass_out, a->pos_out}, op, "lens_out");
+    own_buffer(a->mass_out, {p.c.lens, p.c.next_pos, p.c.pos, p.c.k, p.c.v}, op, "mass_out");
+    own_buffer(a->pos_out, {p.c.lens, p.c.next_pos, p.c.k, p.c.v, a->mass, a->mass_out}, op, "pos_out");
     p.mass = a->mass;
     p.mass_out = a->mass_out;
     p.pos_out = a->pos_out;
@@ -388,6 +404,9 @@ int mrtdf_q4_quantize(const mrtdf_q4_pack_args* a, void* stream) {
     check_element(a->w, es, op, "w");
     check_element(a->scales, es, op, "scales");
     check_element(a->biases, es, op, "biases");
+    own_buffer(a->packed, {a->w, a->scales, a->biases}, op, "packed");
+    own_buffer(a->scales, {a->w, a->biases}, op, "scales");
+    own_buffer(a->biases, {a->w}, op, "biases");
     Q4PackParams p{};
     p.w = a->w;
     p.packed = static_cast<uint8_t*>(a->packed);
