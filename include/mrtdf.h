@@ -481,7 +481,10 @@ int mrtdf_stream_cache(mrtdf_stream* st, int kind, int layer, mrtdf_cache* out, 
  * inputs below 2^127 in rows that are seen. The rows of an absent node, and of
  * a sequence that is passed over, are zeros with lse = -inf; so is a row whose
  * every score is -inf. Values in rows that a query row does not see do not
- * reach it, NaN and infinities included. No rounding but that of the result
+ * reach it, NaN and infinities included. A NaN score makes its row NaN. A NaN or
+ * an infinity among the values that a row sees stays in its column, which is then
+ * not finite (NaN also for an infinity, if it is a cached one: the weights meet it
+ * in parts of either sign). No rounding but that of the result
  * depends on how the work is split; results are the same from run to run.
  */
 typedef struct mrtdf_tree_args {

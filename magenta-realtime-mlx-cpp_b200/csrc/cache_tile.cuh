@@ -182,7 +182,8 @@ __device__ __forceinline__ void qk_tile(float (*s)[4], const QFrag<float, D>& q,
 
 // o[n][.] += p . value rows of the tile at `vals` (p in the layout of s).
 // bf16: p goes in as two bf16 parts, hi + lo, so that the weights keep 16
-// bits; the second product is free while the tile waits for memory.
+// bits; the second product is free while the tile waits for memory. An infinite
+// value meets parts of either sign or 0 and comes out as NaN.
 // HALF: rows g + 8 do not exist, their weights are taken as zero.
 template <int D, int NT, bool HALF>
 __device__ __forceinline__ void pv_tile(float (*o)[4], const float (*p)[4], uint32_t vals, int lane, __nv_bfloat16) {

@@ -151,3 +151,18 @@ def test_q4_is_done_when_the_next_kernel_starts(ops, dtype, m, n, k, group):
         ops.q4_linear(x, packed, scales, biases, out=out)
         assert not int(out.isnan().sum())
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype,D,H,KV,N", [(BF, 64, 2, 1, 3), (F32, 64, 2, 1, 3), (BF, 128, 16, 1, 8), (BF, 64, 16, 1, 8)])
+@pytest.mark.parametrize("cap", [200, 3000])
+def test_tree_infinite_values_that_rows_see_stay_in_their_columns(ops, dtype, D, H, KV, N, cap):
+    """Cached infinities and a NaN make their columns not finite, and nothing else."""
+    x = tree_inputs(6, dtype, 2, H, KV, N, D, cap)
+    lens = ints([cap, cap - 9])
+    wo, wl, to, tl = attend(*x, lens)
+    x[4][0, :, 5, 3], x[4][0, :, cap - 2, 9], x[4][0, :, 77, D - 1] = math.inf, -math.inf, math.nan
+    out, lse = ops.tree_attention(*x, lens)
+    near(lse, wl, tl)
+    assert not bool(torch.isfinite(out[0][..., [3, 9, D - 1]]).any())
+    out[0][..., [3, 9, D - 1]], wo[0][..., [3, 9, D - 1]] = 0.0, 0.0
+    near(out, wo, to)
