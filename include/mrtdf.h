@@ -484,8 +484,11 @@ int mrtdf_stream_cache(mrtdf_stream* st, int kind, int layer, mrtdf_cache* out, 
  * reach it, NaN and infinities included. A NaN score makes its row NaN. A NaN or
  * an infinity among the values that a row sees stays in its column, which is then
  * not finite (NaN also for an infinity, if it is a cached one: the weights meet it
- * in parts of either sign). No rounding but that of the result
- * depends on how the work is split; results are the same from run to run.
+ * in parts of either sign). Results are the same from run to run: the same call
+ * on the same device repeats bit for bit. How a long cache is cut over the GPU
+ * depends on the capacity, the device and the lengths of all sequences, so a
+ * sequence's float32 sums, and with them the last bits of out and lse, may
+ * differ when its neighbours do.
  */
 typedef struct mrtdf_tree_args {
   size_t struct_bytes;
@@ -592,8 +595,8 @@ int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* args, vo
  * k <= 2^17 a multiple of the group (32, 64 or 128), n <= 2^24; x's rows and
  * packed on 16-byte boundaries. A row of x with an infinity or a NaN gives
  * results that are not finite, and touches no other row. Finite x gives finite
- * results where x times the weights, summed, fits float32 (scales and biases
- * below 2^100).
+ * results where the sums of x times the weights, over the columns and over parts
+ * of them, fit float32 (scales and biases below 2^100).
  */
 typedef struct mrtdf_q4_args {
   size_t struct_bytes;

@@ -166,3 +166,36 @@ def test_tree_infinite_values_that_rows_see_stay_in_their_columns(ops, dtype, D,
     assert not bool(torch.isfinite(out[0][..., [3, 9, D - 1]]).any())
     out[0][..., [3, 9, D - 1]], wo[0][..., [3, 9, D - 1]] = 0.0, 0.0
     near(out, wo, to)
+
+
+@pytest.mark.parametrize("dtype,D,H,KV,N", TREES)
+def test_the_same_calls_repeat_bit_for_bit(ops, dtype, D, H, KV, N):
+    """Attention and collected weight over split items; beside other neighbours a
+    sequence's results stay within the tolerance."""
+    cap, B = 3000, 3
+    x = tree_inputs(7, dtype, B, H, KV, N, D, cap)
+    lens = ints([cap, 1700, 5])
+    out, lse = ops.tree_attention(*x, lens)
+    path, mass = ints([list(range(N))] * B), normal(8, B, KV, cap).abs()
+
+    def weight():
+        return ops.cache_mass(x[0], lse, x[1], x[3], lens, path, mass, mass_out=torch.zeros_like(mass))
+
+    first = weight()
+    for _ in range(5):
+        again = ops.tree_attention(*x, lens)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse) and torch.equal(weight(), first)
+    wo, wl, to, tl = attend(*(t[:1] for t in x), lens[:1])
+    for now in ([cap, 1700, 5], [cap, 0, 64], [cap, cap, cap]):
+        out, lse = ops.tree_attention(*x, ints(now))
+        near(out[:1], wo, to)
+        near(lse[:1], wl, tl)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m", [2, 8, 40])
+def test_the_same_products_repeat_bit_for_bit(ops, dtype, m):
+    x, packed, scales, biases = q4_case(m, dtype, m, 3333, 2048, 64)
+    first = ops.q4_linear(x, packed, scales, biases)
+    for _ in range(5):
+        assert torch.equal(ops.q4_linear(x, packed, scales, biases), first)
