@@ -592,21 +592,6 @@ __device__ __forceinline__ void q_from_smem(QFrag<float, D>& q, uint32_t base, i
     ldsm_x4_g(q.a[ks], base + Rows<float, D>::at((m & 1) * 8 + r, 2 * ks + (m >> 1)));
 }
 
-// Nodes of the accepted path: up to the first entry that is not a node after
-// the one before it, as many as fit into the cache. One warp.
-__device__ int path_nodes(const int32_t* path, int path_len, int nodes, int room, int lane) {
-  int n = 0;
-  for (int base = 0; base < path_len; base += 32) {
-    const int i = base + lane;
-    const int v = i < path_len ? path[i] : -1, before = i > 0 && i <= path_len ? path[i - 1] : -1;
-    const unsigned ok = __ballot_sync(0xffffffffu, v > before && v >= 0 && v < nodes);
-    const int run = ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
-    n += run;
-    if (run < 32) break;
-  }
-  return min(n, room);
-}
-
 // CTAs per SM, by shared memory (67 KB for bf16 rows of 128: three).
 template <typename T, int D>
 constexpr int mass_ctas() {
@@ -648,7 +633,7 @@ __global__ __launch_bounds__(kThreads, mass_ctas<T, D>()) void cache_mass_kernel
     const bool there = cur.len >= 0;
     __syncthreads();  // the item before is done with the path and the rows
     int count = 0;
-    if (there) count = path_nodes(p.path + b * p.path_len, p.path_len, p.nodes, p.c.capacity - len, lane);
+    if (there) count = accepted(p.path + b * p.path_len, p.path_len, p.nodes, p.c.capacity - len, lane);
     for (int i = tid; i < p.path_len; i += kThreads) path_s[i] = i < count ? p.path[b * p.path_len + i] : 0;
     const int rows = heads_per * count, next = p.c.next_pos ? p.c.next_pos[b] : len;
     const int64_t row_at = ((int64_t)(layer * batch + b) * p.c.kv_heads + kvh) * p.c.capacity;

@@ -1,29 +1,12 @@
 // Rows of a KV cache that move: commit of an accepted path, eviction by
 // collected weight. Both are bound by the rows they move (head_dim elements
 // of K and V, read once and written once) and by latency when there are few.
-#include "cache_ops.cuh"
-#include "common.cuh"
-#include "decode_device.cuh"
+#include "cache_sched.cuh"
 
 namespace mrtdf {
 namespace {
 
 constexpr int kMoveThreads = 256;
-
-// Nodes of the accepted path: up to the first entry that is not a node after
-// the one before it, as many as fit into the cache. One warp.
-__device__ int accepted(const int32_t* path, int path_len, int nodes, int room, int lane) {
-  int n = 0;
-  for (int base = 0; base < path_len; base += 32) {
-    const int i = base + lane;
-    const int v = i < path_len ? path[i] : -1, before = i > 0 && i <= path_len ? path[i - 1] : -1;
-    const unsigned ok = __ballot_sync(0xffffffffu, v > before && v >= 0 && v < nodes);
-    const int run = ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
-    n += run;
-    if (run < 32) break;
-  }
-  return min(n, room);
-}
 
 // K[len + j] = K_new[path[j]], V alike, pos[len + j] = next_pos + j for every
 // layer and kv head of sequence blockIdx.y. The accepted rows of all layers

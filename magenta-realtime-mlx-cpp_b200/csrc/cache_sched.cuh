@@ -1,7 +1,8 @@
 // How the attention over a cache is spread over the GPU, shared by its kernels
 // (cache_attn.cu, cache_attn_tc.cu): a list of key tiles of all (sequence, kv
 // head, row block) items, equal runs of it per CTA, the drafted tree's masks,
-// and the join of items that several CTAs worked on.
+// the accepted path (cache_move.cu reads it too), and the join of items that
+// several CTAs worked on.
 #pragma once
 
 #include "cache_ops.cuh"
@@ -150,6 +151,21 @@ __device__ inline void node_masks(unsigned long long* seen, const int32_t* paren
     seen[i] = there && i < nodes && up[h] == kRoot ? m[h] : 0ull;
   }
   __syncwarp();
+}
+
+// Nodes of the accepted path: up to the first entry that is not a node after
+// the one before it, as many as fit into the cache. One warp.
+__device__ inline int accepted(const int32_t* path, int path_len, int nodes, int room, int lane) {
+  int n = 0;
+  for (int base = 0; base < path_len; base += 32) {
+    const int i = base + lane;
+    const int v = i < path_len ? path[i] : -1, before = i > 0 && i <= path_len ? path[i - 1] : -1;
+    const unsigned ok = __ballot_sync(0xffffffffu, v > before && v >= 0 && v < nodes);
+    const int run = ok == 0xffffffffu ? 32 : __ffs(~ok) - 1;
+    n += run;
+    if (run < 32) break;
+  }
+  return min(n, room);
 }
 
 __device__ __forceinline__ void store2(__nv_bfloat16* p, float a, float b) {
