@@ -401,8 +401,11 @@ cudaError_t launch_q4_linear(const Q4Params& p, int dtype, int out_dtype, int sm
 }
 
 cudaError_t launch_q4_quantize(const Q4PackParams& p, int dtype, cudaStream_t s) {
-  const int64_t all = (int64_t)p.n * (p.k / p.group), want = (all + 7) / 8;
-  const unsigned grid = (unsigned)(want < 148 * 32 ? want : 148 * 32);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const int64_t all = (int64_t)p.n * (p.k / p.group), want = (all + 7) / 8, most = 32 * op_sm_count(dev);
+  const unsigned grid = (unsigned)(want < most ? want : most);
   if (dtype == 0) q4_quantize_kernel<float><<<grid, 256, 0, s>>>(p);
   else q4_quantize_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
   return cudaGetLastError();
