@@ -477,8 +477,9 @@ int mrtdf_stream_cache(mrtdf_stream* st, int kind, int layer, mrtdf_cache* out, 
  * reads kv head h / (heads / kv_heads)). One node and parents NULL is a plain
  * decode step; parents NULL with more nodes is a chain. 1 <= nodes <= 64,
  * nodes * heads / kv_heads <= 1024. Scores, softmax statistics and sums are
- * float32; float32 products use split tf32 operands (2^-23 relative), finite
- * inputs below 2^127 in rows that are seen. The rows of an absent node, and of
+ * float32; bf16 values meet weights of 16 bits (2^-17 relative; the result's own
+ * rounding is 2^-9); float32 products use split tf32 operands
+ * (2^-23 relative), finite inputs below 2^127 in rows that are seen. The rows of an absent node, and of
  * a sequence that is passed over, are zeros with lse = -inf; so is a row whose
  * every score is -inf. Values in rows that a query row does not see do not
  * reach it, NaN and infinities included. A NaN score makes its row NaN. A NaN or
@@ -591,7 +592,8 @@ int mrtdf_cache_evict(const mrtdf_cache* cache, const mrtdf_evict_args* args, vo
  * q[n][k] + biases[n][k / group]), q in 0 .. 15. packed[n][j] holds column 2 j
  * in its low half and 2 j + 1 in its high half. x, scales and biases are of
  * `dtype`; out is of out_dtype (float32 for float32 x). The weights are not
- * rounded: sums of x times whole numbers are scaled in float32. 1 <= m <= 64,
+ * rounded: sums of x times whole numbers are scaled in float32. x keeps all of a
+ * bf16's bits and 22 of a float32's, per group from the largest. 1 <= m <= 64,
  * k <= 2^17 a multiple of the group (32, 64 or 128), n <= 2^24; x's rows and
  * packed on 16-byte boundaries. A row of x with an infinity or a NaN gives
  * results that are not finite, and touches no other row. Finite x gives finite

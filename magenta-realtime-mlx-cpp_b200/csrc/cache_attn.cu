@@ -23,9 +23,9 @@
 //   2 x 16 heads of 64, 16 nodes, 50 rows: 7.3. Latency: of the kernel's 6.3 us
 //     the schedule takes 0.7, finding the run and asking for its first keys 1.3,
 //     the queries 1.3, a tile 1 to 2 and the groups' join 0.5;
-//   2 x 16 heads of 64, 8 nodes, 700 to 1006 rows, float32, 14 MB: 15.6, of which
+//   2 x 16 heads of 64, 8 nodes, 700 to 1006 rows, float32, 14 MB: 15.2, of which
 //     the join of the split items is 3;
-//   21 x 4 heads of 128, one token, 1334 rows, float32, 115 MB: 51 (2.2 TB/s:
+//   21 x 4 heads of 128, one token, 1334 rows, float32, 115 MB: 52 (2.2 TB/s:
 //     bound by issue, a float32 product is three of tf32 and the splitting).
 #include "cache_sched.cuh"
 
@@ -61,7 +61,7 @@ __device__ __forceinline__ float2 val2(uint32_t vals, int row, int n, int c, flo
 // stages leave room for one CTA, whose four warps issue 1.1 instructions a
 // clock. So the ring holds three halves there, the keys of a tile or its values,
 // and the groups' sums are joined one after another: two CTAs fit (21 sequences
-// x 4 heads x 1334 keys: 67 us with one, 51 with two).
+// x 4 heads x 1334 keys: 67 us with one, 52 with two).
 template <typename T, int D>
 constexpr bool halves() {
   return sizeof(T) * D == 512;
@@ -561,8 +561,8 @@ __global__ __launch_bounds__(kThreads, tree_ctas<T, D, BIAS>()) void tree_attn_k
 // 2 layers x 8 sequences x 8 kv heads x 3001 to 8190 rows of 128, bf16, five
 // nodes of four heads each: 41 us for 190 MB (4.7 TB/s; the exponentials of 32
 // padded rows, of which 20 count, go beside the keys; with the weights so far
-// asked for in the tile that adds to them, 50 us); 2 x 16 heads of 64 over 250 rows,
-// float32: 6.6 us, latency.
+// asked for in the tile that adds to them, 50 us); with a bias and stored positions
+// 57; 2 x 16 heads of 64 over 250 rows, float32: 6.9 us, latency.
 constexpr int kMassRows = 64;  // query rows held in shared memory at a time
 
 // Rows of 512 bytes: two stages, so that two CTAs fit an SM.
@@ -821,7 +821,7 @@ cudaError_t tree_variant(const TreeParams& p, int wm, cudaStream_t s) {
 
 // Warps that share a key range: one per 16 query rows, up to four. float32: up
 // to two, since each takes all the keys apart for its products (96 rows of 128
-// x 1334 keys, 21 sequences of 4 heads: 381 us with four, 225 with two).
+// x 1334 keys, 21 sequences of 4 heads: 381 us with four, 220 with two).
 int tree_wm(const TreeParams& p) {
   const int rows = p.heads / p.c.kv_heads * p.nodes;
   return rows <= 16 ? 1 : rows <= 32 || p.c.dtype == 0 ? 2 : 4;
@@ -850,7 +850,9 @@ constexpr int kSmSmem = 227 * 1024;
 //  128 x  1024     22.0/ 26.8   30.2/ 28.2    44.0/ 31.7   75.0/ 43.9
 //  128 x  4096     47.3/ 47.9   67.8/ 51.8     116/ 56      217/ 85
 //  128 x 16384      139/ 112     207/ 125      396/ 131     773/ 239
-// (256 kv heads alike; head_dim 64 and 64 rows even out there.)
+// (256 kv heads alike; head_dim 64 and 64 rows even out there.) The rule goes by
+// capacity, since lengths are not known on the host: a long buffer that is mostly
+// empty is priced as a full one.
 bool tree_uses_tc(const TreeParams& p, int rows) {
   const int cap = p.c.capacity;
   if (rows > 64) return cap > 512;

@@ -33,7 +33,7 @@
 // from global memory at the end.
 //
 // Measured on a B200, us in a graph: 4 sequences x 8 kv heads of 128, 24 nodes of
-// four heads each (96 rows), 4097 to 16360 rows, 169 MB: 65 (2.6 TB/s, 270
+// four heads each (96 rows), 4097 to 16360 rows, 169 MB: 64 (2.6 TB/s, 275
 // TFLOP/s of real rows). A tile of 64 keys takes 0.95 us per SM, 0.75 of it its
 // products (two for the weights, since they keep 16 bits); the run's start (the
 // schedule and the queries to TMEM) 6, its end 4, the join of split items 3. With

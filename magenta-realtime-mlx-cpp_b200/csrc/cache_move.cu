@@ -12,9 +12,9 @@ constexpr int kMoveThreads = 256;
 // layer and kv head of sequence blockIdx.y. The accepted rows of all layers
 // are one flat list of 16-byte chunks, so a sequence's CTAs share it evenly
 // whatever its path length. Each thread has four K and four V loads in flight.
-// 20 layers x 2 x 16 heads of 64, bf16, five rows each: 4 us (one launch of
+// 20 layers x 2 x 16 heads of 64, bf16, five rows each: 4.1 us (one launch of
 // dependent loads: length, path, rows). 32 layers x 32 x 8 heads of 128, float32,
-// up to twelve rows: 22 us for 100 MB (4.6 TB/s, reads and writes).
+// up to twelve rows: 21 us for 100 MB (4.7 TB/s, reads and writes).
 template <int CH>  // 16-byte chunks per row
 __global__ __launch_bounds__(kMoveThreads) void cache_commit_kernel(const __grid_constant__ CommitParams p, int esize) {
   const int b = blockIdx.y, lane = threadIdx.x & 31;
@@ -72,8 +72,8 @@ __global__ __launch_bounds__(kMoveThreads) void cache_commit_kernel(const __grid
 // below the budget (a hole) takes the i-th kept slot at or above it. Holes are
 // below the budget and sources at or above it, so every row moves once, in
 // place, in any order.
-// 4 layers x 4 x 8 heads, 9000 to 16384 rows of 128 to 2048, bf16, 250 MB: 71 us
-// (3.5 TB/s): the passes 17, bitmap and lists 15, both bound by shared memory and
+// 4 layers x 4 x 8 heads, 9000 to 16384 rows of 128 to 2048, bf16, 250 MB: 72 us
+// (3.5 TB/s; float32, 485 MB: 115): the passes 17, bitmap and lists 15, both bound by shared memory and
 // barriers with one wave of clusters resident, the moves 30 at the memory's rate.
 // 2 x 16 heads, 50 rows to 40: 5.2 us, latency. 44 heads of up to 369: 9.9 us.
 constexpr int kEvictThreads = 256;

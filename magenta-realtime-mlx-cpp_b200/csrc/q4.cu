@@ -14,7 +14,7 @@
 // an offset of 1024 per weight goes through the products' sums and comes off
 // afterwards; the matrix instructions cut sums off towards zero, so x of one sign
 // (after a gated activation) then put every result 2.3e-4 of its size too low (16384
-// x 8192, 8 rows: 24.2 us, 22.8 with the offset).
+// x 8192: 8 rows 24.0 us, 22.8 with the offset; one row 21.6, 19.6 with it).
 // x is brought to fp16 by a power of two per row and group that puts the
 // group's largest |x| into [2^14, 2^15): bf16 x keeps all its bits (smaller
 // ones down to 2^-31 of the largest), float32 x becomes two columns, x = hi + lo
@@ -369,10 +369,12 @@ cudaError_t q4_launch(const Q4Params& p, const Q4Plan& q, cudaStream_t s) {
 // shared memory; otherwise the one that streams everything. Microseconds, bf16,
 // group 128, this kernel and the other:
 //   rows of x        1           4           8
-//   1024 x 1024      4.6  6.1    6.0  6.2    7.4  6.1
-//   4096 x 4096      7.8  8.7    8.9  8.9    (streams)
-//   16388 x 1024     6.6  8.2    7.2  8.7    7.8  8.9
-//   16384 x 8192    19.4 21.2    (streams)
+//   1024 x 1024      4.2  6.2    5.7  6.3    7.3  6.2
+//   4096 x 4096      7.6  9.0    8.7  9.4    (does not fit)
+//   16388 x 1024     6.4  8.4    7.2  8.9    7.7  9.2
+//   16384 x 8192    21.6 23.1   23.5 23.6   26.2 23.7
+// (a word per thread decides: 4 rows of 4096 and 8 rows of 16388 x 1024 would
+// gain 7 and 17 %, 8 rows of the other sizes lose as much).
 template <typename T, typename O, int G>
 cudaError_t q4_run(const Q4Params& p, int dtype, int out_dtype, int sms, size_t* ws_bytes, cudaStream_t s) {
   const Q4Plan q = q4_plan(p, sms);

@@ -16,9 +16,9 @@
 // it: for eight columns the chain of a warp's step (load, unpack, product,
 // scale), twice the weights' time over HBM; from 32 on the products themselves
 // (mma.sync) and then, with small groups, the scaling. Microseconds of the
-// whole call, bf16, 16384 x 8192, rows of x 8, 16, 32, 64, groups of 128: 22.3,
-// 28.7, 42.5, 76.2 (weights alone 10.9); groups of 32: 29.5, 41.6, 69.1, 126.9.
-// With the rows of x resident instead, in as many chunks as the shared memory
+// whole call, bf16, 16384 x 8192, rows of x 8, 16, 32, 64, groups of 128: 23.7,
+// 30.3, 43.1, 74.4 (weights alone 10.9); groups of 32: 30.0, 42.1, 59.3, 102.9;
+// float32, groups of 128: 29.0, 38.0, 62.6, 114.6. With the rows of x resident instead, in as many chunks as the shared memory
 // asked for, groups of 128 took 21.8, 35.6, 77.6, 153, groups of 32 143 to 614.
 #include "q4_tile.cuh"
 #include "tcgen05.cuh"
