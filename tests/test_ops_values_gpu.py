@@ -9,7 +9,8 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from test_ops_gpu import (  # noqa: E402,F401
-    BF, DEV, F32, attend, check_q4, collected, half_step, ints, near, normal, ops, q4_case, tree_inputs, unpack)
+    BF, DEV, F32, attend, check_q4, check_tree, collected, half_step, ints, near, normal, ops, q4_case, tree_inputs,
+    unpack)
 
 pytestmark = pytest.mark.gpu
 
@@ -199,3 +200,29 @@ def test_the_same_products_repeat_bit_for_bit(ops, dtype, m):
     first = ops.q4_linear(x, packed, scales, biases)
     for _ in range(5):
         assert torch.equal(ops.q4_linear(x, packed, scales, biases), first)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("step", [8, 72, 64])
+def test_tree_over_rows_that_share_memory(ops, dtype, D, step):
+    """Read-only rows may overlap: a sliding window over one buffer."""
+    B, H, KV, N, cap = 1, 16, 2, 8, 1500
+    q, kn, vn, _, _ = tree_inputs(1, dtype, B, H, KV, N, D, 8)
+    buf = normal(2, cap * step + 4 * D, dtype=dtype)
+    k = buf.as_strided((B, KV, cap, D), (0, 16, step, 1))
+    v = buf.flip(0).contiguous().as_strided((B, KV, cap, D), (0, 16, step, 1))
+    check_tree(ops, (q, kn, vn, k, v), ints([cap - 3]), None)
+
+
+def test_mass_of_many_rows(ops):
+    """1024 query rows of one kv head: sixteen blocks, each onto the sums of the one
+    before."""
+    L, B, H, KV, N, D, cap = 1, 2, 16, 1, 64, 64, 200
+    q, k, kn = normal(1, L, B, H, N, D, dtype=BF, std=0.2), normal(2, L, B, KV, cap, D, dtype=BF), normal(3, L, B, KV, N, D, dtype=BF)
+    lse = normal(4, L, B, H, N) + 6
+    mass = normal(5, L, B, KV, cap).abs()
+    path = ints([list(range(64)), list(range(0, 64))])
+    want, tol = collected(q, lse, kn, k, ints([130, 190]), path, mass, torch.zeros_like(mass))
+    got = ops.cache_mass(q, lse, kn, k, ints([130, 190]), path, mass, mass_out=torch.zeros_like(mass))
+    near(got, want, tol)
