@@ -164,9 +164,12 @@ __global__ __launch_bounds__((Wide<T, G, NT>::kThreads), 1) void q4_wide_kernel(
     };
     const int head = min(u1, u0 + ST);
     int issued = head;  // stages [u0, issued)
-    // No copy may still be landing when the CTA exits.
+    // No copy may still be landing when the CTA exits. After an aborted wait a
+    // stage may lack its scales and never be full; its copies and the others' have
+    // landed by the end of one such wait.
     auto landed = [&] {
-      for (int u = max(u0, issued - ST); u < issued; ++u) mbar_wait_bounded(full + (u - u0) % ST, (u - u0) / ST & 1, nullptr);
+      for (int u = max(u0, issued - ST); u < issued; ++u)
+        if (!mbar_wait_bounded(full + (u - u0) % ST, (u - u0) / ST & 1, nullptr)) break;
     };
     At to_copy = begin();
     if (issues)
